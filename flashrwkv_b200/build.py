@@ -37,6 +37,7 @@ CUDA_SOURCES = [
     "tmix_elementwise.cu",
     "tmix_norm.cu",
     "tmix_train.cu",
+    "tmix_norm_train.cu",
     "tmix_linear.cu",
     "tmix_gemm_tma.cu",
     "wkv7_backward.cu",

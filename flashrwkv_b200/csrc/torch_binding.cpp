@@ -1926,6 +1926,77 @@ std::vector<torch::Tensor> pretrain_tmix_lnx_rkvres_xg_backward(torch::Tensor gr
   return {gx, gr, gk, gv, grk, gw, gb, gg};
 }
 
+// ---- block-level LayerNorm for training (x [...,C] bf16) --------------------------------------------------------------
+void check_norm_rows(const torch::Tensor& x) {
+  check_cuda_contiguous(x, "x");
+  TORCH_CHECK(x.scalar_type() == torch::kBFloat16, "x must be bfloat16");
+  TORCH_CHECK(x.dim() >= 2 && x.numel() > 0, "x must have non-empty shape [...,C]");
+}
+void check_norm_like(const torch::Tensor& t, const char* name, const torch::Tensor& x) {
+  check_cuda_contiguous(t, name);
+  TORCH_CHECK(t.scalar_type() == torch::kBFloat16 && t.device() == x.device() && t.sizes() == x.sizes(), name,
+              " must match x");
+}
+void check_norm_vector(const torch::Tensor& t, const char* name, const torch::Tensor& x) {
+  check_cuda_contiguous(t, name);
+  TORCH_CHECK(t.scalar_type() == torch::kBFloat16 && t.device() == x.device() && t.dim() == 1 &&
+                  t.size(0) == x.size(-1),
+              name, " must be bfloat16 [C] on x's device");
+}
+
+// returns {sum (x itself without a residual), normalised rows, mean, rstd}
+std::vector<torch::Tensor> pretrain_tmix_layer_norm_forward(torch::Tensor x, std::optional<torch::Tensor> residual,
+                                                            torch::Tensor weight, torch::Tensor bias, double eps) {
+  check_norm_rows(x);
+  if (residual.has_value()) check_norm_like(*residual, "residual", x);
+  check_norm_vector(weight, "weight", x);
+  check_norm_vector(bias, "bias", x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t channels = x.size(-1), rows = x.numel() / channels;
+  auto sum = residual.has_value() ? torch::empty_like(x) : x;
+  auto out = torch::empty_like(x);
+  auto stats = torch::empty({2, rows}, x.options().dtype(torch::kFloat32));
+  auto mean = stats.select(0, 0), rstd = stats.select(0, 1);
+  check_rc(frwkv_pretrain_layer_norm_forward(
+      x.data_ptr(), residual.has_value() ? residual->data_ptr() : nullptr, weight.data_ptr(), bias.data_ptr(),
+      residual.has_value() ? sum.data_ptr() : nullptr, out.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(),
+      rows, static_cast<int>(channels), static_cast<float>(eps), current_stream(x)));
+  return {sum, out, mean, rstd};
+}
+
+// returns {gradient of the normalised rows' source} or {that, gradient of weight, gradient of bias}
+std::vector<torch::Tensor> pretrain_tmix_layer_norm_backward(torch::Tensor grad_out,
+                                                             std::optional<torch::Tensor> grad_sum, torch::Tensor sum,
+                                                             torch::Tensor weight, torch::Tensor mean,
+                                                             torch::Tensor rstd, bool parameters) {
+  check_norm_rows(sum);
+  check_norm_like(grad_out, "grad_out", sum);
+  if (grad_sum.has_value()) check_norm_like(*grad_sum, "grad_sum", sum);
+  check_norm_vector(weight, "weight", sum);
+  const int64_t channels = sum.size(-1), rows = sum.numel() / channels;
+  for (const auto& t : {mean, rstd}) {
+    check_cuda_contiguous(t, "mean and rstd");
+    TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.numel() == rows && t.device() == sum.device(),
+                "mean and rstd must be float32 [rows] on x's device");
+  }
+  const c10::cuda::CUDAGuard guard(sum.device());
+  auto grad_x = torch::empty_like(sum);
+  torch::Tensor grad_weight, grad_bias, workspace;
+  if (parameters) {
+    grad_weight = torch::empty_like(weight);
+    grad_bias = torch::empty_like(weight);
+    workspace = torch::empty({frwkv_pretrain_layer_norm_workspace_floats(rows, static_cast<int>(channels))},
+                             sum.options().dtype(torch::kFloat32));
+  }
+  check_rc(frwkv_pretrain_layer_norm_backward(
+      grad_out.data_ptr(), grad_sum.has_value() ? grad_sum->data_ptr() : nullptr, sum.data_ptr(), weight.data_ptr(),
+      mean.data_ptr<float>(), rstd.data_ptr<float>(), grad_x.data_ptr(), parameters ? grad_weight.data_ptr() : nullptr,
+      parameters ? grad_bias.data_ptr() : nullptr, parameters ? workspace.data_ptr<float>() : nullptr,
+      parameters ? workspace.numel() : 0, rows, static_cast<int>(channels), current_stream(sum)));
+  if (!parameters) return {grad_x};
+  return {grad_x, grad_weight, grad_bias};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -2060,6 +2131,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pretrain_tmix_kk_pre_backward", &pretrain_tmix_kk_pre_backward);
   m.def("pretrain_tmix_lnx_rkvres_xg_forward", &pretrain_tmix_lnx_rkvres_xg_forward);
   m.def("pretrain_tmix_lnx_rkvres_xg_backward", &pretrain_tmix_lnx_rkvres_xg_backward);
+  m.def("pretrain_tmix_layer_norm_forward", &pretrain_tmix_layer_norm_forward, py::arg("x"), py::arg("residual"),
+        py::arg("weight"), py::arg("bias"), py::arg("eps"));
+  m.def("pretrain_tmix_layer_norm_backward", &pretrain_tmix_layer_norm_backward, py::arg("grad_out"),
+        py::arg("grad_sum"), py::arg("sum"), py::arg("weight"), py::arg("mean"), py::arg("rstd"),
+        py::arg("parameters"));
   m.def("recurrent_add_vec_forward_varlen", &recurrent_add_vec_forward_varlen, py::arg("x"), py::arg("vec"));
   m.def("tmix_act_forward", &tmix_act_forward, py::arg("x"), py::arg("act"));
   m.def("tmix_linear_runtime_layout", &linear_runtime_layout, py::arg("x"), py::arg("weight_kn"), py::arg("act") = 0,

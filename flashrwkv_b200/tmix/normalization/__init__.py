@@ -2,7 +2,7 @@
 
 Mirror of the reference's `flashrwkv2/tmix/normalization/__init__.py:31-90` (names, keyword-only parameters,
 returned tuples); fp16 as in the reference, bf16 in addition.  One kernel serves the four operators; statistics are
-taken in fp32 from the rounded sum, the tensor the caller gets back.
+taken in fp32 from the rounded sum, the tensor the caller gets back.  The training forms are in `pretrain.py`.
 """
 from __future__ import annotations
 
@@ -10,6 +10,7 @@ import torch
 
 from ..._ext import extension
 from .._checks import check_io
+from .pretrain import pretrain_tmix_add_layer_norm_bf16, pretrain_tmix_layer_norm_bf16
 
 
 def _check_rows(tensor, name, reference=None) -> None:
@@ -70,4 +71,6 @@ __all__ = [
     "infer_tmix_add_layer_norm_forward_varlen",
     "infer_tmix_add_last_layer_norm_forward_varlen",
     "infer_tmix_add_forward_varlen",
+    "pretrain_tmix_layer_norm_bf16",
+    "pretrain_tmix_add_layer_norm_bf16",
 ]

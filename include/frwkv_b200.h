@@ -582,6 +582,23 @@ int frwkv_pretrain_lnx_rkvres_xg_backward(const void* grad_out, const void* x, c
                                           long long rows, int channels, int head_size, int io_dtype,
                                           frwkv_stream_t stream);
 
+/*
+ * Block-level LayerNorm for training, optionally of a sum: s = x + residual (rounded to bf16, written to sum_out; with
+ * residual and sum_out NULL s is x), out = (s - mean) * rstd * weight + bias; mean and rstd fp32 [rows] of s (biased
+ * variance) are saved for the backward.  bf16 tensors, 16-byte aligned; channels a multiple of 8 up to 16384.
+ * Backward: grad_x is the gradient of s (x and residual share it); grad_sum (may be NULL) is the gradient that reaches s
+ * beside the norm; grad_weight and grad_bias (both or neither) are fixed-order fp32 sums over the rows.  The inference
+ * forms are frwkv_tmix_add_layer_norm_forward.
+ */
+int frwkv_pretrain_layer_norm_forward(const void* x, const void* residual, const void* weight, const void* bias,
+                                      void* sum_out, void* out, float* mean, float* rstd, long long rows, int channels,
+                                      float eps, frwkv_stream_t stream);
+long long frwkv_pretrain_layer_norm_workspace_floats(long long rows, int channels);
+int frwkv_pretrain_layer_norm_backward(const void* grad_out, const void* grad_sum, const void* sum, const void* weight,
+                                       const float* mean, const float* rstd, void* grad_x, void* grad_weight,
+                                       void* grad_bias, float* workspace, long long workspace_floats, long long rows,
+                                       int channels, frwkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
