@@ -8,10 +8,14 @@
 //
 // A row belongs to a group of T threads with V 16-byte pieces each, which stays in registers from its one read to its
 // one write: every tensor crosses HBM once, which is the bound of both passes (forward 2 or 4, backward 3 or 4 tensors
-// of rows x C).  A group is a warp up to 512 channels (no barrier at all), 2 to 16 warps above; small groups share a
-// CTA of 256 threads.  The backward pass walks a slab of rows per CTA, keeps the column sums of dw and db in registers
-// along the walk, requests the next row before it reduces the present one, and writes one fp32 partial per CTA;
-// sum_slabs_kernel adds the partials in a fixed order, so the parameter gradients are the same on every run.
+// of rows x C).  Groups of one warp need no barrier; small groups share a CTA of 256 threads.  Forward: four pieces per
+// thread (8192 x 4096 in 25 us; two pieces 33 us, for want of bytes under way; with residual 38 us, its bytes take 42 at
+// the rate of a plain copy).  Backward: two pieces per thread; a CTA walks a slab of rows, keeps the column sums of dw and
+// db in registers along the walk, requests the next row before it reduces the present one, does its arithmetic on fp32
+// pairs (the pass is bound by instruction issue as much as by bytes) and writes one fp32 partial per CTA;
+// sum_slabs_kernel adds the partials in a fixed order, so the parameter gradients are the same on every run.  8192 x 4096
+// in 39 us, with a second gradient into the sum 47 us, where the bytes take 31 and 42.  A ring of rows in shared memory in
+// place of the row in registers was slower (56 us): the bytes were not what it waited for.
 //
 // The reference has the inference forms only (flashrwkv2/tmix/normalization/__init__.py:31-90).
 
@@ -40,11 +44,9 @@ __device__ __forceinline__ uint4 load16(const bf16* row, int piece) {
   return __ldg(reinterpret_cast<const uint4*>(row) + piece);
 }
 
-__host__ __device__ constexpr int cta_threads(int T) { return T < 256 ? 256 : T; }
-
 // Sums over the T threads of a row's group.  `scratch` holds two float2 per warp; `turn` alternates so that one barrier
 // per call is enough (a slot is written again only after the barrier of the call in between).
-template <int T>
+template <int T, int kThreads>
 __device__ __forceinline__ float2 group_sum(float2 v, float2* scratch, int turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -52,7 +54,9 @@ __device__ __forceinline__ float2 group_sum(float2 v, float2* scratch, int turn)
     v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
   }
   if (T == 32) return v;
-  constexpr int kWarps = T / 32, kAllWarps = cta_threads(T) / 32;
+  static_assert(T % 32 == 0, "a group is whole warps: its barrier counts them");
+  constexpr int kWarps = T / 32, kAllWarps = kThreads / 32;
+  static_assert(kThreads / T < 16 || T == 32, "a barrier per group, and barrier 0 is the CTA's");
   const int warp = threadIdx.x >> 5, group = threadIdx.x / T;
   float2* slot = scratch + turn * kAllWarps;
   if ((threadIdx.x & 31) == 0) slot[warp] = v;
@@ -67,14 +71,16 @@ __device__ __forceinline__ float2 group_sum(float2 v, float2* scratch, int turn)
   return v;
 }
 
+__host__ __device__ constexpr int forward_threads(int T) { return T < 256 ? 256 : T; }
+
 template <int T, int V, bool kAdd>
-__global__ __launch_bounds__(cta_threads(T)) void norm_forward_kernel(
+__global__ __launch_bounds__(forward_threads(T)) void norm_forward_kernel(
     const bf16* __restrict__ x, const bf16* __restrict__ residual, const bf16* __restrict__ weight,
     const bf16* __restrict__ bias, bf16* __restrict__ sum_out, bf16* __restrict__ out, float* __restrict__ mean_out,
     float* __restrict__ rstd_out, long long rows, int channels, float eps) {
   chain_begin();
-  __shared__ float2 scratch[2 * (cta_threads(T) / 32)];
-  constexpr int kGroups = cta_threads(T) / T;
+  __shared__ float2 scratch[2 * (forward_threads(T) / 32)];
+  constexpr int kGroups = forward_threads(T) / T;
   const int lane = threadIdx.x % T, pieces = channels >> 3;
   const long long row = (long long)blockIdx.x * kGroups + threadIdx.x / T;
   if (row >= rows) return;  // whole groups leave: the barriers are per group
@@ -103,7 +109,7 @@ __global__ __launch_bounds__(cta_threads(T)) void norm_forward_kernel(
     for (int e = 0; e < 8; ++e) part.x += f[v][e];
   }
   const float inv = 1.f / (float)channels;
-  const float mean = group_sum<T>(part, scratch, 0).x * inv;
+  const float mean = group_sum<T, forward_threads(T)>(part, scratch, 0).x * inv;
   part.x = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -115,7 +121,7 @@ __global__ __launch_bounds__(cta_threads(T)) void norm_forward_kernel(
       }
     }
   }
-  const float rstd = rsqrtf(group_sum<T>(part, scratch, 1).x * inv + eps);
+  const float rstd = rsqrtf(group_sum<T, forward_threads(T)>(part, scratch, 1).x * inv + eps);
   if (lane == 0) {
     mean_out[row] = mean;
     rstd_out[row] = rstd;
@@ -134,26 +140,63 @@ __global__ __launch_bounds__(cta_threads(T)) void norm_forward_kernel(
   }
 }
 
+// ---- backward ------------------------------------------------------------------------------------------------------
+// fp32 pairs: fma.rn.f32x2 and its kin do two elements per issue slot, each rounded as the scalar instruction rounds
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_pairs(const uint4& u, f32x2 (&f)[4]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = IO::unpack(w[i]);
+    f[i] = pair(t.x, t.y);
+  }
+}
+
+__host__ __device__ constexpr int backward_threads(int T) { return T < 256 ? 256 : T; }
+
 // One row of the backward pass as it comes from memory.
 template <int V>
 struct RowPieces {
-  uint4 s[V], dy[V], ds[V];
+  uint4 s[V], dy[V];
   float mean, rstd;
 };
 
-template <int T, int V, bool kSum>
-__device__ __forceinline__ void load_row(RowPieces<V>& r, const bf16* s, const bf16* dy, const bf16* dsum,
-                                         const float* mean, const float* rstd, long long row, int channels, int lane) {
+template <int T, int V>
+__device__ __forceinline__ void load_row(RowPieces<V>& r, const bf16* s, const bf16* dy, const float* mean, const float* rstd, long long row, int channels, int lane) {
   const long long at = row * channels;
   const int pieces = channels >> 3;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int p = lane + v * T;
-    r.s[v] = r.dy[v] = r.ds[v] = make_uint4(0u, 0u, 0u, 0u);
+    r.s[v] = r.dy[v] = make_uint4(0u, 0u, 0u, 0u);
     if (p < pieces) {
       r.s[v] = load16(s + at, p);
       r.dy[v] = load16(dy + at, p);
-      if (kSum) r.ds[v] = load16(dsum + at, p);
     }
   }
   r.mean = __ldg(mean + row);
@@ -162,100 +205,106 @@ __device__ __forceinline__ void load_row(RowPieces<V>& r, const bf16* s, const b
 
 // kSum: a gradient reaches s beside the one through the norm.  kParams: dw and db are wanted.
 template <int T, int V, bool kSum, bool kParams>
-__global__ __launch_bounds__(cta_threads(T)) void norm_backward_kernel(
+__global__ __launch_bounds__(backward_threads(T), backward_threads(T) >= 512 ? 1 : 2) void norm_backward_kernel(
     const bf16* __restrict__ dy, const bf16* __restrict__ dsum, const bf16* __restrict__ s,
     const bf16* __restrict__ weight, const float* __restrict__ mean, const float* __restrict__ rstd,
     bf16* __restrict__ dx, bf16* __restrict__ dw, bf16* __restrict__ db, float* __restrict__ partials, long long rows,
     int channels, long long rows_per_cta) {
   chain_begin();
-  constexpr int kAllWarps = cta_threads(T) / 32, kGroups = cta_threads(T) / T;
-  constexpr bool kAhead = V <= 2;  // the next row's pieces fit the registers beside the column sums
+  constexpr int kThreads = backward_threads(T), kAllWarps = kThreads / 32, kGroups = kThreads / T;
   __shared__ float2 scratch[2 * kAllWarps];
   const int lane = threadIdx.x % T, group = threadIdx.x / T, pieces = channels >> 3;
   const long long begin = blockIdx.x * rows_per_cta;
   const long long end = begin + rows_per_cta < rows ? begin + rows_per_cta : rows;
   const float inv = 1.f / (float)channels;
-  float aw[V][8], ab[V][8];
+  f32x2 sw[V][4], sb[V][4];
+  uint4 w[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v)
+  for (int v = 0; v < V; ++v) {
+    w[v] = lane + v * T < pieces ? load16(weight, lane + v * T) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) aw[v][e] = ab[v][e] = 0.f;
+    for (int i = 0; i < 4; ++i) sw[v][i] = sb[v][i] = pair(0.f, 0.f);
+  }
   RowPieces<V> now;
   long long row = begin + group;
-  if (row < end) load_row<T, V, kSum>(now, s, dy, dsum, mean, rstd, row, channels, lane);
+  if (row < end) load_row<T, V>(now, s, dy, mean, rstd, row, channels, lane);
   for (int turn = 0; row < end; turn ^= 1) {
     const long long next_row = row + kGroups;
     RowPieces<V> next = now;
-    if (kAhead && next_row < end) load_row<T, V, kSum>(next, s, dy, dsum, mean, rstd, next_row, channels, lane);
-    float2 part = make_float2(0.f, 0.f);
+    if (next_row < end) load_row<T, V>(next, s, dy, mean, rstd, next_row, channels, lane);
+    uint4 ds[V];  // wanted after the sums only: it needs no row of lead
+    if (kSum) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (lane + v * T < pieces) ds[v] = load16(dsum + row * channels, lane + v * T);
+    }
+    f32x2 unit[V][4], hw[V][4], p1 = pair(0.f, 0.f), p2 = p1;
+    const f32x2 scale = pair(now.rstd, now.rstd), shift = pair(-now.mean * now.rstd, -now.mean * now.rstd);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float h[8], w[8], c[8];
-      unpack8(now.s[v], c);
-      unpack8(now.dy[v], h);
-      unpack8(lane + v * T < pieces ? load16(weight, lane + v * T) : make_uint4(0u, 0u, 0u, 0u), w);
+      f32x2 c[4], h[4], g[4];
+      unpack_pairs(now.s[v], c);
+      unpack_pairs(now.dy[v], h);
+      unpack_pairs(w[v], g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float unit = (c[e] - now.mean) * now.rstd;
+      for (int i = 0; i < 4; ++i) {
+        unit[v][i] = fma2(c[i], scale, shift);
         if (kParams) {
-          aw[v][e] = fmaf(h[e], unit, aw[v][e]);
-          ab[v][e] += h[e];
+          sw[v][i] = fma2(h[i], unit[v][i], sw[v][i]);
+          sb[v][i] = add2(sb[v][i], h[i]);
         }
-        const float hw = h[e] * w[e];
-        part.x += hw;
-        part.y = fmaf(hw, unit, part.y);
+        hw[v][i] = mul2(h[i], g[i]);
+        p1 = add2(p1, hw[v][i]);
+        p2 = fma2(hw[v][i], unit[v][i], p2);
       }
     }
-    const float2 total = group_sum<T>(part, scratch, turn);
-    const float m1 = total.x * inv, m2 = total.y * inv;
+    const float2 q1 = halves(p1), q2 = halves(p2);
+    const float2 total = group_sum<T, kThreads>(make_float2(q1.x + q1.y, q2.x + q2.y), scratch, turn);
+    // ds = rstd * hw - (rstd * mean(h)) - unit * (rstd * mean(h * xhat))
+    const float m1 = -now.rstd * total.x * inv, m2 = -now.rstd * total.y * inv;
+    const f32x2 n1 = pair(m1, m1), n2 = pair(m2, m2);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int p = lane + v * T;
       if (p < pieces) {
-        float h[8], w[8], c[8], d[8];
-        unpack8(now.s[v], c);
-        unpack8(now.dy[v], h);
-        unpack8(load16(weight, p), w);
-        if (kSum) unpack8(now.ds[v], d);
+        f32x2 d[4];
+        if (kSum) unpack_pairs(ds[v], d);
+        uint32_t out[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float unit = (c[e] - now.mean) * now.rstd;
-          const float g = now.rstd * (h[e] * w[e] - m1 - unit * m2);
-          c[e] = kSum ? g + d[e] : g;
+        for (int i = 0; i < 4; ++i) {
+          f32x2 g = fma2(hw[v][i], scale, fma2(unit[v][i], n2, n1));
+          if (kSum) g = add2(g, d[i]);
+          const float2 t = halves(g);
+          out[i] = IO::pack(t.x, t.y);
         }
-        reinterpret_cast<uint4*>(dx + row * channels)[p] = pack8(c);
+        reinterpret_cast<uint4*>(dx + row * channels)[p] = make_uint4(out[0], out[1], out[2], out[3]);
       }
     }
     row = next_row;
-    if (kAhead) {
-      now = next;
-    } else if (row < end) {
-      load_row<T, V, kSum>(now, s, dy, dsum, mean, rstd, row, channels, lane);
-    }
+    now = next;
   }
   if (!kParams) return;
   // the CTA's groups are added in their order, then one partial per CTA leaves (or, of a single CTA, the result)
   if (kGroups > 1) {
-    __shared__ float4 sums[kGroups > 1 ? (kGroups - 1) * T * 4 : 1];
+    __shared__ f32x2 sums[kGroups > 1 ? (kGroups - 1) * T * 8 : 1];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       __syncthreads();
       if (group > 0) {
-        float4* q = sums + (group - 1) * T * 4 + lane;
-        q[0 * T] = make_float4(aw[v][0], aw[v][1], aw[v][2], aw[v][3]);
-        q[1 * T] = make_float4(aw[v][4], aw[v][5], aw[v][6], aw[v][7]);
-        q[2 * T] = make_float4(ab[v][0], ab[v][1], ab[v][2], ab[v][3]);
-        q[3 * T] = make_float4(ab[v][4], ab[v][5], ab[v][6], ab[v][7]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sums[((group - 1) * 8 + i) * T + lane] = sw[v][i];
+          sums[((group - 1) * 8 + 4 + i) * T + lane] = sb[v][i];
+        }
       }
       __syncthreads();
       if (group == 0) {
         for (int g = 0; g < kGroups - 1; ++g) {
-          const float4* q = sums + g * T * 4 + lane;
-          const float4 a = q[0 * T], b = q[1 * T], c = q[2 * T], d = q[3 * T];
-          aw[v][0] += a.x; aw[v][1] += a.y; aw[v][2] += a.z; aw[v][3] += a.w;
-          aw[v][4] += b.x; aw[v][5] += b.y; aw[v][6] += b.z; aw[v][7] += b.w;
-          ab[v][0] += c.x; ab[v][1] += c.y; ab[v][2] += c.z; ab[v][3] += c.w;
-          ab[v][4] += d.x; ab[v][5] += d.y; ab[v][6] += d.z; ab[v][7] += d.w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sw[v][i] = add2(sw[v][i], sums[(g * 8 + i) * T + lane]);
+            sb[v][i] = add2(sb[v][i], sums[(g * 8 + 4 + i) * T + lane]);
+          }
         }
       }
     }
@@ -265,49 +314,111 @@ __global__ __launch_bounds__(cta_threads(T)) void norm_backward_kernel(
   for (int v = 0; v < V; ++v) {
     const int p = lane + v * T;
     if (p >= pieces) continue;
+    uint32_t ow[4], ob[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = halves(sw[v][i]), b = halves(sb[v][i]);
+      if (gridDim.x > 1) {
+        float* q = partials + (long long)blockIdx.x * 2 * channels + 8 * p + 2 * i;
+        *reinterpret_cast<float2*>(q) = a;
+        *reinterpret_cast<float2*>(q + channels) = b;
+      }
+      ow[i] = IO::pack(a.x, a.y);
+      ob[i] = IO::pack(b.x, b.y);
+    }
     if (gridDim.x == 1) {
-      reinterpret_cast<uint4*>(dw)[p] = pack8(aw[v]);
-      reinterpret_cast<uint4*>(db)[p] = pack8(ab[v]);
-    } else {
-      float4* q = reinterpret_cast<float4*>(partials + (long long)blockIdx.x * 2 * channels) + 2 * p;
-      q[0] = make_float4(aw[v][0], aw[v][1], aw[v][2], aw[v][3]);
-      q[1] = make_float4(aw[v][4], aw[v][5], aw[v][6], aw[v][7]);
-      q += channels / 4;
-      q[0] = make_float4(ab[v][0], ab[v][1], ab[v][2], ab[v][3]);
-      q[1] = make_float4(ab[v][4], ab[v][5], ab[v][6], ab[v][7]);
+      reinterpret_cast<uint4*>(dw)[p] = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+      reinterpret_cast<uint4*>(db)[p] = make_uint4(ob[0], ob[1], ob[2], ob[3]);
     }
   }
 }
 
-// dw[c], db[c] = sum over the slabs of partials[slab][2][C].  A CTA takes 32 of the 2C columns; each of its eight warps
-// walks every eighth slab, and the warps' sums are added in their order.
-__global__ __launch_bounds__(256) void sum_slabs_kernel(const float* __restrict__ partials, bf16* __restrict__ dw,
+// dw and db of rows too wide for one CTA's registers to hold the column sums beside the row: a pass of its own over s and
+// dy.  A warp takes 256 channels, a CTA's four warps a quarter of its slab each.
+__global__ __launch_bounds__(128) void norm_columns_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ s,
+                                                           const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                           float* __restrict__ partials, long long rows, int channels,
+                                                           long long rows_per_cta) {
+  chain_begin();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, p = blockIdx.x * 32 + lane;
+  const long long begin = blockIdx.y * rows_per_cta;
+  const long long end = begin + rows_per_cta < rows ? begin + rows_per_cta : rows;
+  const bool mine = p < (channels >> 3);
+  f32x2 sw[4], sb[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sw[i] = sb[i] = pair(0.f, 0.f);
+  if (mine) {
+#pragma unroll 4
+    for (long long row = begin + warp; row < end; row += 4) {
+      f32x2 c[4], h[4];
+      unpack_pairs(load16(s + row * channels, p), c);
+      unpack_pairs(load16(dy + row * channels, p), h);
+      const float r = __ldg(rstd + row), m = -__ldg(mean + row) * r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sw[i] = fma2(h[i], fma2(c[i], pair(r, r), pair(m, m)), sw[i]);
+        sb[i] = add2(sb[i], h[i]);
+      }
+    }
+  }
+  __shared__ f32x2 sums[3][8][32];
+  if (warp > 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sums[warp - 1][i][lane] = sw[i];
+      sums[warp - 1][4 + i][lane] = sb[i];
+    }
+  }
+  __syncthreads();
+  if (warp > 0 || !mine) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      sw[i] = add2(sw[i], sums[j][i][lane]);
+      sb[i] = add2(sb[i], sums[j][4 + i][lane]);
+    }
+    float* q = partials + (long long)blockIdx.y * 2 * channels + 8 * p + 2 * i;
+    *reinterpret_cast<float2*>(q) = halves(sw[i]);
+    *reinterpret_cast<float2*>(q + channels) = halves(sb[i]);
+  }
+}
+
+// dw[c], db[c] = sum over the slabs of partials[slab][2][C].  A CTA takes 32 of the 2C columns; each of its sixteen warps
+// walks every sixteenth slab with eight requests in flight, and the warps' sums are added in their order.
+constexpr int kSumWarps = 16;
+__global__ __launch_bounds__(kSumWarps * 32) void sum_slabs_kernel(const float* __restrict__ partials, bf16* __restrict__ dw,
                                                         bf16* __restrict__ db, int slabs, int channels) {
   chain_begin();
-  __shared__ float sums[8][33];
+  __shared__ float sums[kSumWarps][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int column = blockIdx.x * 32 + lane, columns = 2 * channels;
-  float a0 = 0.f, a1 = 0.f;
+  float acc = 0.f;
   if (column < columns) {
-    int s = warp;
-    for (; s + 8 < slabs; s += 16) {
-      a0 += partials[(long long)s * columns + column];
-      a1 += partials[(long long)(s + 8) * columns + column];
+    for (int s = warp; s < slabs; s += kSumWarps * 8) {
+      float v[8];  // the eight requests leave together: the row is clamped rather than the load skipped
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = s + j * kSumWarps;
+        v[j] = __ldg(partials + (long long)(at < slabs ? at : s) * columns + column);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc += s + j * kSumWarps < slabs ? v[j] : 0.f;
     }
-    if (s < slabs) a0 += partials[(long long)s * columns + column];
   }
-  sums[warp][lane] = a0 + a1;
+  sums[warp][lane] = acc;
   __syncthreads();
   if (warp != 0 || column >= columns) return;
   float total = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) total += sums[w][lane];
+  for (int w = 0; w < kSumWarps; ++w) total += sums[w][lane];
   (column < channels ? dw[column] : db[column - channels]) = IO::store(total);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
 constexpr int kMaxChannels = 512 * 4 * 8;
-constexpr int kSlabsPerSm = 4;
+constexpr int kSlabsPerSm = 2;
+constexpr int kForwardPieces = 4, kBackwardPieces = 2;
 
 int sm_count() {
   int dev = 0, n = 0;
@@ -329,19 +440,19 @@ NormPlan plan_backward(long long rows, int resident) {
   return {(int)((rows + per - 1) / per), per};
 }
 
-// calls f with the group size and the pieces per thread that cover the channels
-template <typename F>
+// Calls f with the group size and the pieces per thread that cover the channels; kMost pieces per thread at most.
+template <int kMost, typename F>
 int by_width(int channels, F&& f) {
   const int pieces = channels / 8;
   using std::integral_constant;
 #define WIDTH(T, V) f(integral_constant<int, T>{}, integral_constant<int, V>{})
   if (pieces <= 32) return WIDTH(32, 1);
   if (pieces <= 64) return WIDTH(32, 2);
-  if (pieces <= 128) return WIDTH(64, 2);
-  if (pieces <= 256) return WIDTH(128, 2);
-  if (pieces <= 512) return WIDTH(256, 2);
-  if (pieces <= 1024) return WIDTH(512, 2);
-  return WIDTH(512, 4);
+  if (pieces <= 128) return WIDTH(128 / kMost, kMost);
+  if (pieces <= 256) return WIDTH(256 / kMost, kMost);
+  if (pieces <= 512) return WIDTH(512 / kMost, kMost);
+  if (pieces <= 1024) return WIDTH(1024 / kMost, kMost);
+  return WIDTH(2048 / kMost, kMost);
 #undef WIDTH
 }
 
@@ -373,9 +484,9 @@ extern "C" int frwkv_pretrain_layer_norm_forward(const void* x, const void* resi
   FRWKV_REQUIRE(aligned16({x, residual, weight, bias, sum_out, out}),
                 "pretrain_layer_norm: tensors must be 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return by_width(channels, [&](auto t, auto v) {
-    constexpr int T = decltype(t)::value, V = decltype(v)::value, kGroups = cta_threads(T) / T;
-    const dim3 grid((unsigned)((rows + kGroups - 1) / kGroups)), block(cta_threads(T));
+  return by_width<kForwardPieces>(channels, [&](auto t, auto v) {
+    constexpr int T = decltype(t)::value, V = decltype(v)::value, kGroups = forward_threads(T) / T;
+    const dim3 grid((unsigned)((rows + kGroups - 1) / kGroups)), block(forward_threads(T));
     const auto kernel = residual != nullptr ? norm_forward_kernel<T, V, true> : norm_forward_kernel<T, V, false>;
     launch_chained(kernel, grid, block, 0, s, static_cast<const bf16*>(x), static_cast<const bf16*>(residual),
                    static_cast<const bf16*>(weight), static_cast<const bf16*>(bias), static_cast<bf16*>(sum_out),
@@ -387,7 +498,7 @@ extern "C" int frwkv_pretrain_layer_norm_forward(const void* x, const void* resi
 extern "C" long long frwkv_pretrain_layer_norm_workspace_floats(long long rows, int channels) {
   if (rows <= 0 || channels <= 0) return 0;
   const long long slabs = frwkv::plan_backward(rows, frwkv::kSlabsPerSm).slabs;
-  return slabs > 1 ? slabs * 2 * channels : 1;
+  return slabs * 2 * channels;
 }
 
 extern "C" int frwkv_pretrain_layer_norm_backward(const void* grad_out, const void* grad_sum, const void* sum,
@@ -407,22 +518,31 @@ extern "C" int frwkv_pretrain_layer_norm_backward(const void* grad_out, const vo
   FRWKV_REQUIRE(aligned16({grad_out, grad_sum, sum, weight, grad_x, grad_weight, grad_bias, workspace}),
                 "pretrain_layer_norm_backward: tensors must be 16-byte aligned");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return by_width(channels, [&](auto t, auto v) {
+  return by_width<kBackwardPieces>(channels, [&](auto t, auto v) {
     constexpr int T = decltype(t)::value, V = decltype(v)::value;
-    const auto kernel = grad_weight != nullptr
-                            ? (grad_sum != nullptr ? norm_backward_kernel<T, V, true, true> : norm_backward_kernel<T, V, false, true>)
+    constexpr bool kApart = T > 512;  // the column sums take a pass of their own
+    const bool parameters = grad_weight != nullptr;
+    const auto kernel = parameters && !kApart
+                            ? (grad_sum != nullptr ? norm_backward_kernel<T, V, true, !kApart> : norm_backward_kernel<T, V, false, !kApart>)
                             : (grad_sum != nullptr ? norm_backward_kernel<T, V, true, false> : norm_backward_kernel<T, V, false, false>);
     int resident = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, cta_threads(T), 0) != cudaSuccess || resident < 1)
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, backward_threads(T), 0) != cudaSuccess || resident < 1)
       return fail(FRWKV_ERR_CUDA, "pretrain_layer_norm_backward: %s", cudaGetErrorString(cudaGetLastError()));
     const NormPlan plan = plan_backward(rows, resident < kSlabsPerSm ? resident : kSlabsPerSm);
-    launch_chained(kernel, dim3(plan.slabs), dim3(cta_threads(T)), 0, s, static_cast<const bf16*>(grad_out),
+    launch_chained(kernel, dim3(plan.slabs), dim3(backward_threads(T)), 0, s, static_cast<const bf16*>(grad_out),
                    static_cast<const bf16*>(grad_sum), static_cast<const bf16*>(sum), static_cast<const bf16*>(weight), mean,
                    rstd, static_cast<bf16*>(grad_x), static_cast<bf16*>(grad_weight), static_cast<bf16*>(grad_bias),
                    workspace, rows, channels, plan.rows_per_cta);
     if (int rc = check_launch("norm_backward_kernel")) return rc;
-    if (grad_weight == nullptr || plan.slabs == 1) return (int)FRWKV_OK;
-    launch_chained(sum_slabs_kernel, dim3((2 * channels + 31) / 32), dim3(256), 0, s, static_cast<const float*>(workspace),
+    if (!parameters || (plan.slabs == 1 && !kApart)) return (int)FRWKV_OK;
+    if (kApart) {
+      launch_chained(norm_columns_kernel, dim3((channels + 255) / 256, plan.slabs), dim3(128), 0, s,
+                     static_cast<const bf16*>(grad_out), static_cast<const bf16*>(sum), mean, rstd, workspace, rows, channels,
+                     plan.rows_per_cta);
+      if (int rc = check_launch("norm_columns_kernel")) return rc;
+    }
+    launch_chained(sum_slabs_kernel, dim3((2 * channels + 31) / 32), dim3(kSumWarps * 32), 0, s,
+                   static_cast<const float*>(workspace),
                    static_cast<bf16*>(grad_weight), static_cast<bf16*>(grad_bias), plan.slabs, channels);
     return check_launch("sum_slabs_kernel");
   });

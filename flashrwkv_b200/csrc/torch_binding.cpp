@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <array>
 #include <cmath>
 #include <limits>
 #include <map>
@@ -1927,59 +1928,62 @@ std::vector<torch::Tensor> pretrain_tmix_lnx_rkvres_xg_backward(torch::Tensor gr
 }
 
 // ---- block-level LayerNorm for training (x [...,C] bf16) --------------------------------------------------------------
-void check_norm_rows(const torch::Tensor& x) {
-  check_cuda_contiguous(x, "x");
-  TORCH_CHECK(x.scalar_type() == torch::kBFloat16, "x must be bfloat16");
-  TORCH_CHECK(x.dim() >= 2 && x.numel() > 0, "x must have non-empty shape [...,C]");
-}
-void check_norm_like(const torch::Tensor& t, const char* name, const torch::Tensor& x) {
-  check_cuda_contiguous(t, name);
-  TORCH_CHECK(t.scalar_type() == torch::kBFloat16 && t.device() == x.device() && t.sizes() == x.sizes(), name,
-              " must match x");
-}
-void check_norm_vector(const torch::Tensor& t, const char* name, const torch::Tensor& x) {
-  check_cuda_contiguous(t, name);
-  TORCH_CHECK(t.scalar_type() == torch::kBFloat16 && t.device() == x.device() && t.dim() == 1 &&
-                  t.size(0) == x.size(-1),
-              name, " must be bfloat16 [C] on x's device");
+// These operators are autograd functions of this layer rather than of Python: a call on a short batch is bound by its host
+// time, and a backward node that runs here needs neither the interpreter nor its lock.
+torch::Tensor packed16(const torch::Tensor& t) {  // an upstream gradient as the kernels read it
+  auto g = t.contiguous();
+  return reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0 ? g : g.clone();
 }
 
-// returns {sum (x itself without a residual), normalised rows, mean, rstd}
-std::vector<torch::Tensor> pretrain_tmix_layer_norm_forward(torch::Tensor x, std::optional<torch::Tensor> residual,
-                                                            torch::Tensor weight, torch::Tensor bias, double eps) {
-  check_norm_rows(x);
-  if (residual.has_value()) check_norm_like(*residual, "residual", x);
-  check_norm_vector(weight, "weight", x);
-  check_norm_vector(bias, "bias", x);
+void check_norm_tensor(const torch::Tensor& t, const char* name, const torch::Tensor& x) {
+  if (!(t.is_cuda() && t.scalar_type() == torch::kBFloat16 && t.is_contiguous()))
+    throw py::value_error(std::string(name) + " must be contiguous CUDA bfloat16");
+  if (t.device() != x.device()) throw py::value_error(std::string(name) + " must share x's device");
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) throw py::value_error(std::string(name) + " must be 16-byte aligned");
+}
+
+void check_norm(const torch::Tensor& x, const torch::Tensor* residual, const torch::Tensor& weight,
+                const torch::Tensor& bias, double eps) {
+  check_norm_tensor(x, "x", x);
+  if (x.dim() < 2 || x.numel() == 0) throw py::value_error("x must have non-empty shape [...,C]");
+  if (x.size(-1) % 8 || x.size(-1) > 16384) throw py::value_error("C must be a multiple of 8 up to 16384");
+  if (residual != nullptr) {
+    check_norm_tensor(*residual, "residual", x);
+    if (residual->sizes() != x.sizes()) throw py::value_error("residual must have the same shape as x");
+  }
+  check_norm_tensor(weight, "weight", x);
+  check_norm_tensor(bias, "bias", x);
+  if (weight.dim() != 1 || weight.size(0) != x.size(-1)) throw py::value_error("weight must have shape [C]");
+  if (bias.dim() != 1 || bias.size(0) != x.size(-1)) throw py::value_error("bias must have shape [C]");
+  const float e = static_cast<float>(eps);
+  if (!(e > 0.f) || !std::isfinite(e)) throw py::value_error("eps must be positive");
+}
+
+// forward values; `stats` [2, rows] receives mean and rstd
+void norm_forward(const torch::Tensor& x, const torch::Tensor* residual, const torch::Tensor& weight,
+                  const torch::Tensor& bias, double eps, torch::Tensor& sum, torch::Tensor& out, torch::Tensor& stats) {
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t channels = x.size(-1), rows = x.numel() / channels;
-  auto sum = residual.has_value() ? torch::empty_like(x) : x;
-  auto out = torch::empty_like(x);
-  auto stats = torch::empty({2, rows}, x.options().dtype(torch::kFloat32));
-  auto mean = stats.select(0, 0), rstd = stats.select(0, 1);
-  check_rc(frwkv_pretrain_layer_norm_forward(
-      x.data_ptr(), residual.has_value() ? residual->data_ptr() : nullptr, weight.data_ptr(), bias.data_ptr(),
-      residual.has_value() ? sum.data_ptr() : nullptr, out.data_ptr(), mean.data_ptr<float>(), rstd.data_ptr<float>(),
-      rows, static_cast<int>(channels), static_cast<float>(eps), current_stream(x)));
-  return {sum, out, mean, rstd};
+  sum = residual != nullptr ? torch::empty_like(x) : x;
+  out = torch::empty_like(x);
+  stats = torch::empty({2, rows}, x.options().dtype(torch::kFloat32));
+  float* mean = stats.data_ptr<float>();
+  check_rc(frwkv_pretrain_layer_norm_forward(x.data_ptr(), residual != nullptr ? residual->data_ptr() : nullptr,
+                                             weight.data_ptr(), bias.data_ptr(),
+                                             residual != nullptr ? sum.data_ptr() : nullptr, out.data_ptr(), mean,
+                                             mean + rows, rows, static_cast<int>(channels), static_cast<float>(eps),
+                                             current_stream(x)));
 }
 
-// returns {gradient of the normalised rows' source} or {that, gradient of weight, gradient of bias}
-std::vector<torch::Tensor> pretrain_tmix_layer_norm_backward(torch::Tensor grad_out,
-                                                             std::optional<torch::Tensor> grad_sum, torch::Tensor sum,
-                                                             torch::Tensor weight, torch::Tensor mean,
-                                                             torch::Tensor rstd, bool parameters) {
-  check_norm_rows(sum);
-  check_norm_like(grad_out, "grad_out", sum);
-  if (grad_sum.has_value()) check_norm_like(*grad_sum, "grad_sum", sum);
-  check_norm_vector(weight, "weight", sum);
-  const int64_t channels = sum.size(-1), rows = sum.numel() / channels;
-  for (const auto& t : {mean, rstd}) {
-    check_cuda_contiguous(t, "mean and rstd");
-    TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.numel() == rows && t.device() == sum.device(),
-                "mean and rstd must be float32 [rows] on x's device");
-  }
+// {gradient of the sum, of weight, of bias}; undefined where nothing is asked or nothing arrives
+std::array<torch::Tensor, 3> norm_backward(const torch::Tensor& grad_sum, const torch::Tensor& grad_out,
+                                           const torch::autograd::variable_list& saved, bool parameters) {
+  if (!grad_out.defined()) return {grad_sum, torch::Tensor(), torch::Tensor()};
+  const torch::Tensor &sum = saved[0], &weight = saved[1], &stats = saved[2];
   const c10::cuda::CUDAGuard guard(sum.device());
+  const int64_t channels = sum.size(-1), rows = sum.numel() / channels;
+  const auto g = packed16(grad_out);
+  const auto gs = grad_sum.defined() ? packed16(grad_sum) : torch::Tensor();
   auto grad_x = torch::empty_like(sum);
   torch::Tensor grad_weight, grad_bias, workspace;
   if (parameters) {
@@ -1988,13 +1992,69 @@ std::vector<torch::Tensor> pretrain_tmix_layer_norm_backward(torch::Tensor grad_
     workspace = torch::empty({frwkv_pretrain_layer_norm_workspace_floats(rows, static_cast<int>(channels))},
                              sum.options().dtype(torch::kFloat32));
   }
+  const float* mean = stats.data_ptr<float>();
   check_rc(frwkv_pretrain_layer_norm_backward(
-      grad_out.data_ptr(), grad_sum.has_value() ? grad_sum->data_ptr() : nullptr, sum.data_ptr(), weight.data_ptr(),
-      mean.data_ptr<float>(), rstd.data_ptr<float>(), grad_x.data_ptr(), parameters ? grad_weight.data_ptr() : nullptr,
-      parameters ? grad_bias.data_ptr() : nullptr, parameters ? workspace.data_ptr<float>() : nullptr,
-      parameters ? workspace.numel() : 0, rows, static_cast<int>(channels), current_stream(sum)));
-  if (!parameters) return {grad_x};
+      g.data_ptr(), gs.defined() ? gs.data_ptr() : nullptr, sum.data_ptr(), weight.data_ptr(), mean, mean + rows,
+      grad_x.data_ptr(), parameters ? grad_weight.data_ptr() : nullptr, parameters ? grad_bias.data_ptr() : nullptr,
+      parameters ? workspace.data_ptr<float>() : nullptr, parameters ? workspace.numel() : 0, rows,
+      static_cast<int>(channels), current_stream(sum)));
   return {grad_x, grad_weight, grad_bias};
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void refuse_second_order() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "this operator's backward pass is not itself differentiable (create_graph)");
+}
+
+struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
+                               const torch::Tensor& bias, double eps) {
+    torch::Tensor sum, out, stats;
+    norm_forward(x, nullptr, weight, bias, eps, sum, out, stats);
+    ctx->save_for_backward({x, weight, stats});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_order();
+    auto [gx, gw, gb] = norm_backward(torch::Tensor(), grads[0], ctx->get_saved_variables(),
+                                      ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
+    return {gx, gw, gb, torch::Tensor()};
+  }
+};
+
+struct AddLayerNormTrain : torch::autograd::Function<AddLayerNormTrain> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& residual,
+                               const torch::Tensor& weight, const torch::Tensor& bias, double eps) {
+    torch::Tensor sum, out, stats;
+    norm_forward(x, &residual, weight, bias, eps, sum, out, stats);
+    ctx->save_for_backward({sum, weight, stats});
+    ctx->set_materialize_grads(false);
+    return {sum, out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_order();
+    auto [gx, gw, gb] = norm_backward(grads[0], grads[1], ctx->get_saved_variables(),
+                                      ctx->needs_input_grad(2) || ctx->needs_input_grad(3));
+    return {gx, gx, gw, gb, torch::Tensor()};
+  }
+};
+
+torch::Tensor pretrain_tmix_layer_norm(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& bias,
+                                       double eps) {
+  check_norm(x, nullptr, weight, bias, eps);
+  return LayerNormTrain::apply(x, weight, bias, eps);
+}
+
+std::tuple<torch::Tensor, torch::Tensor> pretrain_tmix_add_layer_norm(const torch::Tensor& x,
+                                                                      const torch::Tensor& residual,
+                                                                      const torch::Tensor& weight,
+                                                                      const torch::Tensor& bias, double eps) {
+  check_norm(x, &residual, weight, bias, eps);
+  auto out = AddLayerNormTrain::apply(x, residual, weight, bias, eps);
+  return {out[0], out[1]};
 }
 
 }  // namespace
@@ -2131,11 +2191,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("pretrain_tmix_kk_pre_backward", &pretrain_tmix_kk_pre_backward);
   m.def("pretrain_tmix_lnx_rkvres_xg_forward", &pretrain_tmix_lnx_rkvres_xg_forward);
   m.def("pretrain_tmix_lnx_rkvres_xg_backward", &pretrain_tmix_lnx_rkvres_xg_backward);
-  m.def("pretrain_tmix_layer_norm_forward", &pretrain_tmix_layer_norm_forward, py::arg("x"), py::arg("residual"),
+  m.def("pretrain_tmix_layer_norm", &pretrain_tmix_layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"),
+        py::arg("eps"));
+  m.def("pretrain_tmix_add_layer_norm", &pretrain_tmix_add_layer_norm, py::arg("x"), py::arg("residual"),
         py::arg("weight"), py::arg("bias"), py::arg("eps"));
-  m.def("pretrain_tmix_layer_norm_backward", &pretrain_tmix_layer_norm_backward, py::arg("grad_out"),
-        py::arg("grad_sum"), py::arg("sum"), py::arg("weight"), py::arg("mean"), py::arg("rstd"),
-        py::arg("parameters"));
   m.def("recurrent_add_vec_forward_varlen", &recurrent_add_vec_forward_varlen, py::arg("x"), py::arg("vec"));
   m.def("tmix_act_forward", &tmix_act_forward, py::arg("x"), py::arg("act"));
   m.def("tmix_linear_runtime_layout", &linear_runtime_layout, py::arg("x"), py::arg("weight_kn"), py::arg("act") = 0,

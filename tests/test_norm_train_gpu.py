@@ -206,3 +206,34 @@ def test_many_rows_fall_into_many_slabs():
     out = F.pretrain_tmix_layer_norm_bf16(x, w, b)
     _, db = torch.autograd.grad(out, (w, b), torch.ones_like(out))
     assert torch.equal(db, torch.full_like(db, 9000.0))
+
+
+def test_second_order_is_refused():
+    import flashrwkv_b200 as F
+
+    i = _inputs(1, 4, 64, 3)
+    x = i["x"].requires_grad_()
+    out = F.pretrain_tmix_layer_norm_bf16(x, i["weight"], i["bias"])
+    with pytest.raises(RuntimeError, match="not itself differentiable"):
+        torch.autograd.grad(out, x, i["g"], create_graph=True)
+
+
+def test_refusals_on_the_device():
+    import flashrwkv_b200 as F
+
+    i = _inputs(2, 4, 64, 3)
+    x, w, b = i["x"], i["weight"], i["bias"]
+    shifted = torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view_as(x)
+    wide = torch.zeros(1, 16392, dtype=x.dtype, device="cuda")
+    for args, message in (((shifted, w, b), "16-byte aligned"), ((x[:, ::2], w, b), "contiguous"),
+                          ((x.float(), w, b), "bfloat16"), ((x, w[:8], b), "weight must have shape"),
+                          ((x, w, b[:8].contiguous()), "bias must have shape"), ((x[0, 0], w, b), "non-empty shape"),
+                          ((x[:0], w, b), "non-empty shape"), ((x.view(-1, 4), w[:4], b[:4]), "multiple of 8"),
+                          ((wide, wide[0], wide[0]), "up to 16384"), ((x, w.cpu(), b), "CUDA")):
+        with pytest.raises(ValueError, match=message):
+            F.pretrain_tmix_layer_norm_bf16(*args)
+    with pytest.raises(ValueError, match="same shape as x"):
+        F.pretrain_tmix_add_layer_norm_bf16(x, x[:1], w, b)
+    for eps in (0.0, -1.0, float("nan"), float("inf"), 1e-60):
+        with pytest.raises(ValueError, match="eps must be positive"):
+            F.pretrain_tmix_layer_norm_bf16(x, w, b, eps=eps)
