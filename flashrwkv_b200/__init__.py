@@ -18,6 +18,8 @@ from .tmix.wkv7 import (
     statetune_recurrent_fp32io16,
 )
 
+from .head import *  # noqa: F401,F403
+from .head import __all__ as _head_all
 from .tmix.a_gate import pretrain_tmix_a_gate_bf16
 from .tmix.kk_a_gate import infer_tmix_kk_a_gate_forward_varlen
 from .tmix.kk_pre import pretrain_tmix_kk_pre_bf16
@@ -50,6 +52,7 @@ __all__ = [
     "check_device_error_flags",
     "infer_tmix_vres_gate_forward_varlen",
     *_linear_all,
+    *_head_all,
     "infer_chunk_bf16_forward_varlen",
     "infer_recurrent_add_vec_forward_varlen",
     "infer_recurrent_fp16_advance_i32",

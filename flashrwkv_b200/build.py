@@ -38,6 +38,8 @@ CUDA_SOURCES = [
     "tmix_norm.cu",
     "tmix_train.cu",
     "tmix_norm_train.cu",
+    "head_loss.cu",
+    "head_gemm.cu",
     "tmix_linear.cu",
     "tmix_gemm_tma.cu",
     "wkv7_backward.cu",

@@ -1,0 +1,451 @@
+// The three matrix products of the head's losses on the 5th-generation tensor cores:
+//
+//   statistics    z = x W^T                 per 256 columns: row maximum and sum of exponentials (and the exponentials)
+//   grad_x        dx = g W                  contraction over the vocabulary
+//   grad_weight   dW = g^T x                contraction over the rows
+//
+// One persistent kernel, specialised by warp and run by pairs of CTAs (tcgen05, cta_group::2): a pair owns a 256 x 256
+// output tile, each CTA loads its 128 rows of A and its half of B, so that a byte of shared memory feeds twice the
+// arithmetic of a single CTA's 128 x 256 tile, which is bound by the fill of its shared memory.
+//   warp 0      producer: TMA tiles of 64 contraction values into a ring of six stages; both CTAs' bytes are counted on
+//               the leader's barrier
+//   warp 1      (leader) MMA issuer: four tcgen05.mma per stage into one of two accumulators in tensor memory; commits
+//               release the stage, and hand over the accumulator, in both CTAs
+//   warps 2..5  epilogue of the other accumulator meanwhile
+// All three operand layouts are read where they lie: x and W are K-major in z = x W^T; W in g W, and both g and x in g^T x,
+// are MN-major (the contraction index numbers the rows of the matrix in memory).  The number of rows that take part is known
+// on the device only (labels may be missing), so the kernels read it there.
+// Every wait is bounded; a role whose wait runs out sets the error flag and leaves, the others run into their own limits,
+// outputs that could not be made are NaN.
+
+#include "head_loss.cuh"
+#include "umma_pair.cuh"
+
+namespace frwkv {
+namespace head {
+namespace {
+
+using bf16 = __nv_bfloat16;
+using IO = Io16<bf16>;
+
+constexpr int kHalf = kTile / 2, kBK = 64;
+constexpr uint32_t kOperandBytes = kHalf * kBK * 2;  // 16 KB of each operand per CTA and stage
+constexpr uint32_t kStageBytes = 2 * kOperandBytes;
+constexpr int kStages = 6;
+constexpr uint32_t kSmem = kStages * kStageBytes + 1024;  // + slack to align the tiles to 1024 bytes
+constexpr int kThreads = 192;
+constexpr uint32_t kTmemCols = 2 * kTile;
+
+enum Product { kStats, kGradX, kGradWeight };
+
+struct Params {
+  CUtensorMap map_a, map_b;
+  CUtensorMap map_compact;  // kStats: A, kGradWeight: B, when some rows take no part
+  Rows rows;
+  int channels, vocab, splits;
+  float log2_scale;        // kStats
+  float2* stats;
+  int stats_stride;
+  __half* power;
+  long long ldp;
+  bf16* out;               // kGradX, kGradWeight
+  float* partials;
+  bool add;
+};
+
+struct Unit {
+  int m0, n0, split, kb_begin, kb_end;
+};
+
+// the work of a launch, from the number of rows that take part
+template <Product P>
+struct Work {
+  int tiles_m, tiles_n, units, kb_total, splits;
+  __device__ Work(const Params& p, int rows_here) {
+    const int m = P == kGradWeight ? p.vocab : rows_here;
+    const int n = P == kStats ? p.vocab : p.channels;
+    const int k = P == kStats ? p.channels : (P == kGradX ? p.vocab : rows_here);
+    tiles_m = (m + kTile - 1) / kTile;
+    tiles_n = (n + kTile - 1) / kTile;
+    kb_total = (k + kBK - 1) / kBK;
+    splits = P == kStats ? 1 : p.splits;
+    units = tiles_m * tiles_n * splits;
+  }
+  // Pairs that run at the same time work on neighbouring tiles of the same part of the contraction, so that they share
+  // their operands in L2.  Statistics: rows vary fastest (the whole x against a few tiles of W); the gradients: columns.
+  __device__ Unit at(int unit) const {
+    Unit u;
+    const int tiles = tiles_m * tiles_n;
+    u.split = unit / tiles;
+    const int t = unit - u.split * tiles;
+    u.m0 = (P == kStats ? t % tiles_m : t / tiles_n) * kTile;
+    u.n0 = (P == kStats ? t / tiles_m : t % tiles_n) * kTile;
+    u.kb_begin = (int)((long long)kb_total * u.split / splits);
+    u.kb_end = (int)((long long)kb_total * (u.split + 1) / splits);
+    return u;
+  }
+};
+
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8], bool wide) {
+  if (wide) {
+    stg256(p, make_uint4(v[0], v[1], v[2], v[3]), make_uint4(v[4], v[5], v[6], v[7]));
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+template <Product P>
+__global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_gemm_kernel(
+    const __grid_constant__ Params prm, int* __restrict__ error_flag) {
+  constexpr bool kAMn = P == kGradWeight, kBMn = P != kStats;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_holder;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = umma2::cluster_rank();
+  const uint32_t tiles_base = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
+
+  chain_release();
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      umma::mbar_init(&full_bar[i], 1);   // the leader's producer; the bytes of both CTAs
+      umma::mbar_init(&empty_bar[i], 1);  // a commit
+    }
+    for (int i = 0; i < 2; ++i) {
+      umma::mbar_init(&acc_full[i], 1);   // a commit
+      umma::mbar_init(&acc_empty[i], 8);  // the epilogue warps of both CTAs
+    }
+    umma::mbar_fence_init();
+  }
+  if (warp == 1) umma2::tmem_alloc(&tmem_holder, kTmemCols);
+  umma::fence_before_sync();
+  __syncthreads();
+  umma2::cluster_sync();
+  umma::fence_after_sync();
+  const uint32_t tmem = tmem_holder;
+  chain_wait();
+
+  const int count = *prm.rows.count;
+  const int left = count - prm.rows.piece_begin;
+  const int rows_here = left < 0 ? 0 : (left < prm.rows.piece_rows ? left : prm.rows.piece_rows);
+  const bool compact = count != prm.rows.total;
+  const Work<P> work(prm, rows_here);
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const CUtensorMap* map_a = P == kStats && compact ? &prm.map_compact : &prm.map_a;
+      const CUtensorMap* map_b = P == kGradWeight && compact ? &prm.map_compact : &prm.map_b;
+      const int a_row = P == kStats ? prm.rows.piece_begin : 0, b_row = P == kGradWeight ? prm.rows.piece_begin : 0;
+      uint32_t it = 0;
+      for (int unit = pair; unit < work.units && ok; unit += pairs) {
+        const Unit u = work.at(unit);
+        for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
+          const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
+          if (!umma2::wait_cluster(&empty_bar[s], ph ^ 1u)) { ok = false; break; }
+          const uint32_t full = umma2::in_leader(&full_bar[s]);
+          if (rank == 0) umma::mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
+          const uint32_t a_dst = tiles_base + s * kStageBytes, b_dst = a_dst + kOperandBytes;
+          const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * kHalf, k = kb * kBK;
+          if (kAMn) {
+            umma2::tma_load_2d(a_dst, map_a, m, a_row + k, full);
+            umma2::tma_load_2d(a_dst + 8192, map_a, m + 64, a_row + k, full);
+          } else {
+            umma2::tma_load_2d(a_dst, map_a, k, a_row + m, full);
+          }
+          if (kBMn) {
+            umma2::tma_load_2d(b_dst, map_b, n, b_row + k, full);
+            umma2::tma_load_2d(b_dst + 8192, map_b, n + 64, b_row + k, full);
+          } else {
+            umma2::tma_load_2d(b_dst, map_b, k, n, full);
+          }
+        }
+      }
+      // the last commits must have arrived here before this CTA may leave
+      for (uint32_t i = 0; i < (uint32_t)kStages && i < it && ok; ++i) {
+        const uint32_t j = it - 1 - i;
+        if (!umma2::wait_cluster(&empty_bar[j % kStages], (j / kStages) & 1u)) ok = false;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = umma2::idesc_bf16_256(kAMn, kBMn);
+      uint32_t it = 0, t = 0;
+      for (int unit = pair; unit < work.units && ok; unit += pairs) {
+        const Unit u = work.at(unit);
+        if (u.kb_begin == u.kb_end) continue;  // nothing to contract: the epilogue writes zeros
+        const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
+        ++t;
+        if (!umma2::wait_cluster(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
+        umma::fence_after_sync();
+        const uint32_t d_tmem = tmem + acc * kTile;
+        for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
+          const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
+          if (!umma2::wait_cluster(&full_bar[s], ph)) { ok = false; break; }
+          umma::fence_after_sync();
+          const uint32_t a = tiles_base + s * kStageBytes, b = a + kOperandBytes;
+#pragma unroll
+          for (int ks = 0; ks < kBK / 16; ++ks)
+            umma2::mma_bf16(d_tmem, kAMn ? umma2::desc_mn_major(a + ks * 2048) : umma2::desc_k_major(a + ks * 32),
+                            kBMn ? umma2::desc_mn_major(b + ks * 2048) : umma2::desc_k_major(b + ks * 32), idesc,
+                            (kb > u.kb_begin || ks > 0) ? 1u : 0u);
+          umma2::commit_both(&empty_bar[s]);
+        }
+        if (ok) umma2::commit_both(&acc_full[acc]);
+      }
+    }
+  } else {
+    const uint32_t quarter = warp & 3u;  // the tensor-memory lanes this warp may read: 32 * (warp % 4) ..
+    const uint32_t lanes = (32u * quarter) << 16;
+    const int row_in_tile = (int)rank * kHalf + 32 * (int)quarter + lane;
+    const int m_end = P == kGradWeight ? prm.vocab : rows_here;
+    uint32_t t = 0;
+    for (int unit = pair; unit < work.units; unit += pairs) {
+      const Unit u = work.at(unit);
+      const bool empty = u.kb_begin == u.kb_end;
+      const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
+      if (!empty) ++t;
+      // Warp-uniform outcome: the tensor-memory loads below need the whole warp.  Once a wait has run out, this unit and all
+      // later ones read as NaN.
+      if (ok && !empty && !__all_sync(0xffffffffu, umma2::wait_cluster(&acc_full[acc], aph))) ok = false;
+      umma::fence_after_sync();
+      const uint32_t source = tmem + lanes + acc * kTile;
+      const int m = u.m0 + row_in_tile;
+      const auto read32 = [&](int c0, float (&z)[32]) {
+        uint32_t v[32];
+        if (ok && !empty) {
+          umma::tmem_ld32(source + c0, v);
+          umma::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z[j] = !ok ? quiet_nan() : (empty ? 0.f : __uint_as_float(v[j]));
+      };
+      if (P == kStats) {
+        // two sweeps over the accumulator: the maximum, then the exponentials and their sum, all in units of log2
+        const int valid = prm.vocab - u.n0;  // columns of the tile inside the vocabulary (may exceed the tile)
+        float z[32], high = -INFINITY;
+        bool nan = false;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          read32(c0, z);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (c0 + j < valid) {
+              high = fmaxf(high, z[j]);
+              nan |= z[j] != z[j];  // fmaxf drops a NaN, the statistics must not
+            }
+          }
+        }
+        high = nan ? quiet_nan() : high * prm.log2_scale;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          read32(c0, z);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            z[j] = c0 + j < valid ? ex2_approx(fmaf(z[j], prm.log2_scale, -high)) : 0.f;
+            sum += z[j];
+          }
+          if (prm.power != nullptr && m < m_end && u.n0 + c0 < prm.ldp) {
+            __half* dst = prm.power + m * prm.ldp + u.n0 + c0;  // rows are padded to 64 columns: whole 64-byte pieces
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t o[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = Io16<__half>::pack(z[16 * h + 2 * j], z[16 * h + 2 * j + 1]);
+              store32(dst + 16 * h, o, true);
+            }
+          }
+        }
+        if (m < m_end) prm.stats[(long long)(u.n0 / kTile) * prm.stats_stride + m] = make_float2(high, sum);
+      } else {
+        const long long slot = (long long)u.split * (P == kGradX ? prm.rows.piece_rows : prm.vocab);
+        const bool inside = m < m_end;
+        const int row = P == kGradX && inside && prm.partials == nullptr ? prm.rows.row_map[prm.rows.piece_begin + m] : m;
+        const bool wide = (prm.channels & 15) == 0 && (reinterpret_cast<uintptr_t>(prm.out) & 31u) == 0;
+#pragma unroll 1
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          float z[32];
+          read32(c0, z);
+          if (inside && prm.partials != nullptr) {
+            float* dst = prm.partials + (slot + m) * prm.channels + u.n0 + c0;
+#pragma unroll
+            for (int h = 0; h < 32; h += 8) {
+              if (u.n0 + c0 + h < prm.channels) {  // channels are a multiple of 8
+                if (prm.add) {
+                  const float4 a = *reinterpret_cast<const float4*>(dst + h), b = *reinterpret_cast<const float4*>(dst + h + 4);
+                  z[h] += a.x; z[h + 1] += a.y; z[h + 2] += a.z; z[h + 3] += a.w;
+                  z[h + 4] += b.x; z[h + 5] += b.y; z[h + 6] += b.z; z[h + 7] += b.w;
+                }
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(z[h + j]);
+                store32(dst + h, o, true);
+              }
+            }
+          } else if (inside) {
+            bf16* dst = prm.out + (long long)row * prm.channels + u.n0 + c0;
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              uint32_t o[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = IO::pack(z[h + 2 * j], z[h + 2 * j + 1]);
+              const int room = prm.channels - (u.n0 + c0 + h);
+              if (room >= 16) {
+                store32(dst + h, o, wide);
+              } else if (room >= 8) {
+                *reinterpret_cast<uint4*>(dst + h) = make_uint4(o[0], o[1], o[2], o[3]);
+              }
+            }
+          }
+        }
+      }
+      if (ok && !empty) {
+        umma::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) umma2::arrive_cluster(umma2::in_leader(&acc_empty[acc]));
+      }
+    }
+  }
+  if (!ok) {
+    if (error_flag != nullptr) atomicExch(error_flag, 1 + (int)P);
+    // give copies and MMAs that may still be in flight time to finish before the shared and tensor memory go away
+    for (int i = 0; i < 64; ++i) __nanosleep(1000);
+  }
+  __syncwarp();
+  umma::fence_before_sync();
+  __syncthreads();
+  umma2::cluster_sync();
+  if (warp == 1) umma2::tmem_dealloc(tmem, kTmemCols);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------------------
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+  static const EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+// [rows][columns] bf16 with rows `stride` values apart, boxes of 64 columns x box_rows, 128-byte swizzle, zeros outside
+bool make_map(CUtensorMap* map, const void* base, long long rows, long long columns, long long stride, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t box[2] = {64u, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  return encode_tiled() != nullptr &&
+         encode_tiled()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, elem,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int pair_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      n < 2)
+    n = 148;
+  return n / 2;
+}
+
+long long tiles_of(long long n) { return (n + kTile - 1) / kTile; }
+
+template <Product P>
+int launch(const Params& prm, long long units, int* error_flag, cudaStream_t stream) {
+  cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+  if (e != cudaSuccess) return fail(FRWKV_ERR_CUDA, "pretrain_head_loss: %s", cudaGetErrorString(e));
+  const int pairs = pair_count();
+  const int grid = 2 * (int)(units < pairs ? units : pairs);
+  launch_chained(head_gemm_kernel<P>, dim3(grid), dim3(kThreads), kSmem, stream, prm, error_flag);
+  return check_launch("head_gemm_kernel");
+}
+
+int map_failure() { return fail(FRWKV_ERR_CUDA, "pretrain_head_loss: cuTensorMapEncodeTiled failed"); }
+
+}  // namespace
+
+// A wave of pairs takes one tile each, so the time goes with ceil(tiles * splits / pairs) / splits; every part is written
+// and read once more in fp32.
+int contraction_splits(long long rows, long long columns, long long k) {
+  const double pairs = pair_count(), tiles = (double)(tiles_of(rows) * tiles_of(columns));
+  const double block_us = 0.30;                                   // 256 x 256 x 64 by a pair, as measured
+  const double part_us = (double)(rows * columns) * 8 / 5.0e6;    // one fp32 part there and back
+  const long long blocks = (k + kBK - 1) / kBK;
+  int best = 1;
+  double best_us = 0;
+  for (int s = 1; s <= 64 && (s == 1 || blocks / s >= 4); ++s) {
+    const double waves = (double)(long long)((tiles * s + pairs - 1) / pairs);
+    const double us = waves * (double)((blocks + s - 1) / s) * block_us + (s > 1 ? 3.0 + s * part_us : 0.0);
+    if (s == 1 || us < best_us) {
+      best = s;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
+int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
+                       float log2_scale, float2* stats, int stats_stride, void* power, long long ldp, int* error_flag,
+                       cudaStream_t stream) {
+  Params prm{};
+  prm.rows = rows;
+  prm.channels = channels;
+  prm.vocab = vocab;
+  prm.splits = 1;
+  prm.log2_scale = log2_scale;
+  prm.stats = stats;
+  prm.stats_stride = stats_stride;
+  prm.power = static_cast<__half*>(power);
+  prm.ldp = ldp;
+  if (!make_map(&prm.map_a, x, rows.total, channels, channels, kHalf) ||
+      !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kHalf) ||
+      !make_map(&prm.map_b, weight, vocab, channels, channels, kHalf))
+    return map_failure();
+  return launch<kStats>(prm, tiles_of(rows.piece_rows) * tiles_of(vocab), error_flag, stream);
+}
+
+int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab, int splits,
+                  void* grad_x, float* partials, int* error_flag, cudaStream_t stream) {
+  Params prm{};
+  prm.rows = rows;
+  prm.channels = channels;
+  prm.vocab = vocab;
+  prm.splits = splits;
+  prm.out = static_cast<bf16*>(grad_x);
+  prm.partials = partials;
+  if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kHalf) ||
+      !make_map(&prm.map_b, weight, vocab, channels, channels, kBK))
+    return map_failure();
+  return launch<kGradX>(prm, tiles_of(rows.piece_rows) * tiles_of(channels) * splits, error_flag, stream);
+}
+
+int launch_grad_weight(const void* g, long long ldg, const void* x, const void* x_compact, const Rows& rows, int channels,
+                       int vocab, int splits, void* grad_weight, float* partials, bool add, int* error_flag,
+                       cudaStream_t stream) {
+  Params prm{};
+  prm.rows = rows;
+  prm.channels = channels;
+  prm.vocab = vocab;
+  prm.splits = splits;
+  prm.out = static_cast<bf16*>(grad_weight);
+  prm.partials = partials;
+  prm.add = add;
+  if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kBK) ||
+      !make_map(&prm.map_b, x, rows.total, channels, channels, kBK) ||
+      !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kBK))
+    return map_failure();
+  return launch<kGradWeight>(prm, tiles_of(vocab) * tiles_of(channels) * splits, error_flag, stream);
+}
+
+}  // namespace head
+}  // namespace frwkv

@@ -1,0 +1,515 @@
+// The head's losses for training: the vocabulary projection, its softmax, a loss against labels or against a teacher's
+// highest logits, and the gradients of the rows and of the weight, without ever holding the logits.
+//
+//   z_n = W x_n / T            q_n = softmax(z_n)           lse_n = log sum_v exp(z_nv)
+//   label t:                   loss_n = lse_n - z_nt                                        (T = 1, one entry, p = 1)
+//   teacher entries (t_k, l_k): p = softmax(l / T) over the entries that are there (l > -inf),
+//                              loss_n = T^2 sum_k p_k (log p_k - z_n,t_k + lse_n)
+//   g_nv = scale_n T (q_nv - sum over k with t_k = v of p_k)      dx = g W,  dW = g^T x
+//
+// Passes over a piece of the rows (all of them while 2 rows x vocabulary bytes fit kPieceBytes):
+//   plan     numbers the rows that have a label; rows without one take no part in any product (compact_kernel copies the
+//            others together, or does nothing where every row takes part), so what they hold, NaN included, reaches nothing
+//   stats    z by 256 columns on the tensor cores; the epilogue leaves each row's maximum and sum of exponentials, and for
+//            gradients the exponentials themselves in fp16, relative to that maximum (error 2^-12 of each, where a bf16
+//            value would add 2^-9 to the one rounding that g needs as a tensor-core operand)
+//   finish   per row: lse from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
+//            the exponentials times their tile's factor in place, now g in bf16; the labels' entries from fp32
+//   products dx and dW
+// so a step costs three products of 2 rows x vocabulary x channels, not the four of recomputing z for the backward pass,
+// and the weight is read twice.  The price is that gradients are made with the loss, before the upstream gradient is known:
+// scale_kernel applies it afterwards (it leaves at once where the gradient is one).
+//
+// The reference fuses the same cross entropy at csrc/sm90/head/l2wrap_ce/pretrain_bf16_forward.cu:282-286 around library
+// products and kept logits; it has no distillation.
+
+#include "head_loss.cuh"
+
+namespace frwkv {
+namespace head {
+namespace {
+
+using bf16 = __nv_bfloat16;
+using IO = Io16<bf16>;
+
+constexpr long long kPieceBytes = 1ll << 30;   // exponentials of one piece
+constexpr long long kStatsBytes = 1ll << 28;   // statistics of one piece
+constexpr int kMaxTop = 512;
+constexpr int kFinishThreads = 256;
+
+struct Labels {
+  const void* index;        // [rows][top] int32 or int64
+  bool wide;                // int64
+  const float* teacher;     // [rows][top] logits, or null: one label per row
+  long long ignore_index;   // labels only
+  int top;
+  float inv_temperature, temperature;
+  __device__ long long at(long long i) const {
+    return wide ? static_cast<const long long*>(index)[i] : (long long)static_cast<const int*>(index)[i];
+  }
+};
+
+// ---- plan: which rows take part --------------------------------------------------------------------------------------
+// flags[row] = the teacher has an entry for this row; a warp per row
+__global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* __restrict__ flags, int rows) {
+  chain_begin();
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  bool any = false;
+  for (int k = lane; k < labels.top; k += 32) any |= !(labels.teacher[(long long)row * labels.top + k] == -INFINITY);
+  any = __any_sync(0xffffffffu, any);
+  if (lane == 0) flags[row] = any;
+}
+
+// One CTA numbers the rows in order: position[row] = compact number or -1, row_map its inverse, count.  `position` holds
+// the teacher's flags on entry.
+__global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position, int* __restrict__ row_map,
+                                                    int* __restrict__ count, int* __restrict__ error_flag, int rows) {
+  chain_begin();
+  __shared__ int warp_sums[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int done = 0;
+  for (int begin = 0; begin < rows; begin += 1024) {
+    const int row = begin + threadIdx.x;
+    const bool used = row < rows && (labels.teacher != nullptr ? position[row] != 0 : labels.at(row) != labels.ignore_index);
+    const unsigned mask = __ballot_sync(0xffffffffu, used);
+    if (lane == 0) warp_sums[warp] = __popc(mask);
+    __syncthreads();
+    const int mine = warp_sums[lane];
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
+    const int all = __reduce_add_sync(0xffffffffu, mine);
+    const int at = done + before + __popc(mask & ((1u << lane) - 1u));
+    if (row < rows) position[row] = used ? at : -1;
+    if (used) row_map[at] = row;
+    done += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    *count = done;
+    *error_flag = 0;
+  }
+}
+
+// Copies the rows that take part together; the others get a zero loss and a zero gradient.  The rows behind the last, up
+// to the next multiple of 64, become zeros: they meet zeros of g in a block of the contraction over rows.
+__global__ __launch_bounds__(256) void compact_kernel(const uint4* __restrict__ x, const int* __restrict__ position,
+                                                      const int* __restrict__ count, uint4* __restrict__ x_compact,
+                                                      uint4* __restrict__ grad_x, float* __restrict__ row_losses, int rows,
+                                                      int pieces) {
+  chain_begin();
+  const int used = *count;
+  if (used == rows) return;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const int at = position[row];
+  for (int p = lane; p < pieces; p += 32) {
+    if (at >= 0) {
+      x_compact[(long long)at * pieces + p] = __ldg(x + (long long)row * pieces + p);
+    } else if (grad_x != nullptr) {
+      grad_x[(long long)row * pieces + p] = zero;
+    }
+    if (row >= used && row < ((used + 63) & ~63)) x_compact[(long long)row * pieces + p] = zero;
+  }
+  if (lane == 0 && at < 0) row_losses[row] = 0.f;
+}
+
+// ---- finish: statistics to losses and logit gradients ------------------------------------------------------------------
+__device__ __forceinline__ float block_reduce(float v, float* scratch, bool maximum) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = maximum ? fmaxf(v, w) : v + w;
+  }
+  __syncthreads();  // scratch may still be read from the reduction before
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = scratch[0];
+#pragma unroll
+  for (int i = 1; i < kFinishThreads / 32; ++i) v = maximum ? fmaxf(v, scratch[i]) : v + scratch[i];
+  return v;
+}
+
+struct FinishArgs {
+  Rows rows;
+  Labels labels;
+  const bf16* x;
+  const bf16* weight;
+  const float2* stats;
+  int stats_stride, vocab, channels;
+  uint4* g;            // exponentials in, logit gradients out, ldg values per row; null without gradients
+  long long ldg;
+  bool mean;
+  const float* row_grads;    // upstream gradients of the row losses, or null
+  const float* grad_scale;   // upstream gradient of the loss, or null
+  float* row_losses;
+};
+
+__global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs a) {
+  chain_begin();
+  extern __shared__ float factor[];  // [tiles] then logit [top] and share [top]
+  __shared__ float scratch[kFinishThreads / 32];
+  const int tiles = (a.vocab + kTile - 1) / kTile, top = a.labels.top;
+  float* logit = factor + tiles;
+  float* share = logit + top;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int count = *a.rows.count, left = count - a.rows.piece_begin;
+  const int rows_here = left < 0 ? 0 : (left < a.rows.piece_rows ? left : a.rows.piece_rows);
+  const int r = blockIdx.x;
+  const int groups = (int)(a.ldg / 8);
+  uint4* g = a.g + (long long)r * groups;
+  if (r >= rows_here) {
+    // zeros behind the last row, to the end of its block of the contraction over rows
+    if (a.g != nullptr && r < ((rows_here + 63) & ~63))
+      for (int i = tid; i < groups; i += kFinishThreads) g[i] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  const long long n = a.rows.row_map[a.rows.piece_begin + r];
+
+  // the softmax's normaliser, in units of log2
+  float high = -INFINITY, sum = 0.f;
+  for (int t = tid; t < tiles; t += kFinishThreads) high = fmaxf(high, a.stats[(long long)t * a.stats_stride + r].x);
+  high = block_reduce(high, scratch, true);
+  for (int t = tid; t < tiles; t += kFinishThreads) {
+    const float2 s = a.stats[(long long)t * a.stats_stride + r];
+    sum = fmaf(s.y, ex2_approx(s.x - high), sum);
+  }
+  sum = block_reduce(sum, scratch, false);
+  const float lse2 = high + log2f(sum);
+  // lse - z is taken as (max - z) + log(sum): both terms are small where the label is likely
+  const float max_z = high * 0.6931471805599453f, log_sum = logf(sum);
+  for (int t = tid; t < tiles; t += kFinishThreads) factor[t] = a.stats[(long long)t * a.stats_stride + r].x - lse2;
+
+  // the labels' logits: a warp per entry
+  const long long entry = n * top;
+  const int pieces = a.channels / 8;
+  bool bad = false;
+  for (int k = warp; k < top; k += kFinishThreads / 32) {
+    const bool there = a.labels.teacher == nullptr || !(a.labels.teacher[entry + k] == -INFINITY);
+    const long long v = there ? a.labels.at(entry + k) : 0;
+    const bool inside = v >= 0 && v < a.vocab;
+    float dot = 0.f;
+    if (there && inside) {
+      const uint4* xr = reinterpret_cast<const uint4*>(a.x + n * a.channels);
+      const uint4* wr = reinterpret_cast<const uint4*>(a.weight + v * a.channels);
+#pragma unroll 4
+      for (int p = lane; p < pieces; p += 32) {
+        const uint4 ux = __ldg(xr + p), uw = __ldg(wr + p);
+        const uint32_t xs[4] = {ux.x, ux.y, ux.z, ux.w}, ws[4] = {uw.x, uw.y, uw.z, uw.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 fx = IO::unpack(xs[e]), fw = IO::unpack(ws[e]);
+          dot = fmaf(fx.x, fw.x, dot);
+          dot = fmaf(fx.y, fw.y, dot);
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    }
+    bad |= there && !inside;
+    if (lane == 0) logit[k] = dot * a.labels.inv_temperature;
+  }
+  bad = __syncthreads_or(bad);
+
+  float loss;
+  if (a.labels.teacher == nullptr) {
+    if (tid == 0) share[0] = 1.f;
+    loss = (max_z - logit[0]) + log_sum;
+  } else {
+    float most = -INFINITY, total = 0.f;
+    for (int k = tid; k < top; k += kFinishThreads) most = fmaxf(most, a.labels.teacher[entry + k] * a.labels.inv_temperature);
+    most = block_reduce(most, scratch, true);
+    for (int k = tid; k < top; k += kFinishThreads) {
+      const float p = expf(a.labels.teacher[entry + k] * a.labels.inv_temperature - most);
+      share[k] = p;
+      total += p;
+    }
+    total = block_reduce(total, scratch, false);
+    const float log_total = logf(total);
+    float part = 0.f;
+    for (int k = tid; k < top; k += kFinishThreads) {
+      const float p = share[k] / total;
+      share[k] = p;
+      const float log_p = a.labels.teacher[entry + k] * a.labels.inv_temperature - most - log_total;
+      if (!(p == 0.f)) part = fmaf(p, (max_z - logit[k]) + (log_sum + log_p), part);  // an absent entry has p = 0
+    }
+    loss = a.labels.temperature * a.labels.temperature * block_reduce(part, scratch, false);
+  }
+  if (bad) loss = quiet_nan();  // a label outside the vocabulary
+  if (tid == 0) a.row_losses[n] = loss;
+  if (a.g == nullptr) return;
+
+  float scale = a.labels.temperature;
+  if (a.mean) scale /= (float)count;
+  if (a.row_grads != nullptr) scale *= a.row_grads[n];
+  if (a.grad_scale != nullptr) scale *= *a.grad_scale;
+  if (loss != loss) scale = quiet_nan();
+  __syncthreads();  // the tiles' factors and the shares
+  for (int i = tid; i < groups; i += kFinishThreads) {
+    const uint4 e = g[i];
+    const float f = scale * ex2_approx(factor[i / (kTile / 8)]);
+    const uint32_t in[4] = {e.x, e.y, e.z, e.w};
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = Io16<__half>::unpack(in[j]);
+      out[j] = IO::pack(t.x * f, t.y * f);
+    }
+    g[i] = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+  __syncthreads();
+  if (bad) return;
+  for (int k = tid; k < top; k += kFinishThreads) {
+    if (a.labels.teacher != nullptr && a.labels.teacher[entry + k] == -INFINITY) continue;
+    const long long v = a.labels.at(entry + k);
+    float p = 0.f;  // an index may occur more than once: each occurrence writes the same value
+    for (int j = 0; j < top; ++j)
+      if ((a.labels.teacher == nullptr || !(a.labels.teacher[entry + j] == -INFINITY)) && a.labels.at(entry + j) == v)
+        p += share[j];
+    const float q = ex2_approx(logit[k] * 1.4426950408889634f - lse2);
+    reinterpret_cast<bf16*>(g)[v] = IO::store(scale * (q - p));
+  }
+}
+
+// ---- small passes ------------------------------------------------------------------------------------------------------
+// loss = sum of the row losses in a fixed order, over the number of rows that take part where `mean`
+__global__ __launch_bounds__(1024) void sum_losses_kernel(const float* __restrict__ row_losses, const int* __restrict__ count,
+                                                          float* __restrict__ loss, int rows, bool mean) {
+  chain_begin();
+  __shared__ float sums[32];
+  float v = 0.f;
+  for (int i = threadIdx.x; i < rows; i += 1024) v += row_losses[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  v = sums[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int used = *count;
+  if (threadIdx.x == 0) *loss = mean && used > 0 ? v / (float)used : v;  // no row takes part: 0
+}
+
+// out[row_map ? row_map[row_begin + row] : row][c] = sum of the parts in their order
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float4* __restrict__ partials, bf16* __restrict__ out,
+                                                        const int* __restrict__ row_map, const int* __restrict__ count,
+                                                        int row_begin, int part_rows, int pieces, int parts) {
+  chain_begin();
+  const int limit = row_map != nullptr ? *count - row_begin : part_rows;
+  const long long rows = limit < part_rows ? limit : part_rows;
+  const long long total = rows * pieces, stride = (long long)part_rows * pieces * 2;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    for (int s = 0; s < parts; ++s) {
+      const float4 u = __ldg(partials + s * stride + 2 * i), v = __ldg(partials + s * stride + 2 * i + 1);
+      a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+      b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+    }
+    const long long row = i / pieces;
+    const long long to = row_map != nullptr ? (long long)row_map[row_begin + row] * pieces + (i - row * pieces) : i;
+    reinterpret_cast<uint4*>(out)[to] = make_uint4(IO::pack(a.x, a.y), IO::pack(a.z, a.w), IO::pack(b.x, b.y), IO::pack(b.z, b.w));
+  }
+}
+
+// values *= *scale, in place; nothing to do where the scale is one
+__global__ __launch_bounds__(256) void scale_kernel(uint4* __restrict__ values, long long pieces, const float* __restrict__ scale) {
+  chain_begin();
+  const float f = *scale;
+  if (f == 1.f) return;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (long long)gridDim.x * 256) {
+    const uint4 u = values[i];
+    const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = IO::unpack(in[j]);
+      out[j] = IO::pack(t.x * f, t.y * f);
+    }
+    values[i] = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------
+// The workspace of a call; sizes depend on the shapes and on which gradients are wanted, not on the labels.
+struct Layout {
+  long long ldg;
+  int piece_rows, pieces, splits_x, splits_w;
+  bool parts_x, parts_w;
+  size_t position, row_map, count, x_compact, stats, power, partial_x, partial_w, bytes;
+};
+
+size_t take(size_t& at, size_t bytes) {
+  const size_t here = at;
+  at += (bytes + 255) & ~size_t(255);
+  return here;
+}
+
+Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad_weight) {
+  Layout l{};
+  const bool grads = grad_x || grad_weight;
+  l.ldg = ((long long)vocab + 63) / 64 * 64;
+  const long long tiles = (vocab + kTile - 1) / kTile;
+  long long most = kStatsBytes / (8 * tiles);
+  if (grads && kPieceBytes / (2 * l.ldg) < most) most = kPieceBytes / (2 * l.ldg);
+  most = most / kTile * kTile;
+  if (most < kTile) most = kTile;
+  l.pieces = (int)((rows + most - 1) / most);
+  // pieces of equal size, whole tiles each; a single piece is the rows themselves
+  l.piece_rows = l.pieces == 1 ? (int)rows : (int)(((rows + l.pieces - 1) / l.pieces + kTile - 1) / kTile * kTile);
+  l.pieces = (int)((rows + l.piece_rows - 1) / l.piece_rows);
+  l.splits_x = grad_x ? contraction_splits(l.piece_rows, channels, vocab) : 1;
+  l.splits_w = grad_weight ? contraction_splits(vocab, channels, l.piece_rows) : 1;
+  l.parts_x = l.splits_x > 1;
+  l.parts_w = l.splits_w > 1 || l.pieces > 1;
+  size_t at = 0;
+  l.count = take(at, 16);
+  l.position = take(at, rows * 4);
+  l.row_map = take(at, rows * 4);
+  l.x_compact = take(at, (size_t)rows * channels * 2);
+  l.stats = take(at, (size_t)tiles * l.piece_rows * 8);
+  l.power = take(at, grads ? (size_t)l.piece_rows * l.ldg * 2 : 0);
+  l.partial_x = take(at, grad_x && l.parts_x ? (size_t)l.splits_x * l.piece_rows * channels * 4 : 0);
+  l.partial_w = take(at, grad_weight && l.parts_w ? (size_t)l.splits_w * vocab * channels * 4 : 0);
+  l.bytes = at;
+  return l;
+}
+
+bool aligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int check_shape(long long rows, int channels, int vocab) {
+  FRWKV_REQUIRE(rows > 0 && channels > 0 && vocab > 0, "pretrain_head_loss: sizes must be positive");
+  FRWKV_REQUIRE(rows <= (1 << 24), "pretrain_head_loss: at most 16777216 rows");
+  FRWKV_REQUIRE(channels % 8 == 0 && channels <= 65536, "pretrain_head_loss: channels must be a multiple of 8 up to 65536");
+  FRWKV_REQUIRE(vocab <= (1 << 20), "pretrain_head_loss: at most 1048576 vocabulary entries");
+  return FRWKV_OK;
+}
+
+}  // namespace
+}  // namespace head
+}  // namespace frwkv
+
+extern "C" size_t frwkv_pretrain_head_loss_workspace_bytes(long long rows, int channels, int vocab, int grad_x,
+                                                           int grad_weight) {
+  using namespace frwkv;
+  if (head::check_shape(rows, channels, vocab) != FRWKV_OK) return 0;
+  return head::layout_of(rows, channels, vocab, grad_x != 0, grad_weight != 0).bytes;
+}
+
+extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_stream_t stream) {
+  using namespace frwkv;
+  using namespace frwkv::head;
+  clear_error();
+  FRWKV_REQUIRE(args != nullptr, "pretrain_head_loss: null pointer argument");
+  const frwkv_head_loss_args& a = *args;
+  FRWKV_REQUIRE(a.x && a.weight && a.labels && a.row_losses && a.workspace && a.error_flag,
+                "pretrain_head_loss: null pointer argument");
+  if (int rc = check_shape(a.rows, a.channels, a.vocab)) return rc;
+  FRWKV_REQUIRE(a.label_bytes == 4 || a.label_bytes == 8, "pretrain_head_loss: labels must be int32 or int64");
+  FRWKV_REQUIRE(a.top >= 1 && a.top <= kMaxTop, "pretrain_head_loss: 1 to 512 entries per row");
+  FRWKV_REQUIRE(a.teacher_logits != nullptr || a.top == 1, "pretrain_head_loss: one label per row");
+  FRWKV_REQUIRE(a.temperature > 0.f && a.temperature - a.temperature == 0.f && 1.f / a.temperature - 1.f / a.temperature == 0.f,
+                "pretrain_head_loss: temperature must be finite and positive");
+  FRWKV_REQUIRE(a.teacher_logits != nullptr || a.temperature == 1.f, "pretrain_head_loss: labels go with temperature 1");
+  FRWKV_REQUIRE(aligned(a.x, 16) && aligned(a.weight, 16) && aligned(a.grad_x, 16) && aligned(a.grad_weight, 16) &&
+                    aligned(a.workspace, 256) && aligned(a.labels, a.label_bytes) && aligned(a.teacher_logits, 4),
+                "pretrain_head_loss: x, weight and their gradients must be 16-byte aligned, the workspace 256-byte aligned");
+  const bool grads = a.grad_x != nullptr || a.grad_weight != nullptr;
+  const Layout l = layout_of(a.rows, a.channels, a.vocab, a.grad_x != nullptr, a.grad_weight != nullptr);
+  FRWKV_REQUIRE(a.workspace_bytes >= l.bytes,
+                "pretrain_head_loss: workspace is smaller than frwkv_pretrain_head_loss_workspace_bytes");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(a.workspace);
+  int* count = reinterpret_cast<int*>(ws + l.count);
+  int* position = reinterpret_cast<int*>(ws + l.position);
+  int* row_map = reinterpret_cast<int*>(ws + l.row_map);
+  float2* stats = reinterpret_cast<float2*>(ws + l.stats);
+  void* power = grads ? ws + l.power : nullptr;
+  float* partial_x = l.parts_x ? reinterpret_cast<float*>(ws + l.partial_x) : nullptr;
+  float* partial_w = l.parts_w ? reinterpret_cast<float*>(ws + l.partial_w) : nullptr;
+  const int rows = (int)a.rows, x_pieces = a.channels / 8, tiles = (a.vocab + kTile - 1) / kTile;
+
+  Labels labels{};
+  labels.index = a.labels;
+  labels.wide = a.label_bytes == 8;
+  labels.teacher = a.teacher_logits;
+  labels.ignore_index = a.ignore_index;
+  labels.top = a.top;
+  labels.temperature = a.temperature;
+  labels.inv_temperature = 1.f / a.temperature;
+
+  const dim3 by_warp((rows + 7) / 8);
+  if (a.teacher_logits != nullptr) {
+    launch_chained(teacher_rows_kernel, by_warp, dim3(256), 0, s, labels, position, rows);
+    if (int rc = check_launch("teacher_rows_kernel")) return rc;
+  }
+  launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, position, row_map, count, a.error_flag, rows);
+  if (int rc = check_launch("plan_kernel")) return rc;
+  launch_chained(compact_kernel, by_warp, dim3(256), 0, s, static_cast<const uint4*>(a.x), position, count,
+                 reinterpret_cast<uint4*>(ws + l.x_compact), static_cast<uint4*>(a.grad_x), a.row_losses, rows, x_pieces);
+  if (int rc = check_launch("compact_kernel")) return rc;
+
+  const size_t finish_smem = (size_t)(tiles + 2 * a.top) * sizeof(float);
+  for (int piece = 0; piece < l.pieces; ++piece) {
+    const Rows here{count, row_map, rows, piece * l.piece_rows, l.piece_rows};
+    if (int rc = launch_logit_stats(a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab,
+                                    1.4426950408889634f * labels.inv_temperature, stats, l.piece_rows, power, l.ldg,
+                                    a.error_flag, s))
+      return rc;
+    FinishArgs f{};
+    f.rows = here;
+    f.labels = labels;
+    f.x = static_cast<const bf16*>(a.x);
+    f.weight = static_cast<const bf16*>(a.weight);
+    f.stats = stats;
+    f.stats_stride = l.piece_rows;
+    f.vocab = a.vocab;
+    f.channels = a.channels;
+    f.g = static_cast<uint4*>(power);
+    f.ldg = l.ldg;
+    f.mean = a.mean != 0;
+    f.row_grads = a.row_grads;
+    f.grad_scale = a.grad_scale;
+    f.row_losses = a.row_losses;
+    launch_chained(finish_kernel, dim3(l.piece_rows), dim3(kFinishThreads), finish_smem, s, f);
+    if (int rc = check_launch("finish_kernel")) return rc;
+    if (a.grad_x != nullptr) {
+      if (int rc = launch_grad_x(power, l.ldg, a.weight, here, a.channels, a.vocab, l.splits_x, a.grad_x, partial_x,
+                                 a.error_flag, s))
+        return rc;
+      if (l.parts_x) {
+        launch_chained(sum_parts_kernel, dim3(592), dim3(256), 0, s, reinterpret_cast<const float4*>(partial_x),
+                       static_cast<bf16*>(a.grad_x), row_map, count, here.piece_begin, l.piece_rows, x_pieces, l.splits_x);
+        if (int rc = check_launch("sum_parts_kernel")) return rc;
+      }
+    }
+    if (a.grad_weight != nullptr)
+      if (int rc = launch_grad_weight(power, l.ldg, a.x, ws + l.x_compact, here, a.channels, a.vocab, l.splits_w, a.grad_weight,
+                                      partial_w, piece > 0, a.error_flag, s))
+        return rc;
+  }
+  if (a.grad_weight != nullptr && l.parts_w) {
+    launch_chained(sum_parts_kernel, dim3(592), dim3(256), 0, s, reinterpret_cast<const float4*>(partial_w),
+                   static_cast<bf16*>(a.grad_weight), static_cast<const int*>(nullptr), count, 0, a.vocab, x_pieces,
+                   l.splits_w);
+    if (int rc = check_launch("sum_parts_kernel")) return rc;
+  }
+  if (a.loss != nullptr) {
+    launch_chained(sum_losses_kernel, dim3(1), dim3(1024), 0, s, a.row_losses, count, a.loss, rows, a.mean != 0);
+    if (int rc = check_launch("sum_losses_kernel")) return rc;
+  }
+  return FRWKV_OK;
+}
+
+extern "C" int frwkv_scale_bf16(void* values, long long numel, const float* scale, frwkv_stream_t stream) {
+  using namespace frwkv;
+  using namespace frwkv::head;
+  clear_error();
+  FRWKV_REQUIRE(values && scale, "scale_bf16: null pointer argument");
+  FRWKV_REQUIRE(numel > 0 && numel % 8 == 0, "scale_bf16: the number of values must be a positive multiple of 8");
+  FRWKV_REQUIRE(aligned(values, 16), "scale_bf16: values must be 16-byte aligned");
+  const long long pieces = numel / 8, blocks = (pieces + 255) / 256;
+  launch_chained(scale_kernel, dim3((unsigned)(blocks < 1184 ? blocks : 1184)), dim3(256), 0,
+                 reinterpret_cast<cudaStream_t>(stream), static_cast<uint4*>(values), pieces, scale);
+  return check_launch("scale_kernel");
+}

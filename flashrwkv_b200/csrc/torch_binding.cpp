@@ -2057,6 +2057,155 @@ std::tuple<torch::Tensor, torch::Tensor> pretrain_tmix_add_layer_norm(const torc
   return {out[0], out[1]};
 }
 
+// ---- the head's losses for training -------------------------------------------------------------------------------------
+// Labels [N], or [N, K] with a teacher's logits [N, K].
+struct HeadInputs {
+  torch::Tensor x, weight, labels, teacher;
+  int64_t ignore_index = -100;
+  double temperature = 1.0;
+};
+
+struct HeadResult {
+  torch::Tensor row_losses, loss, grad_x, grad_weight;
+};
+
+// One pass: the losses and, where wanted, the gradients of sum_n scale_n loss_n (frwkv_pretrain_head_loss).
+HeadResult head_pass(const HeadInputs& in, bool mean, bool want_x, bool want_weight, const torch::Tensor& row_grads,
+                     const torch::Tensor& grad_scale) {
+  const c10::cuda::CUDAGuard guard(in.x.device());
+  const int64_t channels = in.x.size(-1), rows = in.x.numel() / channels, vocab = in.weight.size(0);
+  const auto f32 = in.x.options().dtype(torch::kFloat32);
+  HeadResult out;
+  out.row_losses = torch::empty({rows}, f32);
+  out.loss = torch::empty({}, f32);
+  if (want_x) out.grad_x = torch::empty_like(in.x);
+  if (want_weight) out.grad_weight = torch::empty_like(in.weight);
+  const size_t bytes = frwkv_pretrain_head_loss_workspace_bytes(rows, static_cast<int>(channels), static_cast<int>(vocab),
+                                                                want_x, want_weight);
+  auto workspace = torch::empty({static_cast<int64_t>(bytes)}, in.x.options().dtype(torch::kUInt8));
+  auto flag = torch::empty({1}, in.x.options().dtype(torch::kInt32));
+  frwkv_head_loss_args a{};
+  a.x = in.x.data_ptr();
+  a.weight = in.weight.data_ptr();
+  a.labels = in.labels.data_ptr();
+  a.teacher_logits = in.teacher.defined() ? in.teacher.data_ptr<float>() : nullptr;
+  a.row_grads = row_grads.defined() ? row_grads.data_ptr<float>() : nullptr;
+  a.grad_scale = grad_scale.defined() ? grad_scale.data_ptr<float>() : nullptr;
+  a.row_losses = out.row_losses.data_ptr<float>();
+  a.loss = out.loss.data_ptr<float>();
+  a.grad_x = want_x ? out.grad_x.data_ptr() : nullptr;
+  a.grad_weight = want_weight ? out.grad_weight.data_ptr() : nullptr;
+  a.workspace = workspace.data_ptr();
+  a.workspace_bytes = bytes;
+  a.error_flag = flag.data_ptr<int>();
+  a.rows = rows;
+  a.ignore_index = in.ignore_index;
+  a.channels = static_cast<int>(channels);
+  a.vocab = static_cast<int>(vocab);
+  a.top = in.teacher.defined() ? static_cast<int>(in.labels.size(-1)) : 1;
+  a.label_bytes = in.labels.scalar_type() == torch::kInt64 ? 8 : 4;
+  a.mean = mean;
+  a.temperature = static_cast<float>(in.temperature);
+  check_rc(frwkv_pretrain_head_loss(&a, current_stream(in.x)));
+  remember_flag("pretrain_head_loss", flag);
+  return out;
+}
+
+// Forward makes the losses and, for a scalar loss, the gradients with them: the product that gives the logits is then done
+// once.  The upstream gradient scales them in place, which uses them up; a second backward pass through the same node makes
+// them anew.  Row losses have an upstream gradient per row, which has to be known first: their backward pass makes both.
+struct HeadLoss : torch::autograd::Function<HeadLoss> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
+                               const torch::Tensor& labels, const std::optional<torch::Tensor>& teacher,
+                               int64_t ignore_index, double temperature, int64_t reduction, bool want_x,
+                               bool want_weight) {
+    const HeadInputs in{x, weight, labels, teacher.value_or(torch::Tensor()), ignore_index, temperature};
+    const bool scalar = reduction != 0;
+    auto r = head_pass(in, reduction == 2, want_x && scalar, want_weight && scalar, torch::Tensor(), torch::Tensor());
+    ctx->save_for_backward({x, weight, labels, in.teacher});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["reduction"] = reduction;
+    if (scalar && (want_x || want_weight)) {
+      ctx->saved_data["grads"] = c10::IValue(std::make_tuple(r.grad_x, r.grad_weight));
+    }
+    return scalar ? r.loss : r.row_losses.view(x.sizes().slice(0, x.dim() - 1));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_second_order();
+    const auto saved = ctx->get_saved_variables();
+    const bool want_x = ctx->needs_input_grad(0), want_weight = ctx->needs_input_grad(1);
+    const int64_t reduction = ctx->saved_data["reduction"].toInt();
+    const auto upstream = grads[0].contiguous();
+    torch::Tensor gx, gw;
+    const auto kept = ctx->saved_data.find("grads");
+    if (kept != ctx->saved_data.end()) {
+      const auto pair = kept->second.toTuple();
+      gx = want_x ? pair->elements()[0].toTensor() : torch::Tensor();
+      gw = want_weight ? pair->elements()[1].toTensor() : torch::Tensor();
+      ctx->saved_data.erase(kept);
+      const c10::cuda::CUDAGuard guard(saved[0].device());
+      for (const auto& t : {gx, gw})
+        if (t.defined())
+          check_rc(frwkv_scale_bf16(t.data_ptr(), t.numel(), upstream.data_ptr<float>(), current_stream(t)));
+    } else {
+      const HeadInputs in{saved[0], saved[1], saved[2], saved[3], ctx->saved_data["ignore_index"].toInt(),
+                          ctx->saved_data["temperature"].toDouble()};
+      const auto r = head_pass(in, reduction == 2, want_x, want_weight, reduction == 0 ? upstream : torch::Tensor(),
+                               reduction == 0 ? torch::Tensor() : upstream);
+      gx = r.grad_x;
+      gw = r.grad_weight;
+    }
+    return {gx, gw, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(),
+            torch::Tensor()};
+  }
+};
+
+void check_head_tensor(const torch::Tensor& t, const char* name, const torch::Tensor& x) {
+  if (!t.is_cuda() || !t.is_contiguous()) throw py::value_error(std::string(name) + " must be CUDA and contiguous");
+  if (t.device() != x.device()) throw py::value_error(std::string(name) + " must share x's device");
+}
+
+torch::Tensor pretrain_head_loss(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& labels,
+                                 const std::optional<torch::Tensor>& teacher, int64_t ignore_index, double temperature,
+                                 int64_t reduction) {
+  check_norm_tensor(x, "x", x);
+  check_norm_tensor(weight, "weight", x);
+  if (x.dim() < 2 || x.numel() == 0) throw py::value_error("x must have non-empty shape [...,C]");
+  if (x.size(-1) % 8 || x.size(-1) > 65536) throw py::value_error("C must be a multiple of 8 up to 65536");
+  if (x.numel() / x.size(-1) > (1 << 24)) throw py::value_error("at most 16777216 rows");
+  if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) != x.size(-1))
+    throw py::value_error("weight must have shape [V,C]");
+  if (weight.size(0) > (1 << 20)) throw py::value_error("at most 1048576 vocabulary entries");
+  const char* label_name = teacher.has_value() ? "teacher_indices" : "targets";
+  check_head_tensor(labels, label_name, x);
+  if (labels.scalar_type() != torch::kInt64 && labels.scalar_type() != torch::kInt32)
+    throw py::value_error(std::string(label_name) + " must be int32 or int64");
+  const auto rows = x.sizes().slice(0, x.dim() - 1);
+  std::optional<torch::Tensor> logits;
+  if (teacher.has_value()) {
+    check_head_tensor(*teacher, "teacher_logits", x);
+    if (!teacher->is_floating_point() || teacher->scalar_type() == torch::kFloat64)
+      throw py::value_error("teacher_logits must be float32, float16 or bfloat16");
+    if (teacher->dim() != x.dim() || teacher->sizes().slice(0, x.dim() - 1) != rows || teacher->size(-1) < 1 ||
+        teacher->size(-1) > 512)
+      throw py::value_error("teacher_logits must have shape [...,K], K from 1 to 512, with x's leading shape");
+    if (labels.sizes() != teacher->sizes()) throw py::value_error("teacher_indices must have teacher_logits' shape");
+    if (teacher->requires_grad() && at::GradMode::is_enabled())
+      throw py::value_error("teacher_logits must not require a gradient");
+    const float t = static_cast<float>(temperature);
+    if (!(t > 0.f) || !std::isfinite(t) || !std::isfinite(1.f / t)) throw py::value_error("temperature must be positive");
+    const c10::cuda::CUDAGuard guard(x.device());
+    logits = teacher->to(torch::kFloat32);
+  } else if (labels.sizes() != rows) {
+    throw py::value_error("targets must have x's leading shape");
+  }
+  const bool grad = at::GradMode::is_enabled();
+  return HeadLoss::apply(x, weight, labels, logits, ignore_index, temperature, reduction, grad && x.requires_grad(),
+                         grad && weight.requires_grad());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -2195,6 +2344,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("eps"));
   m.def("pretrain_tmix_add_layer_norm", &pretrain_tmix_add_layer_norm, py::arg("x"), py::arg("residual"),
         py::arg("weight"), py::arg("bias"), py::arg("eps"));
+  m.def("pretrain_head_loss", &pretrain_head_loss, py::arg("x"), py::arg("weight"), py::arg("labels"), py::arg("teacher"),
+        py::arg("ignore_index"), py::arg("temperature"), py::arg("reduction"));
   m.def("recurrent_add_vec_forward_varlen", &recurrent_add_vec_forward_varlen, py::arg("x"), py::arg("vec"));
   m.def("tmix_act_forward", &tmix_act_forward, py::arg("x"), py::arg("act"));
   m.def("tmix_linear_runtime_layout", &linear_runtime_layout, py::arg("x"), py::arg("weight_kn"), py::arg("act") = 0,

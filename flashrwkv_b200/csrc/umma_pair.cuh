@@ -1,0 +1,110 @@
+// Thin inline-PTX layer for tensor-core products by a pair of CTAs (a cluster of two, cta_group::2), beside umma.cuh:
+// tensor memory, MMA, commit to both CTAs' barriers, TMA loads that count on the leader's barrier, and the cluster
+// barrier.  The leader is the CTA of rank 0; the pair's tile has 256 rows, of which each CTA's tensor memory holds its own
+// 128, and each CTA's shared memory holds its own 128 rows of A and its own half of B.
+#pragma once
+
+#include <cuda.h>
+
+#include "umma.cuh"
+
+namespace frwkv {
+namespace umma2 {
+
+using umma::smem_u32;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of the same shared-memory object in the leader CTA
+__device__ __forceinline__ uint32_t in_leader(const void* p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(0u));
+  return r;
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t* smem_result, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+// D[tmem of both CTAs] (+)= A * B over K = 16; one thread of the leader issues it
+__device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// all MMAs issued so far arrive on this barrier in both CTAs when they complete
+__device__ __forceinline__ void commit_both(uint64_t* mbar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(mbar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// A tile into this CTA's shared memory, its bytes counted on `mbar` (a cluster address: the leader's barrier)
+__device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_dst),
+      "l"(map), "r"(x), "r"(y), "r"(mbar)
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t mbar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
+}
+// bounded wait on a barrier of this CTA that the other CTA's threads arrive on
+__device__ __forceinline__ bool wait_cluster(uint64_t* mbar, uint32_t parity, uint32_t limit = (1u << 22)) {
+  for (uint32_t i = 0; i < limit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(mbar)), "r"(parity)
+        : "memory");
+    if (done != 0) return true;
+  }
+  return false;
+}
+
+// Shared-memory descriptors of the two 16-bit operand forms that TMA writes with 128-byte swizzle: rows of 64 contraction
+// values ("K-major": eight rows are 1024 bytes), or rows that run along the other axis and are indexed by the contraction
+// ("MN-major": boxes of 64 columns x 64 rows, 8192 bytes apart).
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+  return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
+  return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(8192 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+// bf16 operands, fp32 accumulator, 256 x 256; bits 15 / 16: A / B is MN-major
+__host__ __device__ constexpr uint32_t idesc_bf16_256(bool a_mn, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(256 >> 3) << 17) |
+         (uint32_t(256 >> 4) << 24);
+}
+
+}  // namespace umma2
+}  // namespace frwkv

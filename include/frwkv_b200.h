@@ -599,6 +599,48 @@ int frwkv_pretrain_layer_norm_backward(const void* grad_out, const void* grad_su
                                        void* grad_bias, float* workspace, long long workspace_floats, long long rows,
                                        int channels, frwkv_stream_t stream);
 
+/*
+ * The head's losses for training: z = x weight^T / temperature, softmax over the vocabulary, a loss per row and, where
+ * wanted, the gradients of x and weight, without keeping the logits.
+ *   teacher_logits NULL: labels [rows], loss_n = log sum exp z_n - z_n[label]; rows whose label is ignore_index take no part.
+ *   teacher_logits fp32 [rows][top], labels [rows][top]: loss_n = temperature^2 KL(p || softmax(z_n)), p = the softmax of
+ *   teacher_logits / temperature over the entries that are not -inf; rows without an entry take no part.
+ * A row that takes no part has loss 0 and a zero gradient, and what x holds there reaches nothing.  A label outside
+ * [0, vocab) gives its row a NaN loss and NaN gradients (no out-of-range access).
+ * row_losses receives every row's loss, loss (may be NULL) their sum, or with `mean` the sum over the number of rows that
+ * take part (0 where there is none).  grad_x / grad_weight (either may be NULL) are those of
+ *   sum_n (mean ? 1 / rows that take part : 1) * (row_grads ? row_grads[n] : 1) * (grad_scale ? *grad_scale : 1) * loss_n.
+ * channels a multiple of 8 up to 65536, vocab up to 2^20, top up to 512, rows up to 2^24; x, weight and the gradients are
+ * bf16, contiguous and 16-byte aligned.  error_flag: one device word, set to 0 and made non-zero if a bounded wait of a
+ * matrix product runs out (outputs are NaN then).  workspace: frwkv_pretrain_head_loss_workspace_bytes bytes, 256-byte
+ * aligned; calls that may overlap need one each.
+ */
+typedef struct {
+  const void* x;               /* bf16 [rows][channels] */
+  const void* weight;          /* bf16 [vocab][channels] */
+  const void* labels;          /* int32 or int64 [rows][top] */
+  const float* teacher_logits; /* [rows][top], or NULL */
+  const float* row_grads;      /* [rows], or NULL */
+  const float* grad_scale;     /* one value, or NULL */
+  float* row_losses;           /* [rows] */
+  float* loss;                 /* one value, or NULL */
+  void* grad_x;                /* bf16 [rows][channels], or NULL */
+  void* grad_weight;           /* bf16 [vocab][channels], or NULL */
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* error_flag;
+  long long rows;
+  long long ignore_index;
+  int channels, vocab, top;
+  int label_bytes;             /* 4 or 8 */
+  int mean;
+  float temperature;           /* 1 without a teacher */
+} frwkv_head_loss_args;
+size_t frwkv_pretrain_head_loss_workspace_bytes(long long rows, int channels, int vocab, int grad_x, int grad_weight);
+int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_stream_t stream);
+/* values (bf16, numel a multiple of 8, 16-byte aligned) *= *scale (a device value) in place. */
+int frwkv_scale_bf16(void* values, long long numel, const float* scale, frwkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,396 @@
+"""The head's losses (cross entropy, distillation) and their gradients against the float64 oracle.
+
+Bounds, with u = 2^-24 and rho = eps(bf16) / 2 = 2^-8.  A logit is an fp32 sum of C exact products; for any order of
+addition, and one unit per addition rather than half (tensor cores may truncate), it is within delta_n = 2 C u B_n / T of its
+value, B_n = max_v sum_c |x_nc w_vc|.  The normaliser sums 256 positive terms per tile, then the tiles: relative error
+<= (256 + tiles + 16) u, each exponential 2^-21.  So with zmax_n = max |z_n|:
+    |loss error| <= T^2 (2 delta_n + (300 + tiles) u + 2^-20 + 32 u (zmax_n + |loss|))  =: T^2 e_n
+A logit gradient g = scale T (q - p) has q's relative error e_n plus that of the fp16 exponential (2^-11, or 2^-24 of the
+tile's maximum where it is subnormal), and its own rounding rho |g|:
+    gerr = rho |g| + scale T (q (2 e_n + 2^-10) + 2^-23 q_tilemax + 4 u)
+dx = g W is then within gerr |W| + V 2 u (|g| |W|) + rho |dx| and dW within gerr^T |x| + N 2 u (|g|^T |x|) + rho |dW|.  These
+hold for every element.  Roundings are independent, so in the Frobenius norm the two of them (g, result) stay below
+sqrt(2) rho / sqrt(3) = 3.2e-3 of sqrt(|result|^2 + sum g^2 w^2); 4e-3 is asked for.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+RHO = torch.finfo(torch.bfloat16).eps / 2
+
+
+def _rows(N, C, V, seed, sure=True):
+    gen = torch.Generator().manual_seed(seed)
+    w = (torch.randn(V, C, generator=gen) * 2 / C ** 0.5).to(torch.bfloat16)
+    t = torch.randint(V, (N,), generator=gen)
+    x = torch.randn(N, C, generator=gen)
+    if sure:
+        x = x + 2 * torch.rand(N, 1, generator=gen) * w[t].float()
+    return x.to(torch.bfloat16).cuda(), w.cuda(), t.cuda(), gen
+
+
+def _reference(x, w, labels, shares, T, row_grads):
+    """Losses, gradients and the bounds above, in pieces of the rows."""
+    N, C = x.shape
+    V = w.shape[0]
+    xd, wd = x.double(), w.double()
+    aw = wd.abs()
+    out = {k: [] for k in ("loss", "eloss", "dx", "edx", "fx")}
+    dw, edw = torch.zeros_like(wd), torch.zeros_like(wd)
+    fw = 0.0
+    tiles = -(-V // 256)
+    step = max(1, 2 ** 26 // V)
+    for lo in range(0, N, step):
+        s = slice(lo, min(N, lo + step))
+        used = (shares[s].sum(1) > 0).double()[:, None]
+        z = xd[s] @ wd.T / T
+        B = (xd[s].abs() @ aw.T).amax(1)
+        lq = torch.log_softmax(z, 1)
+        lab = torch.where(shares[s] > 0, labels[s].long(), 0)
+        loss = T * T * (torch.special.xlogy(shares[s], shares[s]) - shares[s] * lq.gather(1, lab)).sum(1)
+        e = 2 * (2 * C * U * B / T) + (300 + tiles) * U + 2 ** -20 + 32 * U * (z.abs().amax(1) + loss.abs() / T / T)
+        out["loss"].append(loss)
+        out["eloss"].append(T * T * e * used[:, 0])
+        q = lq.exp()
+        g = q.clone().scatter_add_(1, lab, -shares[s])
+        sc = (T * row_grads[s].double().abs())[:, None] * used
+        g = g * T * row_grads[s].double()[:, None] * used
+        pad = torch.zeros(q.shape[0], tiles * 256 - V, dtype=q.dtype, device=q.device)
+        top = torch.cat((q, pad), 1).view(-1, tiles, 256).amax(2).repeat_interleave(256, 1)[:, :V]
+        gerr = RHO * g.abs() + sc * (q * (2 * e[:, None] + 2 ** -10) + 2 ** -23 * top + 4 * U)
+        dx = g @ wd
+        out["dx"].append(dx)
+        out["edx"].append(gerr @ aw + 2 * V * U * (g.abs() @ aw) + RHO * dx.abs() * 1.01)
+        out["fx"].append((dx ** 2).sum() + ((g ** 2) @ (wd ** 2)).sum())
+        dw += g.T @ xd[s]
+        edw += gerr.T @ xd[s].abs() + 2 * N * U * (g.abs().T @ xd[s].abs())
+        fw = fw + ((g ** 2).T @ (xd[s] ** 2)).sum()
+    res = {k: torch.cat(v) for k, v in out.items() if k != "fx"}
+    res.update(dw=dw, edw=edw + RHO * dw.abs() * 1.01, fx=sum(out["fx"]), fw=fw + (dw ** 2).sum())
+    return res
+
+
+def _near(got, want, bound, name):
+    got = got.double()
+    assert torch.isfinite(got).all(), name
+    over = (got - want).abs() - bound
+    assert float(over.max()) <= 1e-30, f"{name}: {float(over.max())} beyond the bound"
+
+
+def _check_grads(dx, dw, r):
+    for got, want, bound, norm, name in ((dx, r["dx"], r["edx"], r["fx"], "d x"), (dw, r["dw"], r["edw"], r["fw"], "d weight")):
+        if got is not None:
+            _near(got, want, bound, name)
+            assert float((got.double() - want).norm()) <= 4e-3 * float(norm) ** 0.5 + 1e-30, name
+
+
+# rows, channels, vocabulary: one of each; tiles of 256 with their edges; several row and vocabulary tiles; odd vocabularies
+SHAPES = [(1, 8, 1), (1, 8, 5), (3, 64, 257), (16, 40, 255), (64, 512, 8191), (130, 72, 1000), (256, 64, 256), (257, 264, 511),
+          (300, 1032, 3001), (513, 128, 769), (1000, 2048, 777), (33, 2048, 20011), (2000, 64, 300)]
+
+
+@pytest.mark.parametrize("N,C,V", SHAPES)
+def test_cross_entropy(N, C, V):
+    import flashrwkv_b200 as F
+
+    x, w, t, gen = _rows(N, C, V, N + C + V)
+    if N > 4:
+        t[::5] = -100
+    used = t != -100
+    shares = used.double()[:, None]
+    x.requires_grad_(), w.requires_grad_()
+    rows = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    count = int(used.sum())
+    r = _reference(x.detach(), w.detach(), t[:, None], shares, 1.0, torch.full((N,), 1.0 / max(count, 1), device="cuda"))
+    _near(rows.detach(), r["loss"], r["eloss"], "row losses")
+    assert bool((rows[~used] == 0).all())
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    assert abs(float(loss.detach()) - float(r["loss"].sum() / count)) <= float(r["eloss"].sum() / count) + (N + 4) * U * float(
+        r["loss"].sum() / count)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    _check_grads(dx, dw, r)
+    assert bool((dx[~used] == 0).all())
+    # row losses with an upstream gradient per row
+    up = torch.randn(N, generator=gen).cuda()
+    dx, dw = torch.autograd.grad(rows, (x, w), up)
+    _check_grads(dx, dw, _reference(x.detach(), w.detach(), t[:, None], shares, 1.0, up))
+
+
+def _teacher(N, K, V, gen, missing=True):
+    idx = torch.stack([torch.randperm(max(V, K), generator=gen)[:K] % V for _ in range(N)]).cuda()
+    logits = (torch.randn(N, K, generator=gen) * 3).cuda()
+    if missing and N > 2:
+        logits[torch.rand(N, K, generator=gen).cuda() < 0.3] = float("-inf")
+        logits[1] = float("-inf")
+    return logits, idx
+
+
+@pytest.mark.parametrize("N,C,V,K,T", [(1, 8, 3, 1, 1.0), (5, 64, 257, 7, 2.0), (33, 512, 8191, 8, 1.0), (130, 72, 1000, 64, 4.0),
+                                       (300, 264, 3001, 300, 1.5), (40, 1032, 600, 512, 0.5), (64, 64, 20, 40, 1.0)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_distill(N, C, V, K, T, wide):
+    """K = 40 of 20 names every token twice; K beyond 256 is more than a CTA's threads."""
+    import flashrwkv_b200 as F
+    from oracle import head_norm_oracle as O
+
+    x, w, _, gen = _rows(N, C, V, N + C + V + K, sure=False)
+    logits, idx = _teacher(N, K, V, gen)
+    shares, used = O.teacher_shares(logits, T)
+    idx = torch.where(logits == float("-inf"), torch.full_like(idx, -7), idx)  # the index of an absent entry is not looked at
+    idx = idx if wide else idx.to(torch.int32)
+    x.requires_grad_(), w.requires_grad_()
+    count = int(used.sum())
+    loss = F.pretrain_head_distill_bf16(x, w, logits, idx, temperature=T)
+    r = _reference(x.detach(), w.detach(), idx, shares, T, torch.full((N,), 1.0 / count, device="cuda"))
+    want = float(r["loss"].sum() / count)
+    # the shares' own fp32 error: (K + 8) u of each, times log p - log q, of which a few tens at most
+    share_error = T * T * (K + 8) * U * 64
+    assert abs(float(loss.detach()) - want) <= float(r["eloss"].sum() / count) + share_error + N * U * abs(want)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    _check_grads(dx, dw, r)
+    rows = F.pretrain_head_distill_bf16(x, w, logits, idx, temperature=T, reduction="none")
+    _near(rows.detach(), r["loss"], r["eloss"] + share_error, "row losses")
+    assert bool((rows[~used] == 0).all()) and bool((dx[~used] == 0).all())
+    total = F.pretrain_head_distill_bf16(x, w, logits, idx, temperature=T, reduction="sum")
+    assert abs(float(total) - float(rows.double().sum())) <= (N + 4) * U * float(rows.double().abs().sum())
+
+
+def test_distill_from_one_certain_entry_is_cross_entropy():
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(70, 128, 900, 4)
+    x.requires_grad_(), w.requires_grad_()
+    a = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    b = F.pretrain_head_distill_bf16(x, w, torch.zeros(70, 1, device="cuda"), t[:, None])
+    for g, h in zip((a, *torch.autograd.grad(a, (x, w))), (b, *torch.autograd.grad(b, (x, w)))):
+        assert torch.equal(g, h)
+
+
+def test_more_rows_than_one_piece_holds():
+    """2^20 vocabulary entries leave 512 rows to a piece of the exponentials."""
+    import flashrwkv_b200 as F
+
+    N, C, V = 700, 32, 1 << 20
+    x, w, t, _ = _rows(N, C, V, 8)
+    t[3:60] = -100
+    used = t != -100
+    x.requires_grad_(), w.requires_grad_()
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    r = _reference(x.detach(), w.detach(), t[:, None], used.double()[:, None], 1.0, torch.ones(N, device="cuda"))
+    assert abs(float(loss) - float(r["loss"].sum())) <= float(r["eloss"].sum()) + N * U * float(r["loss"].sum())
+    _check_grads(dx, dw, r)
+
+
+def test_rows_that_take_no_part_reach_nothing():
+    """NaN and infinities where no label is; and a batch without any label."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(200, 136, 1500, 5)
+    t[10:90] = -100
+    clean = x.clone()
+    x[10:50] = float("nan")
+    x[50:90, ::3] = float("inf")
+    w.requires_grad_()
+    outs = []
+    for rows in (x, clean):
+        rows = rows.requires_grad_()
+        loss = F.pretrain_head_cross_entropy_bf16(rows, w, t)
+        outs.append((loss.detach(), *torch.autograd.grad(loss, (rows, w))))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    kept = [r for r in range(200) if not 10 <= r < 90]
+    few = clean.detach()[kept].contiguous().requires_grad_()
+    loss = F.pretrain_head_cross_entropy_bf16(few, w, t[kept].contiguous())
+    dx, dw = torch.autograd.grad(loss, (few, w))
+    # the same row losses and products, added in the order of another batch size: N u of the loss, one rounding of a gradient
+    assert abs(float(outs[0][0]) - float(loss.detach())) <= 200 * U * float(loss.detach())
+    for a, b in ((outs[0][1][kept], dx), (outs[0][2], dw)):
+        assert float((a.double() - b.double()).norm()) <= RHO * float(b.double().norm())
+    none = torch.full_like(t, -100)
+    for reduction in ("mean", "sum"):
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, none, reduction=reduction)
+        dx, dw = torch.autograd.grad(loss, (x, w))
+        assert float(loss) == 0 and bool((dx == 0).all()) and bool((dw == 0).all())
+    gone = torch.full((200, 3), float("-inf"), device="cuda")
+    loss = F.pretrain_head_distill_bf16(x, w, gone, torch.zeros(200, 3, dtype=torch.int32, device="cuda"))
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert float(loss) == 0 and bool((dx == 0).all()) and bool((dw == 0).all())
+
+
+def test_labels_outside_the_vocabulary_are_nan_and_stay_in_bounds():
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(40, 64, 300, 6)
+    want = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    bad = t.clone()
+    bad[3], bad[17], bad[30] = 300, -1, 2 ** 40
+    x.requires_grad_(), w.requires_grad_()
+    rows = F.pretrain_head_cross_entropy_bf16(x, w, bad, reduction="none")
+    hit = torch.zeros(40, dtype=torch.bool, device="cuda")
+    hit[[3, 17, 30]] = True
+    assert torch.isnan(rows[hit]).all() and torch.equal(rows[~hit].detach(), want[~hit])
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, bad)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert torch.isnan(loss) and torch.isnan(dx[hit]).all() and torch.isfinite(dx[~hit]).all() and torch.isnan(dw).all()
+    # another ignore_index, negative or a token
+    assert float(F.pretrain_head_cross_entropy_bf16(x, w, torch.full_like(t, 7), ignore_index=7)) == 0
+    assert torch.isnan(F.pretrain_head_cross_entropy_bf16(x, w, torch.full_like(t, -100), ignore_index=-1))
+    # values that are not finite in a row that takes part
+    y = x.detach().clone()
+    y[5, 2] = float("nan")
+    rows = F.pretrain_head_cross_entropy_bf16(y, w, t, reduction="none")
+    assert torch.isnan(rows[5]) and torch.equal(torch.cat((rows[:5], rows[6:])), torch.cat((want[:5], want[6:])))
+
+
+def test_teacher_values_that_are_not_numbers():
+    import flashrwkv_b200 as F
+
+    x, w, _, gen = _rows(12, 64, 300, 7)
+    logits, idx = _teacher(12, 5, 300, gen, missing=False)
+    want = F.pretrain_head_distill_bf16(x, w, logits, idx, reduction="none")
+    logits[2, 1] = float("nan")
+    logits[4, 0] = float("inf")
+    idx[6, 3] = 300
+    rows = F.pretrain_head_distill_bf16(x, w, logits, idx, reduction="none")
+    hit = torch.zeros(12, dtype=torch.bool, device="cuda")
+    hit[[2, 4, 6]] = True
+    assert torch.isnan(rows[hit]).all() and torch.equal(rows[~hit], want[~hit])
+
+
+def test_upstream_gradients_and_repeated_backward_passes():
+    """A scalar upstream gradient scales (one more bf16 rounding unless it is a power of two); a second pass over a retained
+    graph makes the same gradients again; only what is asked for is made."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(90, 136, 700, 9)
+    x.requires_grad_(), w.requires_grad_()
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    one = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    kept = [g.clone() for g in one]
+    again = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    quarter = torch.autograd.grad(loss, (x, w), torch.tensor(0.25, device="cuda"))
+    for a, b, c, k in zip(one, again, quarter, kept):
+        assert torch.equal(a, k) and torch.equal(b, k) and torch.equal(c, 0.25 * k)
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    scaled = torch.autograd.grad(3.0 * loss, (x, w))
+    for a, k in zip(scaled, kept):
+        assert bool(((a.double() - 3.0 * k.double()).abs() <= RHO * 3.0 * k.double().abs()).all())
+    for leaf, want in ((x, kept[0]), (w, kept[1])):
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+        assert torch.equal(torch.autograd.grad(loss, leaf)[0], want)
+    assert torch.equal(torch.autograd.grad(F.pretrain_head_cross_entropy_bf16(x, w.detach(), t), x)[0], kept[0])
+    assert torch.equal(torch.autograd.grad(F.pretrain_head_cross_entropy_bf16(x.detach(), w, t), w)[0], kept[1])
+    with torch.no_grad():
+        assert not F.pretrain_head_cross_entropy_bf16(x, w, t).requires_grad
+    with pytest.raises(RuntimeError, match="not itself differentiable"):
+        torch.autograd.grad(F.pretrain_head_cross_entropy_bf16(x, w, t), x, create_graph=True)
+
+
+def test_same_bits_every_time_on_any_stream_and_in_graphs():
+    """Two captured graphs at once, and eager calls between their replays."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(300, 264, 2100, 10)
+    t[::7] = -100
+    x.requires_grad_(), w.requires_grad_()
+    up = torch.tensor(2.0, device="cuda")
+
+    def step():
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w), up))
+
+    want = [v.clone() for v in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = [v.clone() for v in step()]
+    side.synchronize()
+    for a, b in zip(want, again):
+        assert torch.equal(a, b)
+    graphs, held = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(step())
+        graphs.append(g)
+    for k in (0, 1, 0):
+        for v in held[k]:
+            v.fill_(5.0)
+        graphs[k].replay()
+        step()
+        torch.cuda.synchronize()
+        for a, b in zip(want, held[k]):
+            assert torch.equal(a, b)
+    with torch.no_grad():  # other labels, other rows that take part
+        t.copy_(t.roll(3))
+        t[:40] = -100
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    for a, b in zip(step(), held[1]):
+        assert torch.equal(a, b)
+
+
+def test_leading_shape_label_types_and_refusals():
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(60, 64, 300, 11)
+    want = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    got = F.pretrain_head_cross_entropy_bf16(x.view(3, 20, 64), w, t.view(3, 20).to(torch.int32), reduction="none")
+    assert got.shape == (3, 20) and torch.equal(got.flatten(), want)
+    half = torch.randn(60, 4, device="cuda").half()
+    idx = torch.randint(300, (60, 4), device="cuda")
+    assert torch.equal(F.pretrain_head_distill_bf16(x, w, half, idx), F.pretrain_head_distill_bf16(x, w, half.float(), idx))
+    shifted = torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view_as(x)
+    for args, message in (((shifted, w, t), "16-byte aligned"), ((x.float(), w, t), "bfloat16"), ((x, w.half(), t), "bfloat16"),
+                          ((x, w[:, :32].contiguous(), t), "weight must have shape"), ((x[:, ::2], w, t), "contiguous"),
+                          ((x, w, t[:5]), "leading shape"), ((x, w, t.float()), "int32 or int64"), ((x, w, t.cpu()), "CUDA"),
+                          ((x, w, t.repeat_interleave(2)[::2]), "contiguous"), ((x[:0], w, t[:0]), "non-empty"),
+                          ((x, w[:0], t), "weight must have shape"), ((x[:, :4].contiguous(), w[:, :4].contiguous(), t), "multiple of 8")):
+        with pytest.raises(ValueError, match=message):
+            F.pretrain_head_cross_entropy_bf16(*args)
+    logits = torch.randn(60, 4, device="cuda")
+    for args, message in (((logits[:5], idx), "leading shape"), ((logits, idx[:, :3].contiguous()), "teacher_logits' shape"),
+                          ((logits.double(), idx), "float32, float16 or bfloat16"), ((logits, idx.float()), "int32 or int64"),
+                          ((torch.zeros(60, 513, device="cuda"), torch.zeros(60, 513, dtype=torch.int32, device="cuda")), "K from 1 to 512"),
+                          ((logits.clone().requires_grad_(), idx), "must not require"), ((logits.t().contiguous().t(), idx), "contiguous")):
+        with pytest.raises(ValueError, match=message):
+            F.pretrain_head_distill_bf16(x, w, *args)
+    for temperature in (0.0, -1.0, float("nan"), float("inf"), 1e-60, True):
+        with pytest.raises(ValueError, match="temperature must be positive"):
+            F.pretrain_head_distill_bf16(x, w, logits, idx, temperature=temperature)
+    with pytest.raises(ValueError, match="reduction"):
+        F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="batchmean")
+
+
+def test_the_end_of_a_training_step():
+    """Residual stream -> add + norm -> head loss, as a training step runs them; the gradients reach the residual stream, the
+    norm's parameters and the head.  Three bf16 tensors lie between the loss and the residual stream (normalised rows, their
+    gradient, the result): each adds at most rho of its value, so 3 rho in the Frobenius norm (and the oracle takes the
+    normalised rows as the operator returned them)."""
+    import flashrwkv_b200 as F
+    from oracle import head_norm_oracle as O
+
+    gen = torch.Generator().manual_seed(12)
+    N, C, V = 150, 264, 1300
+
+    def rn(*shape, s=1.0, m=0.0):
+        return (torch.randn(*shape, generator=gen) * s + m).to(torch.bfloat16).cuda().requires_grad_()
+
+    x, r, nw, nb, w = rn(2, 75, C), rn(2, 75, C), rn(C, s=0.2, m=1.0), rn(C, s=0.1), rn(V, C, s=2 / C ** 0.5)
+    t = torch.randint(V, (2, 75), generator=gen).cuda()
+    t[0, :20] = -100
+    total, rows = F.pretrain_tmix_add_layer_norm_bf16(x, r, nw, nb)
+    ce = F.pretrain_head_cross_entropy_bf16(rows, w, t)
+    logits, idx = _teacher(N, 16, V, gen)
+    kd = F.pretrain_head_distill_bf16(rows, w, logits.view(2, 75, 16), idx.view(2, 75, 16), temperature=2.0)
+    got = torch.autograd.grad(ce + 0.5 * kd, (x, r, nw, nb, w))
+    flat, used = rows.detach().view(N, C), (t.flatten() != -100)
+    d1, w1 = O.head_backward(used / used.sum(), flat, w.detach(), t.view(N, 1), used.double()[:, None])
+    shares, there = O.teacher_shares(logits, 2.0)
+    d2, w2 = O.head_backward(0.5 * there / there.sum(), flat, w.detach(), idx, shares, 2.0)
+    ds, dnw, dnb = O.layer_norm_backward((d1 + d2).view(2, 75, C), total.detach(), nw.detach(), 1e-5)
+    for g, want, name in zip(got, (ds, ds, dnw, dnb, w1 + w2), ("x", "residual", "norm weight", "norm bias", "head")):
+        assert float((g.double() - want).norm()) <= 3 * RHO * float(want.norm()), name
