@@ -365,6 +365,25 @@ def test_leading_shape_label_types_and_refusals():
         F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="batchmean")
 
 
+@pytest.mark.parametrize("C", [256, 1024, 2048, 4096])
+def test_logits_carry_no_mean_error(C):
+    """With one vocabulary entry a row's loss is its logit's error (the normaliser is the tensor core's logit, the label's an
+    fp32 dot product).  An accumulator that truncates each of its C / 16 additions loses up to one unit, 2^-23 of a sum that
+    is half of the result on average: C / 16 * 2^-24 of the logit at most.  A tenth of that is allowed to the mean over 40000
+    logits, which the random part (3e-7 of each) moves by 1.5e-9; the scale itself is an fp32 number, 2^-24."""
+    import flashrwkv_b200 as F
+
+    gen = torch.Generator().manual_seed(C)
+    w = (torch.randn(1, C, generator=gen) * 2 / C ** 0.5).to(torch.bfloat16).cuda()
+    x = torch.randn(40000, C, generator=gen).cuda() + (2 + 6 * torch.rand(40000, 1, generator=gen)).cuda() * w.float()
+    x = x.to(torch.bfloat16)
+    z = (x.double() @ w.double().T)[:, 0]
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, torch.zeros(40000, dtype=torch.int64, device="cuda"), reduction="none")
+    big = z.abs() > 6
+    assert int(big.sum()) > 20000
+    assert abs(float((loss.double() / z)[big].mean())) <= 0.1 * C / 16 * 2.0 ** -24 + 2.0 ** -24
+
+
 def test_the_end_of_a_training_step():
     """Residual stream -> add + norm -> head loss, as a training step runs them; the gradients reach the residual stream, the
     norm's parameters and the head.  Three bf16 tensors lie between the loss and the residual stream (normalised rows, their
