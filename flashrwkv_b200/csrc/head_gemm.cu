@@ -1,6 +1,6 @@
 // The three matrix products of the head's losses on the 5th-generation tensor cores:
 //
-//   statistics    z = x W^T                 per 256 columns: row maximum and sum of exponentials (and the exponentials)
+//   statistics    z = x W^T                 per 128 columns: row maximum and sum of exponentials (and the exponentials)
 //   grad_x        dx = g W                  contraction over the vocabulary
 //   grad_weight   dW = g^T x                contraction over the rows
 //
@@ -11,7 +11,7 @@
 //               the leader's barrier
 //   warp 1      (leader) MMA issuer: four tcgen05.mma per stage into one of two accumulators in tensor memory; commits
 //               release the stage, and hand over the accumulator, in both CTAs
-//   warps 2..5  epilogue of the other accumulator meanwhile
+//   warps 2..9  epilogue of the other accumulator meanwhile: a warp takes 32 rows and 128 columns
 // All three operand layouts are read where they lie: x and W are K-major in z = x W^T; W in g W, and both g and x in g^T x,
 // are MN-major (the contraction index numbers the rows of the matrix in memory).  The number of rows that take part is known
 // on the device only (labels may be missing), so the kernels read it there.
@@ -33,7 +33,8 @@ constexpr uint32_t kOperandBytes = kHalf * kBK * 2;  // 16 KB of each operand pe
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr int kStages = 6;
 constexpr uint32_t kSmem = kStages * kStageBytes + 1024;  // + slack to align the tiles to 1024 bytes
-constexpr int kThreads = 192;
+constexpr int kEpilogueWarps = 8;  // two per quarter of the tensor-memory lanes, half of the columns each
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 constexpr uint32_t kTmemCols = 2 * kTile;
 
 enum Product { kStats, kGradX, kGradWeight };
@@ -114,7 +115,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
     }
     for (int i = 0; i < 2; ++i) {
       umma::mbar_init(&acc_full[i], 1);   // a commit
-      umma::mbar_init(&acc_empty[i], 8);  // the epilogue warps of both CTAs
+      umma::mbar_init(&acc_empty[i], 2 * kEpilogueWarps);  // those of both CTAs
     }
     umma::mbar_fence_init();
   }
@@ -198,7 +199,8 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
     }
   } else {
     const uint32_t quarter = warp & 3u;  // the tensor-memory lanes this warp may read: 32 * (warp % 4) ..
-    const uint32_t lanes = (32u * quarter) << 16;
+    const int column0 = (warp - 2) / 4 * kStatsTile;
+    const uint32_t source0 = tmem + ((32u * quarter) << 16) + column0;
     const int row_in_tile = (int)rank * kHalf + 32 * (int)quarter + lane;
     const int m_end = P == kGradWeight ? prm.vocab : rows_here;
     uint32_t t = 0;
@@ -211,69 +213,82 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
       // later ones read as NaN.
       if (ok && !empty && !__all_sync(0xffffffffu, umma2::wait_cluster(&acc_full[acc], aph))) ok = false;
       umma::fence_after_sync();
-      const uint32_t source = tmem + lanes + acc * kTile;
-      const int m = u.m0 + row_in_tile;
-      const auto read32 = [&](int c0, float (&z)[32]) {
-        uint32_t v[32];
+      const uint32_t source = source0 + acc * kTile;
+      const int m = u.m0 + row_in_tile, n = u.n0 + column0;
+      // the accumulator goes back to the issuer as soon as its last columns are in registers
+      const auto release = [&] {
         if (ok && !empty) {
-          umma::tmem_ld32(source + c0, v);
-          umma::tmem_ld_wait();
+          umma::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) umma2::arrive_cluster(umma2::in_leader(&acc_empty[acc]));
         }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) z[j] = !ok ? quiet_nan() : (empty ? 0.f : __uint_as_float(v[j]));
       };
       if (P == kStats) {
-        // two sweeps over the accumulator: the maximum, then the exponentials and their sum, all in units of log2
-        const int valid = prm.vocab - u.n0;  // columns of the tile inside the vocabulary (may exceed the tile)
-        float z[32], high = -INFINITY;
-        bool nan = false;
-#pragma unroll 1
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
-          read32(c0, z);
+        float z[kStatsTile];
+        if (ok && !empty) {
+          uint32_t(&v)[kStatsTile / 32][32] = reinterpret_cast<uint32_t(&)[kStatsTile / 32][32]>(z);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (c0 + j < valid) {
-              high = fmaxf(high, z[j]);
-              nan |= z[j] != z[j];  // fmaxf drops a NaN, the statistics must not
+          for (int i = 0; i < kStatsTile / 32; ++i) umma::tmem_ld32(source + 32 * i, v[i]);
+          umma::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int j = 0; j < kStatsTile; ++j) z[j] = ok ? 0.f : quiet_nan();
+        }
+        release();
+        const int valid = prm.vocab - n;  // columns inside the vocabulary, possibly none or more than there are here
+        if (valid > 0) {
+          if (valid < kStatsTile) {
+#pragma unroll
+            for (int j = 0; j < kStatsTile; ++j) z[j] = j < valid ? z[j] : -INFINITY;
+          }
+          // a NaN gets past the maximum, but not past the sum
+          float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < kStatsTile; ++j) high[j & 3] = fmaxf(high[j & 3], z[j]);
+          const float reference = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * prm.log2_scale;
+#pragma unroll
+          for (int j = 0; j < kStatsTile; ++j) {
+            z[j] = ex2_approx(fmaf(z[j], prm.log2_scale, -reference));
+            sum[j & 3] += z[j];
+          }
+          if (m < m_end) {
+            prm.stats[(long long)(n / kStatsTile) * prm.stats_stride + m] =
+                make_float2(reference, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+            if (prm.power != nullptr) {
+              __half* dst = prm.power + m * prm.ldp + n;  // rows are padded to 64 columns
+#pragma unroll
+              for (int h = 0; h < kStatsTile; h += 16) {
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = Io16<__half>::pack(z[h + 2 * j], z[h + 2 * j + 1]);
+                if (n + h < prm.ldp) store32(dst + h, o, true);
+              }
             }
           }
         }
-        high = nan ? quiet_nan() : high * prm.log2_scale;
-        float sum = 0.f;
-#pragma unroll 1
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
-          read32(c0, z);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            z[j] = c0 + j < valid ? ex2_approx(fmaf(z[j], prm.log2_scale, -high)) : 0.f;
-            sum += z[j];
-          }
-          if (prm.power != nullptr && m < m_end && u.n0 + c0 < prm.ldp) {
-            __half* dst = prm.power + m * prm.ldp + u.n0 + c0;  // rows are padded to 64 columns: whole 64-byte pieces
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t o[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) o[j] = Io16<__half>::pack(z[16 * h + 2 * j], z[16 * h + 2 * j + 1]);
-              store32(dst + 16 * h, o, true);
-            }
-          }
-        }
-        if (m < m_end) prm.stats[(long long)(u.n0 / kTile) * prm.stats_stride + m] = make_float2(high, sum);
       } else {
         const long long slot = (long long)u.split * (P == kGradX ? prm.rows.piece_rows : prm.vocab);
         const bool inside = m < m_end;
         const int row = P == kGradX && inside && prm.partials == nullptr ? prm.rows.row_map[prm.rows.piece_begin + m] : m;
         const bool wide = (prm.channels & 15) == 0 && (reinterpret_cast<uintptr_t>(prm.out) & 31u) == 0;
 #pragma unroll 1
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
-          float z[32];
-          read32(c0, z);
-          if (inside && prm.partials != nullptr) {
-            float* dst = prm.partials + (slot + m) * prm.channels + u.n0 + c0;
+        for (int c0 = 0; c0 < kStatsTile; c0 += 64) {
+          float z[64];
+          if (ok && !empty) {
+            uint32_t(&v)[2][32] = reinterpret_cast<uint32_t(&)[2][32]>(z);
+            umma::tmem_ld32(source + c0, v[0]);
+            umma::tmem_ld32(source + c0 + 32, v[1]);
+            umma::tmem_ld_wait();
+          } else {
 #pragma unroll
-            for (int h = 0; h < 32; h += 8) {
-              if (u.n0 + c0 + h < prm.channels) {  // channels are a multiple of 8
+            for (int j = 0; j < 64; ++j) z[j] = ok ? 0.f : quiet_nan();
+          }
+          if (c0 == 64) release();
+          if (inside && prm.partials != nullptr) {
+            float* dst = prm.partials + (slot + m) * prm.channels + n + c0;
+#pragma unroll
+            for (int h = 0; h < 64; h += 8) {
+              if (n + c0 + h < prm.channels) {  // channels are a multiple of 8
                 if (prm.add) {
                   const float4 a = *reinterpret_cast<const float4*>(dst + h), b = *reinterpret_cast<const float4*>(dst + h + 4);
                   z[h] += a.x; z[h + 1] += a.y; z[h + 2] += a.z; z[h + 3] += a.w;
@@ -286,13 +301,13 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
               }
             }
           } else if (inside) {
-            bf16* dst = prm.out + (long long)row * prm.channels + u.n0 + c0;
+            bf16* dst = prm.out + (long long)row * prm.channels + n + c0;
 #pragma unroll
-            for (int h = 0; h < 32; h += 16) {
+            for (int h = 0; h < 64; h += 16) {
               uint32_t o[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j) o[j] = IO::pack(z[h + 2 * j], z[h + 2 * j + 1]);
-              const int room = prm.channels - (u.n0 + c0 + h);
+              const int room = prm.channels - (n + c0 + h);
               if (room >= 16) {
                 store32(dst + h, o, wide);
               } else if (room >= 8) {
@@ -301,11 +316,6 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
             }
           }
         }
-      }
-      if (ok && !empty) {
-        umma::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) umma2::arrive_cluster(umma2::in_leader(&acc_empty[acc]));
       }
     }
   }

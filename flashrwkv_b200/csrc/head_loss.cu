@@ -10,7 +10,7 @@
 // Passes over a piece of the rows (all of them while 2 rows x vocabulary bytes fit kPieceBytes):
 //   plan     numbers the rows that have a label; rows without one take no part in any product (compact_kernel copies the
 //            others together, or does nothing where every row takes part), so what they hold, NaN included, reaches nothing
-//   stats    z by 256 columns on the tensor cores; the epilogue leaves each row's maximum and sum of exponentials, and for
+//   stats    z on the tensor cores; the epilogue leaves, per 128 columns, each row's maximum and sum of exponentials, and for
 //            gradients the exponentials themselves in fp16, relative to that maximum (error 2^-12 of each, where a bf16
 //            value would add 2^-9 to the one rounding that g needs as a tensor-core operand)
 //   finish   per row: lse from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
@@ -72,22 +72,38 @@ __global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* _
 __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position, int* __restrict__ row_map,
                                                     int* __restrict__ count, int* __restrict__ error_flag, int rows) {
   chain_begin();
+  constexpr int kEach = 8;  // consecutive rows of a thread
   __shared__ int warp_sums[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int done = 0;
-  for (int begin = 0; begin < rows; begin += 1024) {
-    const int row = begin + threadIdx.x;
-    const bool used = row < rows && (labels.teacher != nullptr ? position[row] != 0 : labels.at(row) != labels.ignore_index);
-    const unsigned mask = __ballot_sync(0xffffffffu, used);
-    if (lane == 0) warp_sums[warp] = __popc(mask);
+  for (int begin = 0; begin < rows; begin += 1024 * kEach) {
+    const int first = begin + threadIdx.x * kEach;
+    unsigned used = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int row = first + i;
+      if (row < rows && (labels.teacher != nullptr ? position[row] != 0 : labels.at(row) != labels.ignore_index)) used |= 1u << i;
+    }
+    const int mine = __popc(used);
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
-    const int mine = warp_sums[lane];
-    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
-    const int all = __reduce_add_sync(0xffffffffu, mine);
-    const int at = done + before + __popc(mask & ((1u << lane) - 1u));
-    if (row < rows) position[row] = used ? at : -1;
-    if (used) row_map[at] = row;
-    done += all;
+    const int others = warp_sums[lane];
+    int at = done + __reduce_add_sync(0xffffffffu, lane < warp ? others : 0) + upto - mine;
+    done += __reduce_add_sync(0xffffffffu, others);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int row = first + i;
+      if (row >= rows) break;
+      const bool u = used >> i & 1u;
+      position[row] = u ? at : -1;
+      if (u) row_map[at++] = row;
+    }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
@@ -155,7 +171,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   chain_begin();
   extern __shared__ float factor[];  // [tiles] then logit [top] and share [top]
   __shared__ float scratch[kFinishThreads / 32];
-  const int tiles = (a.vocab + kTile - 1) / kTile, top = a.labels.top;
+  const int tiles = (a.vocab + kStatsTile - 1) / kStatsTile, top = a.labels.top;
   float* logit = factor + tiles;
   float* share = logit + top;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -253,7 +269,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   __syncthreads();  // the tiles' factors and the shares
   for (int i = tid; i < groups; i += kFinishThreads) {
     const uint4 e = g[i];
-    const float f = scale * ex2_approx(factor[i / (kTile / 8)]);
+    const float f = scale * ex2_approx(factor[i / (kStatsTile / 8)]);
     const uint32_t in[4] = {e.x, e.y, e.z, e.w};
     uint32_t out[4];
 #pragma unroll
@@ -307,10 +323,21 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float4* __restrict
   const long long total = rows * pieces, stride = (long long)part_rows * pieces * 2;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    for (int s = 0; s < parts; ++s) {
-      const float4 u = __ldg(partials + s * stride + 2 * i), v = __ldg(partials + s * stride + 2 * i + 1);
-      a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
-      b.x += v.x; b.y += v.y; b.z += v.z; b.w += v.w;
+    for (int s = 0; s < parts; s += 4) {  // four parts requested together (the last again where there are fewer)
+      float4 u[4], v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4* q = partials + (s + j < parts ? s + j : parts - 1) * stride + 2 * i;
+        u[j] = __ldg(q);
+        v[j] = __ldg(q + 1);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (s + j < parts) {
+          a.x += u[j].x; a.y += u[j].y; a.z += u[j].z; a.w += u[j].w;
+          b.x += v[j].x; b.y += v[j].y; b.z += v[j].z; b.w += v[j].w;
+        }
+      }
     }
     const long long row = i / pieces;
     const long long to = row_map != nullptr ? (long long)row_map[row_begin + row] * pieces + (i - row * pieces) : i;
@@ -355,7 +382,7 @@ Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad
   Layout l{};
   const bool grads = grad_x || grad_weight;
   l.ldg = ((long long)vocab + 63) / 64 * 64;
-  const long long tiles = (vocab + kTile - 1) / kTile;
+  const long long tiles = (vocab + kStatsTile - 1) / kStatsTile;
   long long most = kStatsBytes / (8 * tiles);
   if (grads && kPieceBytes / (2 * l.ldg) < most) most = kPieceBytes / (2 * l.ldg);
   most = most / kTile * kTile;
@@ -433,7 +460,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   void* power = grads ? ws + l.power : nullptr;
   float* partial_x = l.parts_x ? reinterpret_cast<float*>(ws + l.partial_x) : nullptr;
   float* partial_w = l.parts_w ? reinterpret_cast<float*>(ws + l.partial_w) : nullptr;
-  const int rows = (int)a.rows, x_pieces = a.channels / 8, tiles = (a.vocab + kTile - 1) / kTile;
+  const int rows = (int)a.rows, x_pieces = a.channels / 8, tiles = (a.vocab + kStatsTile - 1) / kStatsTile;
 
   Labels labels{};
   labels.index = a.labels;

@@ -7,7 +7,8 @@
 namespace frwkv {
 namespace head {
 
-constexpr int kTile = 256;  // rows and columns of an output tile
+constexpr int kTile = 256;       // rows and columns of an output tile
+constexpr int kStatsTile = 128;  // vocabulary columns of one maximum and sum of exponentials
 
 // The rows that take part are numbered 0..count-1 ("compact rows"); the first *count entries of row_map are their numbers
 // in x.  A product works on a piece of them: compact rows piece_begin .. piece_begin + piece_rows - 1, cut at *count.
@@ -18,7 +19,7 @@ struct Rows {
   int piece_begin, piece_rows;
 };
 
-// Statistics of the logits z = x W^T / T: for every tile of 256 vocabulary columns and every row of the piece
+// Statistics of the logits z = x W^T / T: for every 128 vocabulary columns and every row of the piece
 // stats[tile * stats_stride + row] = (max, sum exp2(z' - max)) with z' = z log2(e) / T, and, with `power`, the fp16 values
 // exp2(z' - max) in power[row][ldp] (zeros behind the vocabulary).
 int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
