@@ -46,7 +46,7 @@ struct Params {
   int channels, vocab, splits;
   float log2_scale;        // kStats
   float2* stats;
-  int stats_stride;
+  int stats_tiles;
   __half* power;
   long long ldp;
   bf16* out;               // kGradX, kGradWeight
@@ -56,16 +56,18 @@ struct Params {
 
 struct Unit {
   int m0, n0, split, kb_begin, kb_end;
+  int width;  // columns of the tile, a multiple of 32: the last tile of a row may need fewer than 256
 };
 
 // the work of a launch, from the number of rows that take part
 template <Product P>
 struct Work {
-  int tiles_m, tiles_n, units, kb_total, splits;
+  int tiles_m, tiles_n, units, kb_total, splits, columns;
   __device__ Work(const Params& p, int rows_here) {
     const int m = P == kGradWeight ? p.vocab : rows_here;
     const int n = P == kStats ? p.vocab : p.channels;
     const int k = P == kStats ? p.channels : (P == kGradX ? p.vocab : rows_here);
+    columns = n;
     tiles_m = (m + kTile - 1) / kTile;
     tiles_n = (n + kTile - 1) / kTile;
     kb_total = (k + kBK - 1) / kBK;
@@ -81,6 +83,8 @@ struct Work {
     const int t = unit - u.split * tiles;
     u.m0 = (P == kStats ? t % tiles_m : t / tiles_n) * kTile;
     u.n0 = (P == kStats ? t / tiles_m : t % tiles_n) * kTile;
+    const int right = columns - u.n0;
+    u.width = right < kTile ? (right + 31) & ~31 : kTile;
     u.kb_begin = (int)((long long)kb_total * u.split / splits);
     u.kb_end = (int)((long long)kb_total * (u.split + 1) / splits);
     return u;
@@ -149,7 +153,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
           const uint32_t full = umma2::in_leader(&full_bar[s]);
           if (rank == 0) umma::mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
           const uint32_t a_dst = tiles_base + s * kStageBytes, b_dst = a_dst + kOperandBytes;
-          const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * kHalf, k = kb * kBK;
+          const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * (u.width / 2), k = kb * kBK;
           if (kAMn) {
             umma2::tma_load_2d(a_dst, map_a, m, a_row + k, full);
             umma2::tma_load_2d(a_dst + 8192, map_a, m + 64, a_row + k, full);
@@ -172,7 +176,6 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = umma2::idesc_bf16_256(kAMn, kBMn);
       uint32_t it = 0, t = 0;
       for (int unit = pair; unit < work.units && ok; unit += pairs) {
         const Unit u = work.at(unit);
@@ -182,6 +185,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
         if (!umma2::wait_cluster(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
         umma::fence_after_sync();
         const uint32_t d_tmem = tmem + acc * kTile;
+        const uint32_t idesc = umma2::idesc_bf16(u.width, kAMn, kBMn);
         for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
           if (!umma2::wait_cluster(&full_bar[s], ph)) { ok = false; break; }
@@ -252,7 +256,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
             sum[j & 3] += z[j];
           }
           if (m < m_end) {
-            prm.stats[(long long)(n / kStatsTile) * prm.stats_stride + m] =
+            prm.stats[(long long)m * prm.stats_tiles + n / kStatsTile] =
                 make_float2(reference, (sum[0] + sum[1]) + (sum[2] + sum[3]));
             if (prm.power != nullptr) {
               __half* dst = prm.power + m * prm.ldp + n;  // rows are padded to 64 columns
@@ -405,7 +409,7 @@ int contraction_splits(long long rows, long long columns, long long k) {
 }
 
 int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
-                       float log2_scale, float2* stats, int stats_stride, void* power, long long ldp, int* error_flag,
+                       float log2_scale, float2* stats, void* power, long long ldp, int* error_flag,
                        cudaStream_t stream) {
   Params prm{};
   prm.rows = rows;
@@ -414,7 +418,7 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
   prm.splits = 1;
   prm.log2_scale = log2_scale;
   prm.stats = stats;
-  prm.stats_stride = stats_stride;
+  prm.stats_tiles = (vocab + kStatsTile - 1) / kStatsTile;
   prm.power = static_cast<__half*>(power);
   prm.ldp = ldp;
   if (!make_map(&prm.map_a, x, rows.total, channels, channels, kHalf) ||

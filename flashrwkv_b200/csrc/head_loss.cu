@@ -72,19 +72,20 @@ __global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* _
 __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position, int* __restrict__ row_map,
                                                     int* __restrict__ count, int* __restrict__ error_flag, int rows) {
   chain_begin();
-  constexpr int kEach = 8;  // consecutive rows of a thread
+  constexpr int kEach = 8;  // consecutive rows of a thread; the flags come in row order through shared memory
   __shared__ int warp_sums[32];
+  __shared__ unsigned char flags[1024 * kEach];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int done = 0;
   for (int begin = 0; begin < rows; begin += 1024 * kEach) {
-    const int first = begin + threadIdx.x * kEach;
-    unsigned used = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int row = first + i;
-      if (row < rows && (labels.teacher != nullptr ? position[row] != 0 : labels.at(row) != labels.ignore_index)) used |= 1u << i;
+      const int at = i * 1024 + threadIdx.x, row = begin + at;
+      flags[at] = row < rows && (labels.teacher != nullptr ? position[row] != 0 : labels.at(row) != labels.ignore_index);
     }
-    const int mine = __popc(used);
+    __syncthreads();
+    const uint2 mine8 = *reinterpret_cast<const uint2*>(flags + threadIdx.x * kEach);
+    const int mine = __popc(mine8.x) + __popc(mine8.y);
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -98,16 +99,17 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
     done += __reduce_add_sync(0xffffffffu, others);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int row = first + i;
+      const int row = begin + threadIdx.x * kEach + i;
       if (row >= rows) break;
-      const bool u = used >> i & 1u;
-      position[row] = u ? at : -1;
-      if (u) row_map[at++] = row;
+      const bool used = ((i < 4 ? mine8.x : mine8.y) >> (8 * (i & 3))) & 1u;
+      position[row] = used ? at : -1;
+      if (used) row_map[at++] = row;
     }
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    *count = done;
+    count[0] = done;
+    count[1] = 0;  // CTAs that have written their losses
     *error_flag = 0;
   }
 }
@@ -152,20 +154,91 @@ __device__ __forceinline__ float block_reduce(float v, float* scratch, bool maxi
   return v;
 }
 
+// z of one label, a warp's fp32 dot product
+__device__ __forceinline__ float label_logit(const bf16* x_row, const bf16* w_row, int pieces, int lane) {
+  float dot = 0.f;
+#pragma unroll 4
+  for (int p = lane; p < pieces; p += 32) {
+    const uint4 ux = __ldg(reinterpret_cast<const uint4*>(x_row) + p), uw = __ldg(reinterpret_cast<const uint4*>(w_row) + p);
+    const uint32_t xs[4] = {ux.x, ux.y, ux.z, ux.w}, ws[4] = {uw.x, uw.y, uw.z, uw.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 fx = IO::unpack(xs[e]), fw = IO::unpack(ws[e]);
+      dot = fmaf(fx.x, fw.x, dot);
+      dot = fmaf(fx.y, fw.y, dot);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+  return dot;
+}
+
 struct FinishArgs {
   Rows rows;
   Labels labels;
   const bf16* x;
   const bf16* weight;
-  const float2* stats;
-  int stats_stride, vocab, channels;
+  const float2* stats;       // [row of the piece][tiles]
+  int vocab, channels;
   uint4* g;            // exponentials in, logit gradients out, ldg values per row; null without gradients
   long long ldg;
   bool mean;
   const float* row_grads;    // upstream gradients of the row losses, or null
   const float* grad_scale;   // upstream gradient of the loss, or null
   float* row_losses;
+  float* loss;               // the last CTA of the last piece to arrive adds the row losses, in row order; or null
+  int* arrived;
+  int ctas;                  // of all pieces
 };
+
+// Called by every CTA with its row losses written.  The sum does not depend on who arrives last.
+__device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count, float* scratch) {
+  if (a.loss == nullptr) return;
+  __shared__ bool last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(a.arrived, 1) == a.ctas - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  float v = 0.f;
+  for (int i = threadIdx.x; i < a.rows.total; i += kFinishThreads) v += __ldcg(a.row_losses + i);
+  v = block_reduce(v, scratch, false);
+  if (threadIdx.x == 0) *a.loss = a.mean && count > 0 ? v / (float)count : v;  // no row takes part: 0
+}
+
+// The losses of labels alone, without gradients: a warp per row.
+__global__ __launch_bounds__(kFinishThreads) void losses_kernel(const FinishArgs a) {
+  chain_begin();
+  __shared__ float scratch[kFinishThreads / 32];
+  const int tiles = (a.vocab + kStatsTile - 1) / kStatsTile, lane = threadIdx.x & 31;
+  const int count = *a.rows.count, left = count - a.rows.piece_begin;
+  const int rows_here = left < 0 ? 0 : (left < a.rows.piece_rows ? left : a.rows.piece_rows);
+  const int r = blockIdx.x * (kFinishThreads / 32) + (threadIdx.x >> 5);
+  if (r < rows_here) {
+    const long long n = a.rows.row_map[a.rows.piece_begin + r];
+    const long long v = a.labels.at(n);
+    const bool inside = v >= 0 && v < a.vocab;
+    const float2* stats = a.stats + (long long)r * tiles;
+    float high = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (int t = lane; t < tiles; t += 32) high = fmaxf(high, __ldg(&stats[t].x));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+#pragma unroll 4
+    for (int t = lane; t < tiles; t += 32) {
+      const float2 s = __ldg(stats + t);
+      sum = fmaf(s.y, ex2_approx(s.x - high), sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float logit = inside ? label_logit(a.x + n * a.channels, a.weight + v * a.channels, a.channels / 8, lane) : 0.f;
+    if (lane == 0) a.row_losses[n] = inside ? (high * 0.6931471805599453f - logit) + logf(sum) : quiet_nan();
+  }
+  arrive_and_sum(a, count, scratch);
+}
 
 __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs a) {
   chain_begin();
@@ -184,50 +257,34 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     // zeros behind the last row, to the end of its block of the contraction over rows
     if (a.g != nullptr && r < ((rows_here + 63) & ~63))
       for (int i = tid; i < groups; i += kFinishThreads) g[i] = make_uint4(0u, 0u, 0u, 0u);
+    arrive_and_sum(a, count, scratch);
     return;
   }
   const long long n = a.rows.row_map[a.rows.piece_begin + r];
 
   // the softmax's normaliser, in units of log2
+  const float2* stats = a.stats + (long long)r * tiles;
   float high = -INFINITY, sum = 0.f;
-  for (int t = tid; t < tiles; t += kFinishThreads) high = fmaxf(high, a.stats[(long long)t * a.stats_stride + r].x);
+  for (int t = tid; t < tiles; t += kFinishThreads) high = fmaxf(high, stats[t].x);
   high = block_reduce(high, scratch, true);
   for (int t = tid; t < tiles; t += kFinishThreads) {
-    const float2 s = a.stats[(long long)t * a.stats_stride + r];
+    const float2 s = stats[t];
     sum = fmaf(s.y, ex2_approx(s.x - high), sum);
   }
   sum = block_reduce(sum, scratch, false);
   const float lse2 = high + log2f(sum);
   // lse - z is taken as (max - z) + log(sum): both terms are small where the label is likely
   const float max_z = high * 0.6931471805599453f, log_sum = logf(sum);
-  for (int t = tid; t < tiles; t += kFinishThreads) factor[t] = a.stats[(long long)t * a.stats_stride + r].x - lse2;
+  for (int t = tid; t < tiles; t += kFinishThreads) factor[t] = stats[t].x - lse2;
 
   // the labels' logits: a warp per entry
   const long long entry = n * top;
-  const int pieces = a.channels / 8;
   bool bad = false;
   for (int k = warp; k < top; k += kFinishThreads / 32) {
     const bool there = a.labels.teacher == nullptr || !(a.labels.teacher[entry + k] == -INFINITY);
     const long long v = there ? a.labels.at(entry + k) : 0;
     const bool inside = v >= 0 && v < a.vocab;
-    float dot = 0.f;
-    if (there && inside) {
-      const uint4* xr = reinterpret_cast<const uint4*>(a.x + n * a.channels);
-      const uint4* wr = reinterpret_cast<const uint4*>(a.weight + v * a.channels);
-#pragma unroll 4
-      for (int p = lane; p < pieces; p += 32) {
-        const uint4 ux = __ldg(xr + p), uw = __ldg(wr + p);
-        const uint32_t xs[4] = {ux.x, ux.y, ux.z, ux.w}, ws[4] = {uw.x, uw.y, uw.z, uw.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 fx = IO::unpack(xs[e]), fw = IO::unpack(ws[e]);
-          dot = fmaf(fx.x, fw.x, dot);
-          dot = fmaf(fx.y, fw.y, dot);
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    }
+    const float dot = there && inside ? label_logit(a.x + n * a.channels, a.weight + v * a.channels, a.channels / 8, lane) : 0.f;
     bad |= there && !inside;
     if (lane == 0) logit[k] = dot * a.labels.inv_temperature;
   }
@@ -259,6 +316,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   }
   if (bad) loss = quiet_nan();  // a label outside the vocabulary
   if (tid == 0) a.row_losses[n] = loss;
+  arrive_and_sum(a, count, scratch);
   if (a.g == nullptr) return;
 
   float scale = a.labels.temperature;
@@ -294,25 +352,6 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
 }
 
 // ---- small passes ------------------------------------------------------------------------------------------------------
-// loss = sum of the row losses in a fixed order, over the number of rows that take part where `mean`
-__global__ __launch_bounds__(1024) void sum_losses_kernel(const float* __restrict__ row_losses, const int* __restrict__ count,
-                                                          float* __restrict__ loss, int rows, bool mean) {
-  chain_begin();
-  __shared__ float sums[32];
-  float v = 0.f;
-  for (int i = threadIdx.x; i < rows; i += 1024) v += row_losses[i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
-  __syncthreads();
-  if (threadIdx.x >= 32) return;
-  v = sums[threadIdx.x];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int used = *count;
-  if (threadIdx.x == 0) *loss = mean && used > 0 ? v / (float)used : v;  // no row takes part: 0
-}
-
 // out[row_map ? row_map[row_begin + row] : row][c] = sum of the parts in their order
 __global__ __launch_bounds__(256) void sum_parts_kernel(const float4* __restrict__ partials, bf16* __restrict__ out,
                                                         const int* __restrict__ row_map, const int* __restrict__ count,
@@ -345,13 +384,15 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float4* __restrict
   }
 }
 
-// values *= *scale, in place; nothing to do where the scale is one
-__global__ __launch_bounds__(256) void scale_kernel(uint4* __restrict__ values, long long pieces, const float* __restrict__ scale) {
+// Both arrays *= *scale, in place; nothing to do where the scale is one.
+__global__ __launch_bounds__(256) void scale_kernel(uint4* __restrict__ first, long long first_pieces, uint4* __restrict__ second,
+                                                    long long pieces, const float* __restrict__ scale) {
   chain_begin();
   const float f = *scale;
   if (f == 1.f) return;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (long long)gridDim.x * 256) {
-    const uint4 u = values[i];
+    uint4* at = i < first_pieces ? first + i : second + (i - first_pieces);
+    const uint4 u = *at;
     const uint32_t in[4] = {u.x, u.y, u.z, u.w};
     uint32_t out[4];
 #pragma unroll
@@ -359,7 +400,7 @@ __global__ __launch_bounds__(256) void scale_kernel(uint4* __restrict__ values, 
       const float2 t = IO::unpack(in[j]);
       out[j] = IO::pack(t.x * f, t.y * f);
     }
-    values[i] = make_uint4(out[0], out[1], out[2], out[3]);
+    *at = make_uint4(out[0], out[1], out[2], out[3]);
   }
 }
 
@@ -486,7 +527,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   for (int piece = 0; piece < l.pieces; ++piece) {
     const Rows here{count, row_map, rows, piece * l.piece_rows, l.piece_rows};
     if (int rc = launch_logit_stats(a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab,
-                                    (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature), stats, l.piece_rows, power, l.ldg,
+                                    (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature), stats, power, l.ldg,
                                     a.error_flag, s))
       return rc;
     FinishArgs f{};
@@ -495,7 +536,6 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.x = static_cast<const bf16*>(a.x);
     f.weight = static_cast<const bf16*>(a.weight);
     f.stats = stats;
-    f.stats_stride = l.piece_rows;
     f.vocab = a.vocab;
     f.channels = a.channels;
     f.g = static_cast<uint4*>(power);
@@ -504,7 +544,15 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.row_grads = a.row_grads;
     f.grad_scale = a.grad_scale;
     f.row_losses = a.row_losses;
-    launch_chained(finish_kernel, dim3(l.piece_rows), dim3(kFinishThreads), finish_smem, s, f);
+    f.loss = a.loss;
+    f.arrived = count + 1;
+    const bool by_warps = !grads && a.teacher_logits == nullptr;
+    const int ctas = by_warps ? (l.piece_rows + kFinishThreads / 32 - 1) / (kFinishThreads / 32) : l.piece_rows;
+    f.ctas = ctas * l.pieces;
+    if (by_warps)
+      launch_chained(losses_kernel, dim3(ctas), dim3(kFinishThreads), 0, s, f);
+    else
+      launch_chained(finish_kernel, dim3(ctas), dim3(kFinishThreads), finish_smem, s, f);
     if (int rc = check_launch("finish_kernel")) return rc;
     if (a.grad_x != nullptr) {
       if (int rc = launch_grad_x(power, l.ldg, a.weight, here, a.channels, a.vocab, l.splits_x, a.grad_x, partial_x,
@@ -527,22 +575,23 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
                    l.splits_w);
     if (int rc = check_launch("sum_parts_kernel")) return rc;
   }
-  if (a.loss != nullptr) {
-    launch_chained(sum_losses_kernel, dim3(1), dim3(1024), 0, s, a.row_losses, count, a.loss, rows, a.mean != 0);
-    if (int rc = check_launch("sum_losses_kernel")) return rc;
-  }
   return FRWKV_OK;
 }
 
-extern "C" int frwkv_scale_bf16(void* values, long long numel, const float* scale, frwkv_stream_t stream) {
+extern "C" int frwkv_scale_bf16(void* first, long long first_numel, void* second, long long second_numel, const float* scale,
+                                frwkv_stream_t stream) {
   using namespace frwkv;
   using namespace frwkv::head;
   clear_error();
-  FRWKV_REQUIRE(values && scale, "scale_bf16: null pointer argument");
-  FRWKV_REQUIRE(numel > 0 && numel % 8 == 0, "scale_bf16: the number of values must be a positive multiple of 8");
-  FRWKV_REQUIRE(aligned(values, 16), "scale_bf16: values must be 16-byte aligned");
-  const long long pieces = numel / 8, blocks = (pieces + 255) / 256;
+  FRWKV_REQUIRE(scale && (first || second) && (first || first_numel == 0) && (second || second_numel == 0),
+                "scale_bf16: null pointer argument");
+  FRWKV_REQUIRE(first_numel >= 0 && second_numel >= 0 && first_numel % 8 == 0 && second_numel % 8 == 0,
+                "scale_bf16: the numbers of values must be multiples of 8");
+  FRWKV_REQUIRE(aligned(first, 16) && aligned(second, 16), "scale_bf16: values must be 16-byte aligned");
+  const long long pieces = (first_numel + second_numel) / 8, blocks = (pieces + 255) / 256;
+  if (pieces == 0) return FRWKV_OK;
   launch_chained(scale_kernel, dim3((unsigned)(blocks < 1184 ? blocks : 1184)), dim3(256), 0,
-                 reinterpret_cast<cudaStream_t>(stream), static_cast<uint4*>(values), pieces, scale);
+                 reinterpret_cast<cudaStream_t>(stream), static_cast<uint4*>(first), first_numel / 8,
+                 static_cast<uint4*>(second), pieces, scale);
   return check_launch("scale_kernel");
 }

@@ -20,10 +20,10 @@ struct Rows {
 };
 
 // Statistics of the logits z = x W^T / T: for every 128 vocabulary columns and every row of the piece
-// stats[tile * stats_stride + row] = (max, sum exp2(z' - max)) with z' = z log2(e) / T, and, with `power`, the fp16 values
+// stats[row][tile] = (max, sum exp2(z' - max)) with z' = z log2(e) / T, and, with `power`, the fp16 values
 // exp2(z' - max) in power[row][ldp] (zeros behind the vocabulary).
 int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
-                       float log2_scale, float2* stats, int stats_stride, void* power, long long ldp, int* error_flag,
+                       float log2_scale, float2* stats, void* power, long long ldp, int* error_flag,
                        cudaStream_t stream);
 
 // How many parts the contraction of a rows x columns product over k is cut into.

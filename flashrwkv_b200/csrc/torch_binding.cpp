@@ -2146,9 +2146,9 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
       gw = want_weight ? pair->elements()[1].toTensor() : torch::Tensor();
       ctx->saved_data.erase(kept);
       const c10::cuda::CUDAGuard guard(saved[0].device());
-      for (const auto& t : {gx, gw})
-        if (t.defined())
-          check_rc(frwkv_scale_bf16(t.data_ptr(), t.numel(), upstream.data_ptr<float>(), current_stream(t)));
+      check_rc(frwkv_scale_bf16(gx.defined() ? gx.data_ptr() : nullptr, gx.defined() ? gx.numel() : 0,
+                                gw.defined() ? gw.data_ptr() : nullptr, gw.defined() ? gw.numel() : 0,
+                                upstream.data_ptr<float>(), current_stream(upstream)));
     } else {
       const HeadInputs in{saved[0], saved[1], saved[2], saved[3], ctx->saved_data["ignore_index"].toInt(),
                           ctx->saved_data["temperature"].toDouble()};

@@ -100,9 +100,9 @@ __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
   return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(8192 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(2) << 61);
 }
-// bf16 operands, fp32 accumulator, 256 x 256; bits 15 / 16: A / B is MN-major
-__host__ __device__ constexpr uint32_t idesc_bf16_256(bool a_mn, bool b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(256 >> 3) << 17) |
+// bf16 operands, fp32 accumulator, 256 rows x `columns` (a multiple of 32 up to 256); bits 15 / 16: A / B is MN-major
+__host__ __device__ constexpr uint32_t idesc_bf16(int columns, bool a_mn, bool b_mn) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(columns >> 3) << 17) |
          (uint32_t(256 >> 4) << 24);
 }
 

@@ -638,8 +638,10 @@ typedef struct {
 } frwkv_head_loss_args;
 size_t frwkv_pretrain_head_loss_workspace_bytes(long long rows, int channels, int vocab, int grad_x, int grad_weight);
 int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_stream_t stream);
-/* values (bf16, numel a multiple of 8, 16-byte aligned) *= *scale (a device value) in place. */
-int frwkv_scale_bf16(void* values, long long numel, const float* scale, frwkv_stream_t stream);
+/* Both arrays (bf16, lengths multiples of 8, 16-byte aligned; either may be NULL with length 0) *= *scale (a device value),
+ * in place. */
+int frwkv_scale_bf16(void* first, long long first_numel, void* second, long long second_numel, const float* scale,
+                     frwkv_stream_t stream);
 
 #ifdef __cplusplus
 }

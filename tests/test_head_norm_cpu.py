@@ -161,9 +161,12 @@ def test_head_entry_refuses_bad_arguments_without_a_device():
         assert message in lib.frwkv_last_error(), (changes, lib.frwkv_last_error())
     assert lib.frwkv_pretrain_head_loss_workspace_bytes(ctypes.c_longlong(0), 64, 100, 1, 1) == 0
     ok, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4104)
-    assert lib.frwkv_scale_bf16(None, ctypes.c_longlong(8), ok, None) == -1
-    assert lib.frwkv_scale_bf16(ok, ctypes.c_longlong(12), ok, None) == -1 and b"multiple of 8" in lib.frwkv_last_error()
-    assert lib.frwkv_scale_bf16(odd, ctypes.c_longlong(8), ok, None) == -1 and b"aligned" in lib.frwkv_last_error()
+    n, none = ctypes.c_longlong(8), ctypes.c_longlong(0)
+    assert lib.frwkv_scale_bf16(None, none, None, none, ok, None) == -1 and b"null pointer" in lib.frwkv_last_error()
+    assert lib.frwkv_scale_bf16(None, n, ok, n, ok, None) == -1 and lib.frwkv_scale_bf16(ok, n, None, none, None, None) == -1
+    assert lib.frwkv_scale_bf16(ok, ctypes.c_longlong(12), None, none, ok, None) == -1
+    assert b"multiples of 8" in lib.frwkv_last_error()
+    assert lib.frwkv_scale_bf16(ok, n, odd, n, ok, None) == -1 and b"aligned" in lib.frwkv_last_error()
 
 
 def test_head_workspace_stays_bounded():
