@@ -32,8 +32,9 @@ constexpr int kHalf = kTile / 2, kBK = 64;
 constexpr uint32_t kOperandBytes = kHalf * kBK * 2;  // 16 KB of each operand per CTA and stage
 constexpr uint32_t kStageBytes = 2 * kOperandBytes;
 constexpr int kStages = 6;
-constexpr uint32_t kSmem = kStages * kStageBytes + 1024;  // + slack to align the tiles to 1024 bytes
 constexpr int kEpilogueWarps = 8;  // two per quarter of the tensor-memory lanes, half of the columns each
+constexpr uint32_t kBoxBytes = 32 * 64 * 2;  // what an epilogue warp hands to TMA: 32 rows of 64 16-bit values
+constexpr uint32_t kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;  // + slack to align to 1024 bytes
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 constexpr uint32_t kTmemCols = 2 * kTile;
 
@@ -42,13 +43,13 @@ enum Product { kStats, kGradX, kGradWeight };
 struct Params {
   CUtensorMap map_a, map_b;
   CUtensorMap map_compact;  // kStats: A, kGradWeight: B, when some rows take no part
+  CUtensorMap map_out;      // kStats: the exponentials, kGradWeight: the bf16 gradient
   Rows rows;
   int channels, vocab, splits;
   float log2_scale;        // kStats
   float2* stats;
   int stats_tiles;
-  __half* power;
-  long long ldp;
+  bool power;              // kStats: the exponentials are wanted
   bf16* out;               // kGradX, kGradWeight
   float* partials;
   bool add;
@@ -97,6 +98,29 @@ __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8], bool wi
   } else {
     reinterpret_cast<uint4*>(p)[0] = make_uint4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<uint4*>(p)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// 64 columns of a warp's 32 rows, packed to 16 bits, to shared memory as TMA reads it and from there to global memory in
+// whole lines; the warp's box is free again once the store before has read it.
+template <typename T>
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, uint32_t box, const float* z, int lane) {
+  if (lane == 0) umma2::bulk_wait_read();
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = Io16<T>::pack(z[8 * i + 2 * j], z[8 * i + 2 * j + 1]);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(box + lane * 128 + ((i ^ (lane & 7)) << 4)), "r"(o[0]),
+                 "r"(o[1]), "r"(o[2]), "r"(o[3])
+                 : "memory");
+  }
+  umma::fence_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    umma2::tma_store_2d(map, x, y, box);
+    umma2::bulk_commit();
   }
 }
 
@@ -207,6 +231,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
     const uint32_t source0 = tmem + ((32u * quarter) << 16) + column0;
     const int row_in_tile = (int)rank * kHalf + 32 * (int)quarter + lane;
     const int m_end = P == kGradWeight ? prm.vocab : rows_here;
+    const uint32_t box = tiles_base + kStages * kStageBytes + (warp - 2) * kBoxBytes;
     uint32_t t = 0;
     for (int unit = pair; unit < work.units; unit += pairs) {
       const Unit u = work.at(unit);
@@ -258,16 +283,11 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
           if (m < m_end) {
             prm.stats[(long long)m * prm.stats_tiles + n / kStatsTile] =
                 make_float2(reference, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-            if (prm.power != nullptr) {
-              __half* dst = prm.power + m * prm.ldp + n;  // rows are padded to 64 columns
-#pragma unroll
-              for (int h = 0; h < kStatsTile; h += 16) {
-                uint32_t o[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = Io16<__half>::pack(z[h + 2 * j], z[h + 2 * j + 1]);
-                if (n + h < prm.ldp) store32(dst + h, o, true);
-              }
-            }
+          }
+          // rows of a box that take no part get what is there: nothing reads it
+          if (prm.power && m - lane < m_end) {
+            store_box<__half>(&prm.map_out, n, m - lane, box, z, lane);
+            if (valid > 64) store_box<__half>(&prm.map_out, n + 64, m - lane, box, z + 64, lane);
           }
         }
       } else {
@@ -288,7 +308,8 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
             for (int j = 0; j < 64; ++j) z[j] = ok ? 0.f : quiet_nan();
           }
           if (c0 == 64) release();
-          if (inside && prm.partials != nullptr) {
+          if (prm.partials != nullptr) {
+            if (!inside) continue;
             float* dst = prm.partials + (slot + m) * prm.channels + n + c0;
 #pragma unroll
             for (int h = 0; h < 64; h += 8) {
@@ -304,6 +325,8 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
                 store32(dst + h, o, true);
               }
             }
+          } else if (P == kGradWeight) {
+            if (n + c0 < prm.channels && m - lane < m_end) store_box<bf16>(&prm.map_out, n + c0, m - lane, box, z, lane);
           } else if (inside) {
             bf16* dst = prm.out + (long long)row * prm.channels + n + c0;
 #pragma unroll
@@ -323,6 +346,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
       }
     }
   }
+  if (P != kGradX && warp >= 2 && lane == 0) umma2::bulk_wait();  // this warp's stores, before the kernel may end
   if (!ok) {
     if (error_flag != nullptr) atomicExch(error_flag, 1 + (int)P);
     // give copies and MMAs that may still be in flight time to finish before the shared and tensor memory go away
@@ -352,7 +376,7 @@ EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-// [rows][columns] bf16 with rows `stride` values apart, boxes of 64 columns x box_rows, 128-byte swizzle, zeros outside
+// [rows][columns] 16-bit values (copied as they are) with rows `stride` values apart, boxes of 64 columns x box_rows, 128-byte swizzle, zeros outside
 bool make_map(CUtensorMap* map, const void* base, long long rows, long long columns, long long stride, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
@@ -419,11 +443,11 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
   prm.log2_scale = log2_scale;
   prm.stats = stats;
   prm.stats_tiles = (vocab + kStatsTile - 1) / kStatsTile;
-  prm.power = static_cast<__half*>(power);
-  prm.ldp = ldp;
+  prm.power = power != nullptr;
   if (!make_map(&prm.map_a, x, rows.total, channels, channels, kHalf) ||
       !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kHalf) ||
-      !make_map(&prm.map_b, weight, vocab, channels, channels, kHalf))
+      !make_map(&prm.map_b, weight, vocab, channels, channels, kHalf) ||
+      (power != nullptr && !make_map(&prm.map_out, power, rows.piece_rows, ldp, ldp, 32)))
     return map_failure();
   return launch<kStats>(prm, tiles_of(rows.piece_rows) * tiles_of(vocab), error_flag, stream);
 }
@@ -456,7 +480,8 @@ int launch_grad_weight(const void* g, long long ldg, const void* x, const void* 
   prm.add = add;
   if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kBK) ||
       !make_map(&prm.map_b, x, rows.total, channels, channels, kBK) ||
-      !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kBK))
+      !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kBK) ||
+      (partials == nullptr && !make_map(&prm.map_out, grad_weight, vocab, channels, channels, 32)))
     return map_failure();
   return launch<kGradWeight>(prm, tiles_of(vocab) * tiles_of(channels) * splits, error_flag, stream);
 }

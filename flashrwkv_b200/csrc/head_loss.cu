@@ -78,10 +78,22 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int done = 0;
   for (int begin = 0; begin < rows; begin += 1024 * kEach) {
+    long long label[kEach];  // requested together: past the end the last row again
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int at = i * 1024 + threadIdx.x, row = begin + at;
-      flags[at] = row < rows && (labels.teacher != nullptr ? position[row] != 0 : labels.at(row) != labels.ignore_index);
+      const int row = min(begin + i * 1024 + (int)threadIdx.x, rows - 1);
+      if (labels.teacher != nullptr) {
+        label[i] = position[row];
+      } else if (labels.wide) {
+        label[i] = __ldg(static_cast<const long long*>(labels.index) + row);
+      } else {
+        label[i] = __ldg(static_cast<const int*>(labels.index) + row);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = i * 1024 + threadIdx.x;
+      flags[at] = begin + at < rows && label[i] != (labels.teacher != nullptr ? 0 : labels.ignore_index);
     }
     __syncthreads();
     const uint2 mine8 = *reinterpret_cast<const uint2*>(flags + threadIdx.x * kEach);
@@ -250,13 +262,16 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int count = *a.rows.count, left = count - a.rows.piece_begin;
   const int rows_here = left < 0 ? 0 : (left < a.rows.piece_rows ? left : a.rows.piece_rows);
+  // A row belongs to gridDim.y CTAs, which all take its statistics and labels and then scale a part of it each.
   const int r = blockIdx.x;
   const int groups = (int)(a.ldg / 8);
+  const int part = (groups + gridDim.y - 1) / gridDim.y;
+  const int from = min(groups, part * (int)blockIdx.y), to = min(groups, from + part);
   uint4* g = a.g + (long long)r * groups;
   if (r >= rows_here) {
     // zeros behind the last row, to the end of its block of the contraction over rows
     if (a.g != nullptr && r < ((rows_here + 63) & ~63))
-      for (int i = tid; i < groups; i += kFinishThreads) g[i] = make_uint4(0u, 0u, 0u, 0u);
+      for (int i = from + tid; i < to; i += kFinishThreads) g[i] = make_uint4(0u, 0u, 0u, 0u);
     arrive_and_sum(a, count, scratch);
     return;
   }
@@ -315,7 +330,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     loss = a.labels.temperature * a.labels.temperature * block_reduce(part, scratch, false);
   }
   if (bad) loss = quiet_nan();  // a label outside the vocabulary
-  if (tid == 0) a.row_losses[n] = loss;
+  if (tid == 0 && blockIdx.y == 0) a.row_losses[n] = loss;
   arrive_and_sum(a, count, scratch);
   if (a.g == nullptr) return;
 
@@ -325,23 +340,33 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   if (a.grad_scale != nullptr) scale *= *a.grad_scale;
   if (loss != loss) scale = quiet_nan();
   __syncthreads();  // the tiles' factors and the shares
-  for (int i = tid; i < groups; i += kFinishThreads) {
-    const uint4 e = g[i];
-    const float f = scale * ex2_approx(factor[i / (kStatsTile / 8)]);
-    const uint32_t in[4] = {e.x, e.y, e.z, e.w};
-    uint32_t out[4];
+  for (int begin = from + tid; begin < to; begin += 4 * kFinishThreads) {
+    uint4 e[4];  // four pieces requested together
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (begin + j * kFinishThreads < to) e[j] = g[begin + j * kFinishThreads];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 t = Io16<__half>::unpack(in[j]);
-      out[j] = IO::pack(t.x * f, t.y * f);
+      const int i = begin + j * kFinishThreads;
+      if (i < to) {
+        const float f = scale * ex2_approx(factor[i / (kStatsTile / 8)]);
+        const uint32_t in[4] = {e[j].x, e[j].y, e[j].z, e[j].w};
+        uint32_t out[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const float2 t = Io16<__half>::unpack(in[h]);
+          out[h] = IO::pack(t.x * f, t.y * f);
+        }
+        g[i] = make_uint4(out[0], out[1], out[2], out[3]);
+      }
     }
-    g[i] = make_uint4(out[0], out[1], out[2], out[3]);
   }
   __syncthreads();
   if (bad) return;
   for (int k = tid; k < top; k += kFinishThreads) {
     if (a.labels.teacher != nullptr && a.labels.teacher[entry + k] == -INFINITY) continue;
     const long long v = a.labels.at(entry + k);
+    if (v < 8ll * from || v >= 8ll * to) continue;
     float p = 0.f;  // an index may occur more than once: each occurrence writes the same value
     for (int j = 0; j < top; ++j)
       if ((a.labels.teacher == nullptr || !(a.labels.teacher[entry + j] == -INFINITY)) && a.labels.at(entry + j) == v)
@@ -547,12 +572,15 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.loss = a.loss;
     f.arrived = count + 1;
     const bool by_warps = !grads && a.teacher_logits == nullptr;
+    // few rows are cut into parts, so that the device has two CTAs per SM to run (at most 16 parts of a row: one of 65536
+    // entries then is two rounds of requests)
+    const int parts = by_warps || !grads ? 1 : (l.piece_rows >= 148 ? 1 : (l.piece_rows > 18 ? 296 / l.piece_rows : 16));
     const int ctas = by_warps ? (l.piece_rows + kFinishThreads / 32 - 1) / (kFinishThreads / 32) : l.piece_rows;
-    f.ctas = ctas * l.pieces;
+    f.ctas = ctas * parts * l.pieces;
     if (by_warps)
       launch_chained(losses_kernel, dim3(ctas), dim3(kFinishThreads), 0, s, f);
     else
-      launch_chained(finish_kernel, dim3(ctas), dim3(kFinishThreads), finish_smem, s, f);
+      launch_chained(finish_kernel, dim3(ctas, parts), dim3(kFinishThreads), finish_smem, s, f);
     if (int rc = check_launch("finish_kernel")) return rc;
     if (a.grad_x != nullptr) {
       if (int rc = launch_grad_x(power, l.ldg, a.weight, here, a.channels, a.vocab, l.splits_x, a.grad_x, partial_x,
