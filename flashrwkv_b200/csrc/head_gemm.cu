@@ -18,6 +18,8 @@
 // Every wait is bounded; a role whose wait runs out sets the error flag and leaves, the others run into their own limits,
 // outputs that could not be made are NaN.
 
+#include <atomic>
+
 #include "head_loss.cuh"
 #include "umma_pair.cuh"
 
@@ -45,7 +47,8 @@ struct Params {
   CUtensorMap map_compact;  // kStats: A, kGradWeight: B, when some rows take no part
   CUtensorMap map_out;      // kStats: the exponentials, kGradWeight: the bf16 gradient
   Rows rows;
-  int channels, vocab, splits;
+  int channels, vocab;
+  Splits splits;           // kGradX, kGradWeight
   float log2_scale;        // kStats
   float2* stats;
   int stats_tiles;
@@ -72,7 +75,7 @@ struct Work {
     tiles_m = (m + kTile - 1) / kTile;
     tiles_n = (n + kTile - 1) / kTile;
     kb_total = (k + kBK - 1) / kBK;
-    splits = P == kStats ? 1 : p.splits;
+    splits = P == kStats || p.partials == nullptr ? 1 : *p.splits.chosen;
     units = tiles_m * tiles_n * splits;
   }
   // Pairs that run at the same time work on neighbouring tiles of the same part of the contraction, so that they share
@@ -291,7 +294,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
           }
         }
       } else {
-        const long long slot = (long long)u.split * (P == kGradX ? prm.rows.piece_rows : prm.vocab);
+        const long long slot = (long long)u.split * (P == kGradX ? rows_here : prm.vocab);
         const bool inside = m < m_end;
         const int row = P == kGradX && inside && prm.partials == nullptr ? prm.rows.row_map[prm.rows.piece_begin + m] : m;
         const bool wide = (prm.channels & 15) == 0 && (reinterpret_cast<uintptr_t>(prm.out) & 31u) == 0;
@@ -388,20 +391,19 @@ bool make_map(CUtensorMap* map, const void* base, long long rows, long long colu
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int pair_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      n < 2)
-    n = 148;
-  return n / 2;
-}
-
 long long tiles_of(long long n) { return (n + kTile - 1) / kTile; }
 
+// `units`: at most so many; a product with parts may be cut finer than the host knows and takes every pair
 template <Product P>
 int launch(const Params& prm, long long units, int* error_flag, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-  if (e != cudaSuccess) return fail(FRWKV_ERR_CUDA, "pretrain_head_loss: %s", cudaGetErrorString(e));
+  static std::atomic<bool> ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 64;
+  if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
+    cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    if (e != cudaSuccess) return fail(FRWKV_ERR_CUDA, "pretrain_head_loss: %s", cudaGetErrorString(e));
+    if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
+  }
   const int pairs = pair_count();
   const int grid = 2 * (int)(units < pairs ? units : pairs);
   launch_chained(head_gemm_kernel<P>, dim3(grid), dim3(kThreads), kSmem, stream, prm, error_flag);
@@ -412,24 +414,14 @@ int map_failure() { return fail(FRWKV_ERR_CUDA, "pretrain_head_loss: cuTensorMap
 
 }  // namespace
 
-// A wave of pairs takes one tile each, so the time goes with ceil(tiles * splits / pairs) / splits; every part is written
-// and read once more in fp32.
-int contraction_splits(long long rows, long long columns, long long k) {
-  const double pairs = pair_count(), tiles = (double)(tiles_of(rows) * tiles_of(columns));
-  const double block_us = 0.30;                                   // 256 x 256 x 64 by a pair, as measured
-  const double part_us = (double)(rows * columns) * 8 / 5.0e6;    // one fp32 part there and back
-  const long long blocks = (k + kBK - 1) / kBK;
-  int best = 1;
-  double best_us = 0;
-  for (int s = 1; s <= 64 && (s == 1 || blocks / s >= 4); ++s) {
-    const double waves = (double)(long long)((tiles * s + pairs - 1) / pairs);
-    const double us = waves * (double)((blocks + s - 1) / s) * block_us + (s > 1 ? 3.0 + s * part_us : 0.0);
-    if (s == 1 || us < best_us) {
-      best = s;
-      best_us = us;
-    }
-  }
-  return best;
+int pair_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 74;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 2) return 74;
+  if (dev < 64) known[dev].store(n / 2, std::memory_order_relaxed);
+  return n / 2;
 }
 
 int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
@@ -439,7 +431,6 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
   prm.rows = rows;
   prm.channels = channels;
   prm.vocab = vocab;
-  prm.splits = 1;
   prm.log2_scale = log2_scale;
   prm.stats = stats;
   prm.stats_tiles = (vocab + kStatsTile - 1) / kStatsTile;
@@ -452,8 +443,8 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
   return launch<kStats>(prm, tiles_of(rows.piece_rows) * tiles_of(vocab), error_flag, stream);
 }
 
-int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab, int splits,
-                  void* grad_x, float* partials, int* error_flag, cudaStream_t stream) {
+int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab,
+                  const Splits& splits, void* grad_x, float* partials, int* error_flag, cudaStream_t stream) {
   Params prm{};
   prm.rows = rows;
   prm.channels = channels;
@@ -464,11 +455,11 @@ int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& 
   if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kHalf) ||
       !make_map(&prm.map_b, weight, vocab, channels, channels, kBK))
     return map_failure();
-  return launch<kGradX>(prm, tiles_of(rows.piece_rows) * tiles_of(channels) * splits, error_flag, stream);
+  return launch<kGradX>(prm, tiles_of(rows.piece_rows) * tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1), error_flag, stream);
 }
 
 int launch_grad_weight(const void* g, long long ldg, const void* x, const void* x_compact, const Rows& rows, int channels,
-                       int vocab, int splits, void* grad_weight, float* partials, bool add, int* error_flag,
+                       int vocab, const Splits& splits, void* grad_weight, float* partials, bool add, int* error_flag,
                        cudaStream_t stream) {
   Params prm{};
   prm.rows = rows;
@@ -483,7 +474,7 @@ int launch_grad_weight(const void* g, long long ldg, const void* x, const void* 
       !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kBK) ||
       (partials == nullptr && !make_map(&prm.map_out, grad_weight, vocab, channels, channels, 32)))
     return map_failure();
-  return launch<kGradWeight>(prm, tiles_of(vocab) * tiles_of(channels) * splits, error_flag, stream);
+  return launch<kGradWeight>(prm, tiles_of(vocab) * tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1), error_flag, stream);
 }
 
 }  // namespace head

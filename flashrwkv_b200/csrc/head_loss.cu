@@ -67,14 +67,52 @@ __global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* _
   if (lane == 0) flags[row] = any;
 }
 
-// One CTA numbers the rows in order: position[row] = compact number or -1, row_map its inverse, count.  `position` holds
-// the teacher's flags on entry.
+// What the plan leaves on the device for the other kernels.
+struct Plan {
+  int count;     // rows that take part
+  int arrived;   // CTAs that have written their losses
+  int splits_x, splits_w;
+};
+struct SplitSizes {
+  int channels, vocab, most_x, most_w, pairs;
+  long long room_x;  // rows of fp32 parts of grad_x
+  bool fixed;        // several pieces: what the host has room for, whatever the count
+};
+
+// the cheapest number of parts, by one warp
+__device__ int choose_splits(int most, float rows, float columns, float k, float pairs, int lane) {
+  const float tiles = ceilf(rows / kTile) * ceilf(columns / kTile), blocks = ceilf(k / 64.f);
+  float best = INFINITY;
+  int which = 1;
+  for (int s = lane + 1; s <= most; s += 32) {
+    const float cost = s == 1 || blocks >= s * kLeastBlocks ? split_cost(s, tiles, blocks, rows * columns, pairs) : INFINITY;
+    if (cost < best) {
+      best = cost;
+      which = s;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float c = __shfl_xor_sync(0xffffffffu, best, o);
+    const int w = __shfl_xor_sync(0xffffffffu, which, o);
+    if (c < best || (c == best && w < which)) {
+      best = c;
+      which = w;
+    }
+  }
+  return which;
+}
+
+// One CTA numbers the rows in order: position[row] = compact number or -1, row_map its inverse.  `position` holds the
+// teacher's flags on entry.
 __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position, int* __restrict__ row_map,
-                                                    int* __restrict__ count, int* __restrict__ error_flag, int rows) {
+                                                    Plan* __restrict__ plan, SplitSizes sizes, int* __restrict__ error_flag,
+                                                    int rows) {
   chain_begin();
   constexpr int kEach = 8;  // consecutive rows of a thread; the flags come in row order through shared memory
   __shared__ int warp_sums[32];
-  __shared__ unsigned char flags[1024 * kEach];
+  __shared__ __align__(8) unsigned char flags[1024 * kEach];
+  __shared__ int list[1024 * kEach];  // the rows in use of this round, so that they leave in whole lines
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int done = 0;
   for (int begin = 0; begin < rows; begin += 1024 * kEach) {
@@ -107,22 +145,41 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
     if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
     const int others = warp_sums[lane];
-    int at = done + __reduce_add_sync(0xffffffffu, lane < warp ? others : 0) + upto - mine;
-    done += __reduce_add_sync(0xffffffffu, others);
+    int at = __reduce_add_sync(0xffffffffu, lane < warp ? others : 0) + upto - mine;
+    const int used_here = __reduce_add_sync(0xffffffffu, others);
+    const int first = begin + threadIdx.x * kEach;
+    int where[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int row = begin + threadIdx.x * kEach + i;
-      if (row >= rows) break;
       const bool used = ((i < 4 ? mine8.x : mine8.y) >> (8 * (i & 3))) & 1u;
-      position[row] = used ? at : -1;
-      if (used) row_map[at++] = row;
+      where[i] = used ? done + at : -1;
+      if (used) list[at++] = first + i;
+    }
+    if (first + kEach <= rows) {
+      reinterpret_cast<int4*>(position + first)[0] = make_int4(where[0], where[1], where[2], where[3]);
+      reinterpret_cast<int4*>(position + first)[1] = make_int4(where[4], where[5], where[6], where[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if (first + i < rows) position[first + i] = where[i];
     }
     __syncthreads();
+    for (int i = threadIdx.x; i < used_here; i += 1024) row_map[done + i] = list[i];
+    done += used_here;
+    __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    count[0] = done;
-    count[1] = 0;  // CTAs that have written their losses
-    *error_flag = 0;
+  if (warp == 0) {
+    int most_x = sizes.most_x, splits_x = most_x, splits_w = sizes.most_w;
+    if (!sizes.fixed && done > 0) {
+      // fewer rows than the host has made room for leave room for more parts
+      if (most_x > 1) most_x = (int)min((long long)kMaxSplits, sizes.room_x / done);
+      splits_x = choose_splits(most_x, (float)done, (float)sizes.channels, (float)sizes.vocab, (float)sizes.pairs, lane);
+      splits_w = choose_splits(sizes.most_w, (float)sizes.vocab, (float)sizes.channels, (float)done, (float)sizes.pairs, lane);
+    }
+    if (lane == 0) {
+      *plan = Plan{done, 0, splits_x, splits_w};
+      *error_flag = 0;
+    }
   }
 }
 
@@ -377,36 +434,71 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
 }
 
 // ---- small passes ------------------------------------------------------------------------------------------------------
-// out[row_map ? row_map[row_begin + row] : row][c] = sum of the parts in their order
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float4* __restrict__ partials, bf16* __restrict__ out,
-                                                        const int* __restrict__ row_map, const int* __restrict__ count,
-                                                        int row_begin, int part_rows, int pieces, int parts) {
+// out[row_map ? row_map[row_begin + row] : row][c] = sum of the parts.  A thread takes four columns of every kWarps-th part;
+// with eight warps to an output (many parts of few rows) their sums are added in warp order.
+template <int kWarps>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float4* __restrict__ partials, uint2* __restrict__ out,
+                                                        const int* __restrict__ row_map, const Plan* __restrict__ plan,
+                                                        bool of_x, int row_begin, int part_rows, int pieces) {
   chain_begin();
-  const int limit = row_map != nullptr ? *count - row_begin : part_rows;
+  constexpr int kOutputs = 256 / kWarps;
+  __shared__ float4 sums[kWarps > 1 ? kWarps - 1 : 1][32];
+  const int parts = of_x ? plan->splits_x : plan->splits_w;
+  const int limit = of_x ? plan->count - row_begin : part_rows;
   const long long rows = limit < part_rows ? limit : part_rows;
-  const long long total = rows * pieces, stride = (long long)part_rows * pieces * 2;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-    for (int s = 0; s < parts; s += 4) {  // four parts requested together (the last again where there are fewer)
-      float4 u[4], v[4];
+  const long long total = rows * pieces;  // rows <= 0: nothing
+  const int slice = kWarps > 1 ? threadIdx.x / 32 : 0, lane = threadIdx.x % kOutputs;
+  for (long long first = (long long)blockIdx.x * kOutputs; first < total; first += (long long)gridDim.x * kOutputs) {
+    const long long i = first + lane;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < total) {
+      for (int s = slice; s < parts; s += 4 * kWarps) {  // four parts requested together (the first again where there are fewer)
+        float4 u[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float4* q = partials + (s + j < parts ? s + j : parts - 1) * stride + 2 * i;
-        u[j] = __ldg(q);
-        v[j] = __ldg(q + 1);
-      }
+        for (int j = 0; j < 4; ++j) u[j] = __ldg(partials + (s + j * kWarps < parts ? s + j * kWarps : s) * total + i);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (s + j < parts) {
-          a.x += u[j].x; a.y += u[j].y; a.z += u[j].z; a.w += u[j].w;
-          b.x += v[j].x; b.y += v[j].y; b.z += v[j].z; b.w += v[j].w;
+        for (int j = 0; j < 4; ++j) {
+          if (s + j * kWarps < parts) {
+            a.x += u[j].x; a.y += u[j].y; a.z += u[j].z; a.w += u[j].w;
+          }
         }
       }
     }
-    const long long row = i / pieces;
-    const long long to = row_map != nullptr ? (long long)row_map[row_begin + row] * pieces + (i - row * pieces) : i;
-    reinterpret_cast<uint4*>(out)[to] = make_uint4(IO::pack(a.x, a.y), IO::pack(a.z, a.w), IO::pack(b.x, b.y), IO::pack(b.z, b.w));
+    if (kWarps > 1) {
+      if (slice > 0) sums[slice - 1][lane] = a;
+      __syncthreads();
+      if (slice == 0) {
+#pragma unroll
+        for (int j = 0; j < kWarps - 1; ++j) {
+          const float4 u = sums[j][lane];
+          a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+        }
+      }
+      __syncthreads();
+    }
+    if (slice == 0 && i < total) {
+      const long long row = i / pieces;
+      const long long to = of_x ? (long long)row_map[row_begin + row] * pieces + (i - row * pieces) : i;
+      out[to] = make_uint2(IO::pack(a.x, a.y), IO::pack(a.z, a.w));
+    }
   }
+}
+
+int launch_sum_parts(const float* partials, void* out, const int* row_map, const Plan* plan, bool of_x, int row_begin,
+                     int part_rows, int channels, int most, cudaStream_t s) {
+  const long long outputs = (long long)part_rows * (channels / 4);
+  if (most > 4) {
+    const long long ctas = (outputs + 31) / 32;
+    launch_chained(sum_parts_kernel<8>, dim3((unsigned)(ctas < 1184 ? ctas : 1184)), dim3(256), 0, s,
+                   reinterpret_cast<const float4*>(partials), static_cast<uint2*>(out), row_map, plan, of_x, row_begin, part_rows,
+                   channels / 4);
+  } else {
+    const long long ctas = (outputs + 255) / 256;
+    launch_chained(sum_parts_kernel<1>, dim3((unsigned)(ctas < 1184 ? ctas : 1184)), dim3(256), 0, s,
+                   reinterpret_cast<const float4*>(partials), static_cast<uint2*>(out), row_map, plan, of_x, row_begin, part_rows,
+                   channels / 4);
+  }
+  return check_launch("sum_parts_kernel");
 }
 
 // Both arrays *= *scale, in place; nothing to do where the scale is one.
@@ -435,13 +527,22 @@ struct Layout {
   long long ldg;
   int piece_rows, pieces, splits_x, splits_w;
   bool parts_x, parts_w;
-  size_t position, row_map, count, x_compact, stats, power, partial_x, partial_w, bytes;
+  size_t position, row_map, plan, x_compact, stats, power, partial_x, partial_w, bytes;
 };
 
 size_t take(size_t& at, size_t bytes) {
   const size_t here = at;
   at += (bytes + 255) & ~size_t(255);
   return here;
+}
+
+int splits_for(long long rows, long long columns, long long k) {
+  const float tiles = (float)((rows + kTile - 1) / kTile * ((columns + kTile - 1) / kTile)), blocks = (float)((k + 63) / 64);
+  const float pairs = (float)pair_count(), elements = (float)rows * (float)columns;
+  int best = 1;
+  for (int s = 2; s <= kMaxSplits && blocks >= s * kLeastBlocks; ++s)
+    if (split_cost(s, tiles, blocks, elements, pairs) < split_cost(best, tiles, blocks, elements, pairs)) best = s;
+  return best;
 }
 
 Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad_weight) {
@@ -457,12 +558,12 @@ Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad
   // pieces of equal size, whole tiles each; a single piece is the rows themselves
   l.piece_rows = l.pieces == 1 ? (int)rows : (int)(((rows + l.pieces - 1) / l.pieces + kTile - 1) / kTile * kTile);
   l.pieces = (int)((rows + l.piece_rows - 1) / l.piece_rows);
-  l.splits_x = grad_x ? contraction_splits(l.piece_rows, channels, vocab) : 1;
-  l.splits_w = grad_weight ? contraction_splits(vocab, channels, l.piece_rows) : 1;
+  l.splits_x = grad_x ? splits_for(l.piece_rows, channels, vocab) : 1;
+  l.splits_w = grad_weight ? splits_for(vocab, channels, l.piece_rows) : 1;
   l.parts_x = l.splits_x > 1;
   l.parts_w = l.splits_w > 1 || l.pieces > 1;
   size_t at = 0;
-  l.count = take(at, 16);
+  l.plan = take(at, sizeof(Plan));
   l.position = take(at, rows * 4);
   l.row_map = take(at, rows * 4);
   l.x_compact = take(at, (size_t)rows * channels * 2);
@@ -519,7 +620,8 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
                 "pretrain_head_loss: workspace is smaller than frwkv_pretrain_head_loss_workspace_bytes");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(a.workspace);
-  int* count = reinterpret_cast<int*>(ws + l.count);
+  Plan* plan = reinterpret_cast<Plan*>(ws + l.plan);
+  const int* count = &plan->count;
   int* position = reinterpret_cast<int*>(ws + l.position);
   int* row_map = reinterpret_cast<int*>(ws + l.row_map);
   float2* stats = reinterpret_cast<float2*>(ws + l.stats);
@@ -542,7 +644,9 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     launch_chained(teacher_rows_kernel, by_warp, dim3(256), 0, s, labels, position, rows);
     if (int rc = check_launch("teacher_rows_kernel")) return rc;
   }
-  launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, position, row_map, count, a.error_flag, rows);
+  const SplitSizes sizes{a.channels, a.vocab, l.splits_x, l.splits_w, pair_count(), (long long)l.splits_x * l.piece_rows,
+                         l.pieces > 1};
+  launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, position, row_map, plan, sizes, a.error_flag, rows);
   if (int rc = check_launch("plan_kernel")) return rc;
   launch_chained(compact_kernel, by_warp, dim3(256), 0, s, static_cast<const uint4*>(a.x), position, count,
                  reinterpret_cast<uint4*>(ws + l.x_compact), static_cast<uint4*>(a.grad_x), a.row_losses, rows, x_pieces);
@@ -570,7 +674,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.grad_scale = a.grad_scale;
     f.row_losses = a.row_losses;
     f.loss = a.loss;
-    f.arrived = count + 1;
+    f.arrived = &plan->arrived;
     const bool by_warps = !grads && a.teacher_logits == nullptr;
     // few rows are cut into parts, so that the device has two CTAs per SM to run (at most 16 parts of a row: one of 65536
     // entries then is two rounds of requests)
@@ -583,26 +687,21 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
       launch_chained(finish_kernel, dim3(ctas, parts), dim3(kFinishThreads), finish_smem, s, f);
     if (int rc = check_launch("finish_kernel")) return rc;
     if (a.grad_x != nullptr) {
-      if (int rc = launch_grad_x(power, l.ldg, a.weight, here, a.channels, a.vocab, l.splits_x, a.grad_x, partial_x,
+      if (int rc = launch_grad_x(power, l.ldg, a.weight, here, a.channels, a.vocab, Splits{&plan->splits_x, l.splits_x}, a.grad_x, partial_x,
                                  a.error_flag, s))
         return rc;
-      if (l.parts_x) {
-        launch_chained(sum_parts_kernel, dim3(592), dim3(256), 0, s, reinterpret_cast<const float4*>(partial_x),
-                       static_cast<bf16*>(a.grad_x), row_map, count, here.piece_begin, l.piece_rows, x_pieces, l.splits_x);
-        if (int rc = check_launch("sum_parts_kernel")) return rc;
-      }
+      if (l.parts_x)
+        if (int rc = launch_sum_parts(partial_x, a.grad_x, row_map, plan, true, here.piece_begin, l.piece_rows, a.channels,
+                                      l.splits_x, s))
+          return rc;
     }
     if (a.grad_weight != nullptr)
-      if (int rc = launch_grad_weight(power, l.ldg, a.x, ws + l.x_compact, here, a.channels, a.vocab, l.splits_w, a.grad_weight,
-                                      partial_w, piece > 0, a.error_flag, s))
+      if (int rc = launch_grad_weight(power, l.ldg, a.x, ws + l.x_compact, here, a.channels, a.vocab,
+                                      Splits{&plan->splits_w, l.splits_w}, a.grad_weight, partial_w, piece > 0, a.error_flag, s))
         return rc;
   }
-  if (a.grad_weight != nullptr && l.parts_w) {
-    launch_chained(sum_parts_kernel, dim3(592), dim3(256), 0, s, reinterpret_cast<const float4*>(partial_w),
-                   static_cast<bf16*>(a.grad_weight), static_cast<const int*>(nullptr), count, 0, a.vocab, x_pieces,
-                   l.splits_w);
-    if (int rc = check_launch("sum_parts_kernel")) return rc;
-  }
+  if (a.grad_weight != nullptr && l.parts_w)
+    if (int rc = launch_sum_parts(partial_w, a.grad_weight, row_map, plan, false, 0, a.vocab, a.channels, l.splits_w, s)) return rc;
   return FRWKV_OK;
 }
 

@@ -26,19 +26,33 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
                        float log2_scale, float2* stats, void* power, long long ldp, int* error_flag,
                        cudaStream_t stream);
 
-// How many parts the contraction of a rows x columns product over k is cut into.
-int contraction_splits(long long rows, long long columns, long long k);
+// The time of a rows x columns product whose contraction of `blocks` blocks of 64 is cut into s parts: a wave of pairs takes
+// one tile and part each (0.42 us per 256 x 256 x 64, as measured), and every part is written and read once more in fp32.
+__host__ __device__ inline float split_cost(int s, float tiles, float blocks, float elements, float pairs) {
+  const float waves = ceilf(tiles * (float)s / pairs);
+  return waves * ceilf(blocks / (float)s) * 0.42f + (s > 1 ? 3.f + (float)s * elements * (8.f / 5.0e6f) : 0.f);
+}
+constexpr int kMaxSplits = 64;
+constexpr float kLeastBlocks = 4.f;  // of a part
 
-// grad_x[row_map[row]] = g[row] W, contraction over the vocabulary in `splits` parts: with one part bf16 rows go straight to
-// grad_x, with more the fp32 parts go to partials[split][piece_rows][channels].
-int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab, int splits,
-                  void* grad_x, float* partials, int* error_flag, cudaStream_t stream);
+// The parts in use are chosen where the number of rows is known, by plan_kernel, from 1 to what the host has room for.
+struct Splits {
+  const int* chosen;  // device
+  int most;           // partial sums have room for `most` parts of all rows; 1: none are kept
+};
 
-// grad_weight = g^T x, contraction over the rows of the piece in `splits` parts: bf16 straight to grad_weight, or (partials
-// given) fp32 parts in partials[split][vocab][channels], added to what they hold where `add`.
+// grad_x[row_map[row]] = g[row] W, contraction over the vocabulary: with room for one part bf16 rows go straight to grad_x,
+// else fp32 parts to partials[part][rows that take part][channels].
+int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab,
+                  const Splits& splits, void* grad_x, float* partials, int* error_flag, cudaStream_t stream);
+
+// grad_weight = g^T x, contraction over the rows of the piece: bf16 straight to grad_weight, or (partials given) fp32 parts in
+// partials[part][vocab][channels], added to what they hold where `add`.
 int launch_grad_weight(const void* g, long long ldg, const void* x, const void* x_compact, const Rows& rows, int channels,
-                       int vocab, int splits, void* grad_weight, float* partials, bool add, int* error_flag,
+                       int vocab, const Splits& splits, void* grad_weight, float* partials, bool add, int* error_flag,
                        cudaStream_t stream);
+
+int pair_count();  // of CTAs that the current device runs at once
 
 }  // namespace head
 }  // namespace frwkv
