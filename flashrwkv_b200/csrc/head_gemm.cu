@@ -166,21 +166,25 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   bool ok = true;
 
+  const auto wait = [](uint64_t* bar, uint32_t parity) {  // by a whole warp, one outcome for all of it
+    return __all_sync(0xffffffffu, umma::mbar_wait(bar, parity)) != 0;
+  };
   if (warp == 0) {
-    if (lane == 0) {
-      const CUtensorMap* map_a = P == kStats && compact ? &prm.map_compact : &prm.map_a;
-      const CUtensorMap* map_b = P == kGradWeight && compact ? &prm.map_compact : &prm.map_b;
-      const int a_row = P == kStats ? prm.rows.piece_begin : 0, b_row = P == kGradWeight ? prm.rows.piece_begin : 0;
-      uint32_t it = 0;
-      for (int unit = pair; unit < work.units && ok; unit += pairs) {
-        const Unit u = work.at(unit);
-        for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
-          const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
-          if (!umma2::wait_cluster(&empty_bar[s], ph ^ 1u)) { ok = false; break; }
-          const uint32_t full = umma2::in_leader(&full_bar[s]);
+    const CUtensorMap* map_a = P == kStats && compact ? &prm.map_compact : &prm.map_a;
+    const CUtensorMap* map_b = P == kGradWeight && compact ? &prm.map_compact : &prm.map_b;
+    const int a_row = P == kStats ? prm.rows.piece_begin : 0, b_row = P == kGradWeight ? prm.rows.piece_begin : 0;
+    uint32_t it = 0;
+    for (int unit = pair; unit < work.units && ok; unit += pairs) {
+      const Unit u = work.at(unit);
+      const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * (u.width / 2);
+      for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
+        const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
+        if (!wait(&empty_bar[s], ph ^ 1u)) { ok = false; break; }
+        const uint32_t full = umma2::in_leader(&full_bar[s]);
+        const uint32_t a_dst = tiles_base + s * kStageBytes, b_dst = a_dst + kOperandBytes;
+        const int k = kb * kBK;
+        if (umma2::elect_one()) {
           if (rank == 0) umma::mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
-          const uint32_t a_dst = tiles_base + s * kStageBytes, b_dst = a_dst + kOperandBytes;
-          const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * (u.width / 2), k = kb * kBK;
           if (kAMn) {
             umma2::tma_load_2d(a_dst, map_a, m, a_row + k, full);
             umma2::tma_load_2d(a_dst + 8192, map_a, m + 64, a_row + k, full);
@@ -194,38 +198,44 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
             umma2::tma_load_2d(b_dst, map_b, k, n, full);
           }
         }
-      }
-      // the last commits must have arrived here before this CTA may leave
-      for (uint32_t i = 0; i < (uint32_t)kStages && i < it && ok; ++i) {
-        const uint32_t j = it - 1 - i;
-        if (!umma2::wait_cluster(&empty_bar[j % kStages], (j / kStages) & 1u)) ok = false;
+        __syncwarp();
       }
     }
+    // the last commits must have arrived here before this CTA may leave
+    for (uint32_t i = 0; i < (uint32_t)kStages && i < it && ok; ++i) {
+      const uint32_t j = it - 1 - i;
+      if (!wait(&empty_bar[j % kStages], (j / kStages) & 1u)) ok = false;
+    }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      const uint64_t a_desc = kAMn ? umma2::desc_mn_major(tiles_base) : umma2::desc_k_major(tiles_base);
+      const uint64_t b_desc = kBMn ? umma2::desc_mn_major(tiles_base + kOperandBytes) : umma2::desc_k_major(tiles_base + kOperandBytes);
+      constexpr uint32_t kAStep = (kAMn ? 2048 : 32) >> 4, kBStep = (kBMn ? 2048 : 32) >> 4;  // 16 contraction values
       uint32_t it = 0, t = 0;
       for (int unit = pair; unit < work.units && ok; unit += pairs) {
         const Unit u = work.at(unit);
         if (u.kb_begin == u.kb_end) continue;  // nothing to contract: the epilogue writes zeros
         const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
         ++t;
-        if (!umma2::wait_cluster(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
+        if (!wait(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
         umma::fence_after_sync();
         const uint32_t d_tmem = tmem + acc * kTile;
         const uint32_t idesc = umma2::idesc_bf16(u.width, kAMn, kBMn);
         for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
-          if (!umma2::wait_cluster(&full_bar[s], ph)) { ok = false; break; }
+          if (!wait(&full_bar[s], ph)) { ok = false; break; }
           umma::fence_after_sync();
-          const uint32_t a = tiles_base + s * kStageBytes, b = a + kOperandBytes;
+          const uint64_t a = a_desc + s * (kStageBytes >> 4), b = b_desc + s * (kStageBytes >> 4);
+          if (umma2::elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kBK / 16; ++ks)
-            umma2::mma_bf16(d_tmem, kAMn ? umma2::desc_mn_major(a + ks * 2048) : umma2::desc_k_major(a + ks * 32),
-                            kBMn ? umma2::desc_mn_major(b + ks * 2048) : umma2::desc_k_major(b + ks * 32), idesc,
-                            (kb > u.kb_begin || ks > 0) ? 1u : 0u);
-          umma2::commit_both(&empty_bar[s]);
+            for (int ks = 0; ks < kBK / 16; ++ks)
+              umma2::mma_bf16(d_tmem, a + ks * kAStep, b + ks * kBStep, idesc, (kb > u.kb_begin || ks > 0) ? 1u : 0u);
+            umma2::commit_both(&empty_bar[s]);
+          }
+          __syncwarp();
         }
-        if (ok) umma2::commit_both(&acc_full[acc]);
+        if (ok && umma2::elect_one()) umma2::commit_both(&acc_full[acc]);
+        __syncwarp();
       }
     }
   } else {
@@ -243,7 +253,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
       if (!empty) ++t;
       // Warp-uniform outcome: the tensor-memory loads below need the whole warp.  Once a wait has run out, this unit and all
       // later ones read as NaN.
-      if (ok && !empty && !__all_sync(0xffffffffu, umma2::wait_cluster(&acc_full[acc], aph))) ok = false;
+      if (ok && !empty && !wait(&acc_full[acc], aph)) ok = false;
       umma::fence_after_sync();
       const uint32_t source = source0 + acc * kTile;
       const int m = u.m0 + row_in_tile, n = u.n0 + column0;

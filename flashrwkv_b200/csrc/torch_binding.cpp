@@ -2076,7 +2076,7 @@ HeadResult head_pass(const HeadInputs& in, bool mean, bool want_x, bool want_wei
   const int64_t channels = in.x.size(-1), rows = in.x.numel() / channels, vocab = in.weight.size(0);
   const auto f32 = in.x.options().dtype(torch::kFloat32);
   HeadResult out;
-  out.row_losses = torch::empty({rows}, f32);
+  out.row_losses = torch::empty(in.x.sizes().slice(0, in.x.dim() - 1), f32);
   out.loss = torch::empty({}, f32);
   if (want_x) out.grad_x = torch::empty_like(in.x);
   if (want_weight) out.grad_weight = torch::empty_like(in.weight);
@@ -2129,7 +2129,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     if (scalar && (want_x || want_weight)) {
       ctx->saved_data["grads"] = c10::IValue(std::make_tuple(r.grad_x, r.grad_weight));
     }
-    return scalar ? r.loss : r.row_losses.view(x.sizes().slice(0, x.dim() - 1));
+    return scalar ? r.loss : r.row_losses;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {

@@ -22,6 +22,20 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// true in one lane; the whole warp calls it.  Tensor-core and TMA instructions take their operands from uniform registers: a
+// warp that runs its loop together and elects a lane for the instruction alone keeps them there, where a loop of one lane
+// moves every operand over (656 cycles per block of four MMAs against the 512 they run).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}\n"
+      : "=r"(e));
+  return e != 0;
+}
 // the address of the same shared-memory object in the leader CTA
 __device__ __forceinline__ uint32_t in_leader(const void* p) {
   uint32_t r;
@@ -81,24 +95,6 @@ __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_g
 __device__ __forceinline__ void arrive_cluster(uint32_t mbar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mbar) : "memory");
 }
-// bounded wait on a barrier of this CTA that the other CTA's threads arrive on
-__device__ __forceinline__ bool wait_cluster(uint64_t* mbar, uint32_t parity, uint32_t limit = (1u << 22)) {
-  for (uint32_t i = 0; i < limit; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t"
-        "}\n"
-        : "=r"(done)
-        : "r"(smem_u32(mbar)), "r"(parity)
-        : "memory");
-    if (done != 0) return true;
-  }
-  return false;
-}
-
 // Shared-memory descriptors of the two 16-bit operand forms that TMA writes with 128-byte swizzle: rows of 64 contraction
 // values ("K-major": eight rows are 1024 bytes), or rows that run along the other axis and are indexed by the contraction
 // ("MN-major": boxes of 64 columns x 64 rows, 8192 bytes apart).
