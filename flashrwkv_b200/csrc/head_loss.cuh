@@ -27,10 +27,10 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
                        cudaStream_t stream);
 
 // The time of a rows x columns product whose contraction of `blocks` blocks of 64 is cut into s parts: a wave of pairs takes
-// one tile and part each (0.42 us per 256 x 256 x 64, as measured), and every part is written and read once more in fp32.
+// one tile and part each (0.34 us per 256 x 256 x 64, as measured), and every part is written and read once more in fp32.
 __host__ __device__ inline float split_cost(int s, float tiles, float blocks, float elements, float pairs) {
   const float waves = ceilf(tiles * (float)s / pairs);
-  return waves * ceilf(blocks / (float)s) * 0.42f + (s > 1 ? 3.f + (float)s * elements * (8.f / 5.0e6f) : 0.f);
+  return waves * ceilf(blocks / (float)s) * 0.34f + (s > 1 ? 3.f + (float)s * elements * (8.f / 5.0e6f) : 0.f);
 }
 constexpr int kMaxSplits = 64;
 constexpr float kLeastBlocks = 4.f;  // of a part
