@@ -139,6 +139,10 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
   const uint32_t tiles_base = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
 
   chain_release();
+  if (tid == 32) {  // the maps are parameters of this launch: fetched while the kernel before still runs
+    umma2::prefetch_map(&prm.map_a);
+    umma2::prefetch_map(&prm.map_b);
+  }
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       umma::mbar_init(&full_bar[i], 1);   // the leader's producer; the bytes of both CTAs

@@ -19,6 +19,7 @@
 //
 // The reference has the inference forms only (flashrwkv2/tmix/normalization/__init__.py:31-90).
 
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -420,11 +421,31 @@ constexpr int kMaxChannels = 512 * 4 * 8;
 constexpr int kSlabsPerSm = 2;
 constexpr int kForwardPieces = 4, kBackwardPieces = 2;
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return n > 0 ? n : 148;
+constexpr int kKnownDevices = 64;  // what a device answered once is kept: the queries cost as much as a launch
+
+int sm_count(int dev) {
+  static std::atomic<int> known[kKnownDevices];
+  int n = 0;
+  if (dev < kKnownDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev < kKnownDevices) known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+int current_device() {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
+}
+
+// CTAs of a kernel that an SM holds, 0 on an error
+template <auto kernel>
+int resident_ctas(int dev, int threads) {
+  static std::atomic<int> known[kKnownDevices];
+  int n = 0;
+  if (dev < kKnownDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess) return 0;
+  if (dev < kKnownDevices) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 
 struct NormPlan {
@@ -432,8 +453,8 @@ struct NormPlan {
   long long rows_per_cta;
 };
 // Slabs of at least four rows, and no more than `resident` CTAs per SM at once: fewer slabs mean fewer partials.
-NormPlan plan_backward(long long rows, int resident) {
-  const long long most = (long long)sm_count() * resident;
+NormPlan plan_backward(long long rows, int resident, int dev) {
+  const long long most = (long long)sm_count(dev) * resident;
   long long slabs = (rows + 3) / 4;
   if (slabs > most) slabs = most;
   const long long per = (rows + slabs - 1) / slabs;
@@ -497,7 +518,7 @@ extern "C" int frwkv_pretrain_layer_norm_forward(const void* x, const void* resi
 
 extern "C" long long frwkv_pretrain_layer_norm_workspace_floats(long long rows, int channels) {
   if (rows <= 0 || channels <= 0) return 0;
-  const long long slabs = frwkv::plan_backward(rows, frwkv::kSlabsPerSm).slabs;
+  const long long slabs = frwkv::plan_backward(rows, frwkv::kSlabsPerSm, frwkv::current_device()).slabs;
   return slabs * 2 * channels;
 }
 
@@ -522,18 +543,24 @@ extern "C" int frwkv_pretrain_layer_norm_backward(const void* grad_out, const vo
     constexpr int T = decltype(t)::value, V = decltype(v)::value;
     constexpr bool kApart = T > 512;  // the column sums take a pass of their own
     const bool parameters = grad_weight != nullptr;
-    const auto kernel = parameters && !kApart
-                            ? (grad_sum != nullptr ? norm_backward_kernel<T, V, true, !kApart> : norm_backward_kernel<T, V, false, !kApart>)
-                            : (grad_sum != nullptr ? norm_backward_kernel<T, V, true, false> : norm_backward_kernel<T, V, false, false>);
-    int resident = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, backward_threads(T), 0) != cudaSuccess || resident < 1)
-      return fail(FRWKV_ERR_CUDA, "pretrain_layer_norm_backward: %s", cudaGetErrorString(cudaGetLastError()));
-    const NormPlan plan = plan_backward(rows, resident < kSlabsPerSm ? resident : kSlabsPerSm);
-    launch_chained(kernel, dim3(plan.slabs), dim3(backward_threads(T)), 0, s, static_cast<const bf16*>(grad_out),
-                   static_cast<const bf16*>(grad_sum), static_cast<const bf16*>(sum), static_cast<const bf16*>(weight), mean,
-                   rstd, static_cast<bf16*>(grad_x), static_cast<bf16*>(grad_weight), static_cast<bf16*>(grad_bias),
-                   workspace, rows, channels, plan.rows_per_cta);
-    if (int rc = check_launch("norm_backward_kernel")) return rc;
+    NormPlan plan{};
+    const auto run = [&](auto sum_known, auto params) {
+      constexpr auto kernel = norm_backward_kernel<T, V, decltype(sum_known)::value, decltype(params)::value>;
+      const int dev = current_device(), resident = resident_ctas<kernel>(dev, backward_threads(T));
+      if (resident < 1) return fail(FRWKV_ERR_CUDA, "pretrain_layer_norm_backward: no CTA fits an SM");
+      plan = plan_backward(rows, resident < kSlabsPerSm ? resident : kSlabsPerSm, dev);
+      launch_chained(kernel, dim3(plan.slabs), dim3(backward_threads(T)), 0, s, static_cast<const bf16*>(grad_out),
+                     static_cast<const bf16*>(grad_sum), static_cast<const bf16*>(sum), static_cast<const bf16*>(weight), mean,
+                     rstd, static_cast<bf16*>(grad_x), static_cast<bf16*>(grad_weight), static_cast<bf16*>(grad_bias),
+                     workspace, rows, channels, plan.rows_per_cta);
+      return check_launch("norm_backward_kernel");
+    };
+    constexpr std::bool_constant<true> yes{};
+    constexpr std::bool_constant<false> no{};
+    constexpr std::bool_constant<!kApart> here{};
+    const int launched = parameters ? (grad_sum != nullptr ? run(yes, here) : run(no, here))
+                                    : (grad_sum != nullptr ? run(yes, no) : run(no, no));
+    if (launched != FRWKV_OK) return launched;
     if (!parameters || (plan.slabs == 1 && !kApart)) return (int)FRWKV_OK;
     if (kApart) {
       launch_chained(norm_columns_kernel, dim3((channels + 255) / 256, plan.slabs), dim3(128), 0, s,

@@ -73,6 +73,9 @@ __device__ __forceinline__ void commit_both(uint64_t* mbar) {
       : "memory");
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // A tile into this CTA's shared memory, its bytes counted on `mbar` (a cluster address: the leader's barrier)
 __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
   asm volatile(
