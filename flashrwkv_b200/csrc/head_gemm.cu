@@ -165,7 +165,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
   const int count = *prm.rows.count;
   const int left = count - prm.rows.piece_begin;
   const int rows_here = left < 0 ? 0 : (left < prm.rows.piece_rows ? left : prm.rows.piece_rows);
-  const bool compact = count != prm.rows.total;
+  const bool compact = prm.rows.copied || count != prm.rows.total;
   const Work<P> work(prm, rows_here);
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   bool ok = true;
@@ -450,7 +450,7 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
   prm.stats_tiles = (vocab + kStatsTile - 1) / kStatsTile;
   prm.power = power != nullptr;
   if (!make_map(&prm.map_a, x, rows.total, channels, channels, kHalf) ||
-      !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kHalf) ||
+      !make_map(&prm.map_compact, x_compact, rows.total, channels, rows.ldx, kHalf) ||
       !make_map(&prm.map_b, weight, vocab, channels, channels, kHalf) ||
       (power != nullptr && !make_map(&prm.map_out, power, rows.piece_rows, ldp, ldp, 32)))
     return map_failure();
@@ -485,7 +485,7 @@ int launch_grad_weight(const void* g, long long ldg, const void* x, const void* 
   prm.add = add;
   if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kBK) ||
       !make_map(&prm.map_b, x, rows.total, channels, channels, kBK) ||
-      !make_map(&prm.map_compact, x_compact, rows.total, channels, channels, kBK) ||
+      !make_map(&prm.map_compact, x_compact, rows.total, channels, rows.ldx, kBK) ||
       (partials == nullptr && !make_map(&prm.map_out, grad_weight, vocab, channels, channels, 32)))
     return map_failure();
   return launch<kGradWeight>(prm, tiles_of(vocab) * tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1), error_flag, stream);

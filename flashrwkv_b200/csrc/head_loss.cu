@@ -42,6 +42,7 @@ constexpr int kMaxTop = 512;
 // logits into exponents makes the mean good; what remains of a logit's error is random, 3e-7.
 constexpr double kTruncation = 1.03e-9;
 constexpr int kFinishThreads = 256;
+constexpr int kFewRows = 64;
 
 struct Labels {
   const void* index;        // [rows][top] int32 or int64
@@ -65,6 +66,40 @@ __global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* _
   for (int k = lane; k < labels.top; k += 32) any |= !(labels.teacher[(long long)row * labels.top + k] == -INFINITY);
   any = __any_sync(0xffffffffu, any);
   if (lane == 0) flags[row] = any;
+}
+
+// Copies the rows that take part together; the others get a zero loss and a zero gradient.  The rows behind the last, up
+// to the next multiple of 64, become zeros: they meet zeros of g in a block of the contraction over rows.  Where every row
+// takes part there is nothing to do, unless rows that are not whole 128-byte lines apart are copied to lines of their own
+// (`always`): TMA reads such rows a quarter slower.
+struct CompactArgs {
+  const uint4* x;
+  const int* position;
+  uint4* x_compact;
+  uint4* grad_x;
+  float* row_losses;
+  int rows, pieces, pitch;  // in 16-byte pieces
+  bool always;
+};
+__device__ __forceinline__ void compact_row(const CompactArgs& a, int row, int used, int lane) {
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  const int at = a.position[row];
+  const bool tail = row >= used && row < ((used + 63) & ~63);
+  for (int p = lane; p < a.pieces; p += 32) {
+    if (at >= 0) {
+      a.x_compact[(long long)at * a.pitch + p] = __ldg(a.x + (long long)row * a.pieces + p);
+    } else if (a.grad_x != nullptr) {
+      a.grad_x[(long long)row * a.pieces + p] = zero;
+    }
+    if (tail) a.x_compact[(long long)row * a.pitch + p] = zero;
+  }
+  if (lane == 0 && at < 0) a.row_losses[row] = 0.f;
+}
+__global__ __launch_bounds__(256) void compact_kernel(CompactArgs a, const int* __restrict__ count) {
+  chain_begin();
+  const int used = *count, row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if ((used == a.rows && !a.always) || row >= a.rows) return;
+  compact_row(a, row, used, threadIdx.x & 31);
 }
 
 // What the plan leaves on the device for the other kernels.
@@ -106,8 +141,8 @@ __device__ int choose_splits(int most, float rows, float columns, float k, float
 // One CTA numbers the rows in order: position[row] = compact number or -1, row_map its inverse.  `position` holds the
 // teacher's flags on entry.
 __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position, int* __restrict__ row_map,
-                                                    Plan* __restrict__ plan, SplitSizes sizes, int* __restrict__ error_flag,
-                                                    int rows) {
+                                                    Plan* __restrict__ plan, SplitSizes sizes, CompactArgs compact,
+                                                    int* __restrict__ error_flag, int rows) {
   chain_begin();
   constexpr int kEach = 8;  // consecutive rows of a thread; the flags come in row order through shared memory
   __shared__ int warp_sums[32];
@@ -181,30 +216,9 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
       *error_flag = 0;
     }
   }
-}
-
-// Copies the rows that take part together; the others get a zero loss and a zero gradient.  The rows behind the last, up
-// to the next multiple of 64, become zeros: they meet zeros of g in a block of the contraction over rows.
-__global__ __launch_bounds__(256) void compact_kernel(const uint4* __restrict__ x, const int* __restrict__ position,
-                                                      const int* __restrict__ count, uint4* __restrict__ x_compact,
-                                                      uint4* __restrict__ grad_x, float* __restrict__ row_losses, int rows,
-                                                      int pieces) {
-  chain_begin();
-  const int used = *count;
-  if (used == rows) return;
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  const int at = position[row];
-  for (int p = lane; p < pieces; p += 32) {
-    if (at >= 0) {
-      x_compact[(long long)at * pieces + p] = __ldg(x + (long long)row * pieces + p);
-    } else if (grad_x != nullptr) {
-      grad_x[(long long)row * pieces + p] = zero;
-    }
-    if (row >= used && row < ((used + 63) & ~63)) x_compact[(long long)row * pieces + p] = zero;
-  }
-  if (lane == 0 && at < 0) row_losses[row] = 0.f;
+  // a few rows are copied here, by a warp each, rather than by a launch of their own
+  if (rows <= kFewRows && (done < rows || compact.always))
+    for (int row = warp; row < rows; row += 32) compact_row(compact, row, done, lane);
 }
 
 // ---- finish: statistics to losses and logit gradients ------------------------------------------------------------------
@@ -333,6 +347,10 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     return;
   }
   const long long n = a.rows.row_map[a.rows.piece_begin + r];
+  uint4 e[4];  // four of the row's pieces at a time, the first of them requested ahead of all else
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (a.g != nullptr && from + tid + j * kFinishThreads < to) e[j] = g[from + tid + j * kFinishThreads];
 
   // the softmax's normaliser, in units of log2
   const float2* stats = a.stats + (long long)r * tiles;
@@ -398,10 +416,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   if (loss != loss) scale = quiet_nan();
   __syncthreads();  // the tiles' factors and the shares
   for (int begin = from + tid; begin < to; begin += 4 * kFinishThreads) {
-    uint4 e[4];  // four pieces requested together
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (begin + j * kFinishThreads < to) e[j] = g[begin + j * kFinishThreads];
+    uint4 out4[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = begin + j * kFinishThreads;
@@ -414,9 +429,15 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
           const float2 t = Io16<__half>::unpack(in[h]);
           out[h] = IO::pack(t.x * f, t.y * f);
         }
-        g[i] = make_uint4(out[0], out[1], out[2], out[3]);
+        out4[j] = make_uint4(out[0], out[1], out[2], out[3]);
       }
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)  // the next four are under way before these leave
+      if (begin + (4 + j) * kFinishThreads < to) e[j] = g[begin + (4 + j) * kFinishThreads];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (begin + j * kFinishThreads < to) g[begin + j * kFinishThreads] = out4[j];
   }
   __syncthreads();
   if (bad) return;
@@ -524,7 +545,7 @@ __global__ __launch_bounds__(256) void scale_kernel(uint4* __restrict__ first, l
 // ---- host side ---------------------------------------------------------------------------------------------------------
 // The workspace of a call; sizes depend on the shapes and on which gradients are wanted, not on the labels.
 struct Layout {
-  long long ldg;
+  long long ldg, ldx;
   int piece_rows, pieces, splits_x, splits_w;
   bool parts_x, parts_w;
   size_t position, row_map, plan, x_compact, stats, power, partial_x, partial_w, bytes;
@@ -549,6 +570,7 @@ Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad
   Layout l{};
   const bool grads = grad_x || grad_weight;
   l.ldg = ((long long)vocab + 63) / 64 * 64;
+  l.ldx = ((long long)channels + 63) / 64 * 64;
   const long long tiles = (vocab + kStatsTile - 1) / kStatsTile;
   long long most = kStatsBytes / (8 * tiles);
   if (grads && kPieceBytes / (2 * l.ldg) < most) most = kPieceBytes / (2 * l.ldg);
@@ -566,7 +588,7 @@ Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad
   l.plan = take(at, sizeof(Plan));
   l.position = take(at, rows * 4);
   l.row_map = take(at, rows * 4);
-  l.x_compact = take(at, (size_t)rows * channels * 2);
+  l.x_compact = take(at, (size_t)rows * l.ldx * 2);
   l.stats = take(at, (size_t)tiles * l.piece_rows * 8);
   l.power = take(at, grads ? (size_t)l.piece_rows * l.ldg * 2 : 0);
   l.partial_x = take(at, grad_x && l.parts_x ? (size_t)l.splits_x * l.piece_rows * channels * 4 : 0);
@@ -628,7 +650,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   void* power = grads ? ws + l.power : nullptr;
   float* partial_x = l.parts_x ? reinterpret_cast<float*>(ws + l.partial_x) : nullptr;
   float* partial_w = l.parts_w ? reinterpret_cast<float*>(ws + l.partial_w) : nullptr;
-  const int rows = (int)a.rows, x_pieces = a.channels / 8, tiles = (a.vocab + kStatsTile - 1) / kStatsTile;
+  const int rows = (int)a.rows, tiles = (a.vocab + kStatsTile - 1) / kStatsTile;
 
   Labels labels{};
   labels.index = a.labels;
@@ -646,15 +668,26 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   }
   const SplitSizes sizes{a.channels, a.vocab, l.splits_x, l.splits_w, pair_count(), (long long)l.splits_x * l.piece_rows,
                          l.pieces > 1};
-  launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, position, row_map, plan, sizes, a.error_flag, rows);
+  CompactArgs compact{};
+  compact.x = static_cast<const uint4*>(a.x);
+  compact.position = position;
+  compact.x_compact = reinterpret_cast<uint4*>(ws + l.x_compact);
+  compact.grad_x = static_cast<uint4*>(a.grad_x);
+  compact.row_losses = a.row_losses;
+  compact.rows = rows;
+  compact.pieces = a.channels / 8;
+  compact.pitch = (int)(l.ldx / 8);
+  compact.always = l.ldx != a.channels;
+  launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, position, row_map, plan, sizes, compact, a.error_flag, rows);
   if (int rc = check_launch("plan_kernel")) return rc;
-  launch_chained(compact_kernel, by_warp, dim3(256), 0, s, static_cast<const uint4*>(a.x), position, count,
-                 reinterpret_cast<uint4*>(ws + l.x_compact), static_cast<uint4*>(a.grad_x), a.row_losses, rows, x_pieces);
-  if (int rc = check_launch("compact_kernel")) return rc;
+  if (rows > kFewRows) {
+    launch_chained(compact_kernel, by_warp, dim3(256), 0, s, compact, count);
+    if (int rc = check_launch("compact_kernel")) return rc;
+  }
 
   const size_t finish_smem = (size_t)(tiles + 2 * a.top) * sizeof(float);
   for (int piece = 0; piece < l.pieces; ++piece) {
-    const Rows here{count, row_map, rows, piece * l.piece_rows, l.piece_rows};
+    const Rows here{count, row_map, rows, compact.always, l.ldx, piece * l.piece_rows, l.piece_rows};
     if (int rc = launch_logit_stats(a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab,
                                     (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature), stats, power, l.ldg,
                                     a.error_flag, s))

@@ -15,7 +15,9 @@ constexpr int kStatsTile = 128;  // vocabulary columns of one maximum and sum of
 struct Rows {
   const int* count;
   const int* row_map;
-  int total;  // rows of x; where *count equals it, x itself is the compact form
+  int total;        // rows of x; where *count equals it and not `copied`, x itself is the compact form
+  bool copied;      // x is copied in any case
+  long long ldx;    // distance of the copied rows
   int piece_begin, piece_rows;
 };
 
