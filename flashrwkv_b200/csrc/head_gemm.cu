@@ -31,13 +31,18 @@ using bf16 = __nv_bfloat16;
 using IO = Io16<bf16>;
 
 constexpr int kHalf = kTile / 2, kBK = 64;
-constexpr uint32_t kOperandBytes = kHalf * kBK * 2;  // 16 KB of each operand per CTA and stage
-constexpr uint32_t kStageBytes = 2 * kOperandBytes;
-constexpr int kStages = 6;
+constexpr uint32_t kOperandBytes = kHalf * kBK * 2;  // 16 KB: 128 rows of an operand in a stage
 constexpr int kEpilogueWarps = 8;  // two per quarter of the tensor-memory lanes, half of the columns each
 constexpr uint32_t kBoxBytes = 32 * 64 * 2;  // what an epilogue warp hands to TMA: 32 rows of 64 16-bit values
-constexpr uint32_t kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;  // + slack to align to 1024 bytes
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+
+// A pair's CTA loads 128 rows of A and 128 of B per stage; a CTA alone 128 of A and all 256 of B.
+template <int kCtas>
+struct Ring {
+  static constexpr uint32_t kBBytes = kOperandBytes * 2 / kCtas, kStageBytes = kOperandBytes + kBBytes;
+  static constexpr int kStages = kCtas == 2 ? 6 : 4;
+  static constexpr uint32_t kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;  // + slack to align the tiles
+};
 constexpr uint32_t kTmemCols = 2 * kTile;
 
 enum Product { kStats, kGradX, kGradWeight };
@@ -64,15 +69,16 @@ struct Unit {
 };
 
 // the work of a launch, from the number of rows that take part
-template <Product P>
+template <Product P, int kCtas>
 struct Work {
+  static constexpr int kRows = kHalf * kCtas;
   int tiles_m, tiles_n, units, kb_total, splits, columns;
   __device__ Work(const Params& p, int rows_here) {
     const int m = P == kGradWeight ? p.vocab : rows_here;
     const int n = P == kStats ? p.vocab : p.channels;
     const int k = P == kStats ? p.channels : (P == kGradX ? p.vocab : rows_here);
     columns = n;
-    tiles_m = (m + kTile - 1) / kTile;
+    tiles_m = (m + kRows - 1) / kRows;
     tiles_n = (n + kTile - 1) / kTile;
     kb_total = (k + kBK - 1) / kBK;
     splits = P == kStats || p.partials == nullptr ? 1 : *p.splits.chosen;
@@ -85,7 +91,7 @@ struct Work {
     const int tiles = tiles_m * tiles_n;
     u.split = unit / tiles;
     const int t = unit - u.split * tiles;
-    u.m0 = (P == kStats ? t % tiles_m : t / tiles_n) * kTile;
+    u.m0 = (P == kStats ? t % tiles_m : t / tiles_n) * kRows;
     u.n0 = (P == kStats ? t / tiles_m : t % tiles_n) * kTile;
     const int right = columns - u.n0;
     u.width = right < kTile ? (right + 31) & ~31 : kTile;
@@ -127,15 +133,18 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, 
   }
 }
 
-template <Product P>
-__global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_gemm_kernel(
-    const __grid_constant__ Params prm, int* __restrict__ error_flag) {
+template <Product P, int kCtas>
+__device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
+  using R = Ring<kCtas>;
+  constexpr bool kPair = kCtas == 2;
+  constexpr int kStages = R::kStages;
+  constexpr uint32_t kStageBytes = R::kStageBytes;
   constexpr bool kAMn = P == kGradWeight, kBMn = P != kStats;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_holder;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = umma2::cluster_rank();
+  const uint32_t rank = kPair ? umma2::cluster_rank() : 0u;
   const uint32_t tiles_base = (umma::smem_u32(smem_raw) + 1023u) & ~1023u;
 
   chain_release();
@@ -150,14 +159,19 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
     }
     for (int i = 0; i < 2; ++i) {
       umma::mbar_init(&acc_full[i], 1);   // a commit
-      umma::mbar_init(&acc_empty[i], 2 * kEpilogueWarps);  // those of both CTAs
+      umma::mbar_init(&acc_empty[i], kCtas * kEpilogueWarps);  // those of both CTAs
     }
     umma::mbar_fence_init();
   }
-  if (warp == 1) umma2::tmem_alloc(&tmem_holder, kTmemCols);
+  if (warp == 1) {
+    if (kPair)
+      umma2::tmem_alloc(&tmem_holder, kTmemCols);
+    else
+      umma::tmem_alloc(&tmem_holder, kTmemCols);
+  }
   umma::fence_before_sync();
   __syncthreads();
-  umma2::cluster_sync();
+  if (kPair) umma2::cluster_sync();
   umma::fence_after_sync();
   const uint32_t tmem = tmem_holder;
   chain_wait();
@@ -166,8 +180,8 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
   const int left = count - prm.rows.piece_begin;
   const int rows_here = left < 0 ? 0 : (left < prm.rows.piece_rows ? left : prm.rows.piece_rows);
   const bool compact = prm.rows.copied || count != prm.rows.total;
-  const Work<P> work(prm, rows_here);
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const Work<P, kCtas> work(prm, rows_here);
+  const int pair = blockIdx.x / kCtas, pairs = gridDim.x / kCtas;  // "pair" is the CTA where it works alone
   bool ok = true;
 
   const auto wait = [](uint64_t* bar, uint32_t parity) {  // by a whole warp, one outcome for all of it
@@ -180,26 +194,32 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
     uint32_t it = 0;
     for (int unit = pair; unit < work.units && ok; unit += pairs) {
       const Unit u = work.at(unit);
-      const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * (u.width / 2);
+      const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * (u.width / kCtas);
       for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
         const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
         if (!wait(&empty_bar[s], ph ^ 1u)) { ok = false; break; }
-        const uint32_t full = umma2::in_leader(&full_bar[s]);
+        const uint32_t full = kPair ? umma2::in_leader(&full_bar[s]) : umma::smem_u32(&full_bar[s]);
         const uint32_t a_dst = tiles_base + s * kStageBytes, b_dst = a_dst + kOperandBytes;
         const int k = kb * kBK;
+        const auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
+          if (kPair)
+            umma2::tma_load_2d(dst, map, x, y, full);
+          else
+            umma2::tma_load_2d_alone(dst, map, x, y, full);
+        };
         if (umma2::elect_one()) {
-          if (rank == 0) umma::mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
+          if (rank == 0) umma::mbar_expect_tx(&full_bar[s], kCtas * kStageBytes);
           if (kAMn) {
-            umma2::tma_load_2d(a_dst, map_a, m, a_row + k, full);
-            umma2::tma_load_2d(a_dst + 8192, map_a, m + 64, a_row + k, full);
+            load(a_dst, map_a, m, a_row + k);
+            load(a_dst + 8192, map_a, m + 64, a_row + k);
           } else {
-            umma2::tma_load_2d(a_dst, map_a, k, a_row + m, full);
+            load(a_dst, map_a, k, a_row + m);
           }
           if (kBMn) {
-            umma2::tma_load_2d(b_dst, map_b, n, b_row + k, full);
-            umma2::tma_load_2d(b_dst + 8192, map_b, n + 64, b_row + k, full);
+#pragma unroll
+            for (int j = 0; j < 4 / kCtas; ++j) load(b_dst + j * 8192, map_b, n + 64 * j, b_row + k);
           } else {
-            umma2::tma_load_2d(b_dst, map_b, k, n, full);
+            load(b_dst, map_b, k, n);
           }
         }
         __syncwarp();
@@ -215,6 +235,12 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
       const uint64_t a_desc = kAMn ? umma2::desc_mn_major(tiles_base) : umma2::desc_k_major(tiles_base);
       const uint64_t b_desc = kBMn ? umma2::desc_mn_major(tiles_base + kOperandBytes) : umma2::desc_k_major(tiles_base + kOperandBytes);
       constexpr uint32_t kAStep = (kAMn ? 2048 : 32) >> 4, kBStep = (kBMn ? 2048 : 32) >> 4;  // 16 contraction values
+      const auto commit = [](uint64_t* bar) {
+        if (kPair)
+          umma2::commit_both(bar);
+        else
+          umma::mma_commit(bar);
+      };
       uint32_t it = 0, t = 0;
       for (int unit = pair; unit < work.units && ok; unit += pairs) {
         const Unit u = work.at(unit);
@@ -224,7 +250,7 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
         if (!wait(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
         umma::fence_after_sync();
         const uint32_t d_tmem = tmem + acc * kTile;
-        const uint32_t idesc = umma2::idesc_bf16(u.width, kAMn, kBMn);
+        const uint32_t idesc = umma2::idesc_bf16(kHalf * kCtas, u.width, kAMn, kBMn);
         for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
           if (!wait(&full_bar[s], ph)) { ok = false; break; }
@@ -232,13 +258,18 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
           const uint64_t a = a_desc + s * (kStageBytes >> 4), b = b_desc + s * (kStageBytes >> 4);
           if (umma2::elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kBK / 16; ++ks)
-              umma2::mma_bf16(d_tmem, a + ks * kAStep, b + ks * kBStep, idesc, (kb > u.kb_begin || ks > 0) ? 1u : 0u);
-            umma2::commit_both(&empty_bar[s]);
+            for (int ks = 0; ks < kBK / 16; ++ks) {
+              const uint32_t add = (kb > u.kb_begin || ks > 0) ? 1u : 0u;
+              if (kPair)
+                umma2::mma_bf16(d_tmem, a + ks * kAStep, b + ks * kBStep, idesc, add);
+              else
+                umma2::mma_bf16_alone(d_tmem, a + ks * kAStep, b + ks * kBStep, idesc, add);
+            }
+            commit(&empty_bar[s]);
           }
           __syncwarp();
         }
-        if (ok && umma2::elect_one()) umma2::commit_both(&acc_full[acc]);
+        if (ok && umma2::elect_one()) commit(&acc_full[acc]);
         __syncwarp();
       }
     }
@@ -266,7 +297,8 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
         if (ok && !empty) {
           umma::fence_before_sync();
           __syncwarp();
-          if (lane == 0) umma2::arrive_cluster(umma2::in_leader(&acc_empty[acc]));
+          if (lane == 0)
+            umma2::arrive_cluster(kPair ? umma2::in_leader(&acc_empty[acc]) : umma::smem_u32(&acc_empty[acc]));
         }
       };
       if (P == kStats) {
@@ -372,8 +404,23 @@ __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_ge
   __syncwarp();
   umma::fence_before_sync();
   __syncthreads();
-  umma2::cluster_sync();
-  if (warp == 1) umma2::tmem_dealloc(tmem, kTmemCols);
+  if (kPair) umma2::cluster_sync();
+  if (warp == 1) {
+    if (kPair)
+      umma2::tmem_dealloc(tmem, kTmemCols);
+    else
+      umma::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <Product P>
+__global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_gemm_kernel(const __grid_constant__ Params prm,
+                                                                                          int* error_flag) {
+  head_gemm<P, 2>(prm, error_flag);
+}
+template <Product P>
+__global__ __launch_bounds__(kThreads, 1) void head_gemm_alone_kernel(const __grid_constant__ Params prm, int* error_flag) {
+  head_gemm<P, 1>(prm, error_flag);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
@@ -408,19 +455,20 @@ bool make_map(CUtensorMap* map, const void* base, long long rows, long long colu
 long long tiles_of(long long n) { return (n + kTile - 1) / kTile; }
 
 // `units`: at most so many; a product with parts may be cut finer than the host knows and takes every pair
-template <Product P>
+template <Product P, int kCtas>
 int launch(const Params& prm, long long units, int* error_flag, cudaStream_t stream) {
+  constexpr auto kernel = kCtas == 2 ? head_gemm_kernel<P> : head_gemm_alone_kernel<P>;
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = 64;
   if (dev >= 64 || !ready[dev].load(std::memory_order_relaxed)) {
-    cudaError_t e = cudaFuncSetAttribute(head_gemm_kernel<P>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Ring<kCtas>::kSmem);
     if (e != cudaSuccess) return fail(FRWKV_ERR_CUDA, "pretrain_head_loss: %s", cudaGetErrorString(e));
     if (dev < 64) ready[dev].store(true, std::memory_order_relaxed);
   }
-  const int pairs = pair_count();
-  const int grid = 2 * (int)(units < pairs ? units : pairs);
-  launch_chained(head_gemm_kernel<P>, dim3(grid), dim3(kThreads), kSmem, stream, prm, error_flag);
+  const int most = pair_count() * 2 / kCtas;
+  const int grid = kCtas * (int)(units < most ? units : most);
+  launch_chained(kernel, dim3(grid), dim3(kThreads), Ring<kCtas>::kSmem, stream, prm, error_flag);
   return check_launch("head_gemm_kernel");
 }
 
@@ -441,6 +489,7 @@ int pair_count() {
 int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
                        float log2_scale, float2* stats, void* power, long long ldp, int* error_flag,
                        cudaStream_t stream) {
+  const bool few = one_cta(rows.piece_rows);
   Params prm{};
   prm.rows = rows;
   prm.channels = channels;
@@ -451,10 +500,11 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
   prm.power = power != nullptr;
   if (!make_map(&prm.map_a, x, rows.total, channels, channels, kHalf) ||
       !make_map(&prm.map_compact, x_compact, rows.total, channels, rows.ldx, kHalf) ||
-      !make_map(&prm.map_b, weight, vocab, channels, channels, kHalf) ||
+      !make_map(&prm.map_b, weight, vocab, channels, channels, few ? kTile : kHalf) ||
       (power != nullptr && !make_map(&prm.map_out, power, rows.piece_rows, ldp, ldp, 32)))
     return map_failure();
-  return launch<kStats>(prm, tiles_of(rows.piece_rows) * tiles_of(vocab), error_flag, stream);
+  if (few) return launch<kStats, 1>(prm, tiles_of(vocab), error_flag, stream);
+  return launch<kStats, 2>(prm, tiles_of(rows.piece_rows) * tiles_of(vocab), error_flag, stream);
 }
 
 int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab,
@@ -469,7 +519,9 @@ int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& 
   if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kHalf) ||
       !make_map(&prm.map_b, weight, vocab, channels, channels, kBK))
     return map_failure();
-  return launch<kGradX>(prm, tiles_of(rows.piece_rows) * tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1), error_flag, stream);
+  const long long units = tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1);
+  if (one_cta(rows.piece_rows)) return launch<kGradX, 1>(prm, units, error_flag, stream);
+  return launch<kGradX, 2>(prm, tiles_of(rows.piece_rows) * units, error_flag, stream);
 }
 
 int launch_grad_weight(const void* g, long long ldg, const void* x, const void* x_compact, const Rows& rows, int channels,
@@ -488,7 +540,7 @@ int launch_grad_weight(const void* g, long long ldg, const void* x, const void* 
       !make_map(&prm.map_compact, x_compact, rows.total, channels, rows.ldx, kBK) ||
       (partials == nullptr && !make_map(&prm.map_out, grad_weight, vocab, channels, channels, 32)))
     return map_failure();
-  return launch<kGradWeight>(prm, tiles_of(vocab) * tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1), error_flag, stream);
+  return launch<kGradWeight, 2>(prm, tiles_of(vocab) * tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1), error_flag, stream);
 }
 
 }  // namespace head

@@ -110,6 +110,7 @@ struct Plan {
 };
 struct SplitSizes {
   int channels, vocab, most_x, most_w, pairs;
+  int workers_x;     // pairs, or CTAs that work alone, for grad_x
   long long room_x;  // rows of fp32 parts of grad_x
   bool fixed;        // several pieces: what the host has room for, whatever the count
 };
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
     if (!sizes.fixed && done > 0) {
       // fewer rows than the host has made room for leave room for more parts
       if (most_x > 1) most_x = (int)min((long long)kMaxSplits, sizes.room_x / done);
-      splits_x = choose_splits(most_x, (float)done, (float)sizes.channels, (float)sizes.vocab, (float)sizes.pairs, lane);
+      splits_x = choose_splits(most_x, (float)done, (float)sizes.channels, (float)sizes.vocab, (float)sizes.workers_x, lane);
       splits_w = choose_splits(sizes.most_w, (float)sizes.vocab, (float)sizes.channels, (float)done, (float)sizes.pairs, lane);
     }
     if (lane == 0) {
@@ -557,9 +558,9 @@ size_t take(size_t& at, size_t bytes) {
   return here;
 }
 
-int splits_for(long long rows, long long columns, long long k) {
+int splits_for(long long rows, long long columns, long long k, int workers) {
   const float tiles = (float)((rows + kTile - 1) / kTile * ((columns + kTile - 1) / kTile)), blocks = (float)((k + 63) / 64);
-  const float pairs = (float)pair_count(), elements = (float)rows * (float)columns;
+  const float pairs = (float)workers, elements = (float)rows * (float)columns;
   int best = 1;
   for (int s = 2; s <= kMaxSplits && blocks >= s * kLeastBlocks; ++s)
     if (split_cost(s, tiles, blocks, elements, pairs) < split_cost(best, tiles, blocks, elements, pairs)) best = s;
@@ -580,8 +581,8 @@ Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad
   // pieces of equal size, whole tiles each; a single piece is the rows themselves
   l.piece_rows = l.pieces == 1 ? (int)rows : (int)(((rows + l.pieces - 1) / l.pieces + kTile - 1) / kTile * kTile);
   l.pieces = (int)((rows + l.piece_rows - 1) / l.piece_rows);
-  l.splits_x = grad_x ? splits_for(l.piece_rows, channels, vocab) : 1;
-  l.splits_w = grad_weight ? splits_for(vocab, channels, l.piece_rows) : 1;
+  l.splits_x = grad_x ? splits_for(l.piece_rows, channels, vocab, pair_count() * (one_cta(l.piece_rows) ? 2 : 1)) : 1;
+  l.splits_w = grad_weight ? splits_for(vocab, channels, l.piece_rows, pair_count()) : 1;
   l.parts_x = l.splits_x > 1;
   l.parts_w = l.splits_w > 1 || l.pieces > 1;
   size_t at = 0;
@@ -666,8 +667,8 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     launch_chained(teacher_rows_kernel, by_warp, dim3(256), 0, s, labels, position, rows);
     if (int rc = check_launch("teacher_rows_kernel")) return rc;
   }
-  const SplitSizes sizes{a.channels, a.vocab, l.splits_x, l.splits_w, pair_count(), (long long)l.splits_x * l.piece_rows,
-                         l.pieces > 1};
+  const SplitSizes sizes{a.channels, a.vocab, l.splits_x, l.splits_w, pair_count(),
+                         pair_count() * (one_cta(l.piece_rows) ? 2 : 1), (long long)l.splits_x * l.piece_rows, l.pieces > 1};
   CompactArgs compact{};
   compact.x = static_cast<const uint4*>(a.x);
   compact.position = position;

@@ -54,6 +54,10 @@ int launch_grad_weight(const void* g, long long ldg, const void* x, const void* 
                        int vocab, const Splits& splits, void* grad_weight, float* partials, bool add, int* error_flag,
                        cudaStream_t stream);
 
+// Up to 128 rows one CTA works alone on a 128 x 256 tile: a pair's tile would be half empty, and the loads of W, which bound
+// the product then, would wait for twice the tensor-core time per byte.
+constexpr bool one_cta(long long rows) { return rows <= kTile / 2; }
+
 int pair_count();  // of CTAs that the current device runs at once
 
 }  // namespace head

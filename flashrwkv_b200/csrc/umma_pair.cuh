@@ -76,6 +76,27 @@ __device__ __forceinline__ void commit_both(uint64_t* mbar) {
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
+// the same product by one CTA alone, 128 rows
+__device__ __forceinline__ void mma_bf16_alone(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// A tile into this CTA's shared memory, its bytes counted on a barrier of its own
+__device__ __forceinline__ void tma_load_2d_alone(uint32_t smem_dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_dst),
+      "l"(map), "r"(x), "r"(y), "r"(mbar)
+      : "memory");
+}
 // A tile into this CTA's shared memory, its bytes counted on `mbar` (a cluster address: the leader's barrier)
 __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
   asm volatile(
@@ -109,10 +130,11 @@ __device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr) {
   return uint64_t((addr & 0x3ffffu) >> 4) | (uint64_t(8192 >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(2) << 61);
 }
-// bf16 operands, fp32 accumulator, 256 rows x `columns` (a multiple of 32 up to 256); bits 15 / 16: A / B is MN-major
-__host__ __device__ constexpr uint32_t idesc_bf16(int columns, bool a_mn, bool b_mn) {
+// bf16 operands, fp32 accumulator, `rows` (256 by a pair, 128 by one CTA) x `columns` (a multiple of 32 up to 256); bits 15 /
+// 16: A / B is MN-major
+__host__ __device__ constexpr uint32_t idesc_bf16(int rows, int columns, bool a_mn, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(columns >> 3) << 17) |
-         (uint32_t(256 >> 4) << 24);
+         (uint32_t(rows >> 4) << 24);
 }
 
 }  // namespace umma2
