@@ -348,10 +348,6 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     return;
   }
   const long long n = a.rows.row_map[a.rows.piece_begin + r];
-  uint4 e[4];  // four of the row's pieces at a time, the first of them requested ahead of all else
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (a.g != nullptr && from + tid + j * kFinishThreads < to) e[j] = g[from + tid + j * kFinishThreads];
 
   // the softmax's normaliser, in units of log2
   const float2* stats = a.stats + (long long)r * tiles;
@@ -417,7 +413,10 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   if (loss != loss) scale = quiet_nan();
   __syncthreads();  // the tiles' factors and the shares
   for (int begin = from + tid; begin < to; begin += 4 * kFinishThreads) {
-    uint4 out4[4];
+    uint4 e[4];  // four pieces requested together
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (begin + j * kFinishThreads < to) e[j] = g[begin + j * kFinishThreads];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = begin + j * kFinishThreads;
@@ -430,15 +429,9 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
           const float2 t = Io16<__half>::unpack(in[h]);
           out[h] = IO::pack(t.x * f, t.y * f);
         }
-        out4[j] = make_uint4(out[0], out[1], out[2], out[3]);
+        g[i] = make_uint4(out[0], out[1], out[2], out[3]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)  // the next four are under way before these leave
-      if (begin + (4 + j) * kFinishThreads < to) e[j] = g[begin + (4 + j) * kFinishThreads];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (begin + j * kFinishThreads < to) g[begin + j * kFinishThreads] = out4[j];
   }
   __syncthreads();
   if (bad) return;
