@@ -7,7 +7,7 @@
 // One persistent kernel, specialised by warp and run by pairs of CTAs (tcgen05, cta_group::2): a pair owns a 256 x 256
 // output tile, each CTA loads its 128 rows of A and its half of B, so that a byte of shared memory feeds twice the
 // arithmetic of a single CTA's 128 x 256 tile, which is bound by the fill of its shared memory.
-//   warp 0      producer: TMA tiles of 64 contraction values into a ring of six stages; both CTAs' bytes are counted on
+//   warp 0      producer: TMA tiles of 64 contraction values into a ring of five stages; both CTAs' bytes are counted on
 //               the leader's barrier
 //   warp 1      (leader) MMA issuer: four tcgen05.mma per stage into one of two accumulators in tensor memory; commits
 //               release the stage, and hand over the accumulator, in both CTAs
@@ -40,7 +40,7 @@ constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 template <int kCtas>
 struct Ring {
   static constexpr uint32_t kBBytes = kOperandBytes * 2 / kCtas, kStageBytes = kOperandBytes + kBBytes;
-  static constexpr int kStages = kCtas == 2 ? 6 : 4;
+  static constexpr int kStages = kCtas == 2 ? 5 : 4;
   static constexpr uint32_t kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;  // + slack to align the tiles
 };
 constexpr uint32_t kTmemCols = 2 * kTile;

@@ -413,3 +413,125 @@ def test_the_end_of_a_training_step():
     ds, dnw, dnb = O.layer_norm_backward((d1 + d2).view(2, 75, C), total.detach(), nw.detach(), 1e-5)
     for g, want, name in zip(got, (ds, ds, dnw, dnb, w1 + w2), ("x", "residual", "norm weight", "norm bias", "head")):
         assert float((g.double() - want).norm()) <= 3 * RHO * float(want.norm()), name
+
+
+def _plain_rows(x, w, t):
+    z = x.double() @ w.double().T
+    return torch.logsumexp(z, 1) - z.gather(1, t[:, None])[:, 0], torch.softmax(z, 1)
+
+
+def test_offsets_beyond_32_bits_in_the_weight():
+    """2^20 x 2056 weights are 2.16e9 values; the last vocabulary rows are labels.  The row sum of exponentials takes 8192
+    entries.  Bounds as above, with B_n from the rows themselves."""
+    import flashrwkv_b200 as F
+
+    N, C, V = 12, 2056, 1 << 20
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    w = torch.empty(V, C, dtype=torch.bfloat16, device="cuda").normal_(0, 2 / C ** 0.5, generator=gen)
+    x = torch.randn(N, C, generator=gen, device="cuda").to(torch.bfloat16)
+    t = torch.arange(V - N, V, device="cuda")
+    x.requires_grad_(), w.requires_grad_()
+    rows = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    z = torch.cat([x.detach().double() @ part.double().T for part in w.detach().split(1 << 16)], 1)
+    want = torch.logsumexp(z, 1) - z.gather(1, t[:, None])[:, 0]
+    B = torch.stack([(x.detach().double().abs() @ part.double().abs().T).amax(1) for part in w.detach().split(1 << 16)]).amax(0)
+    bound = 2 * (2 * C * U * B) + 9000 * U + 2 ** -20 + 32 * U * (z.abs().amax(1) + want)
+    _near(rows.detach(), want, bound, "row losses")
+    g = torch.softmax(z, 1)
+    g[torch.arange(N), t] -= 1
+    want_dx = sum(p @ q.double() for p, q in zip(g.split(1 << 16, 1), w.detach().split(1 << 16)))
+    assert float((dx.double() - want_dx).norm()) <= 4e-3 * 2 ** 0.5 * float(want_dx.norm())
+    for s in (slice(0, 300), slice(V - 300, V)):
+        want_dw = g[:, s].T @ x.detach().double()
+        assert float((dw[s].double() - want_dw).norm()) <= 4e-3 * 2 ** 0.5 * float(want_dw.norm())
+
+
+def test_offsets_beyond_32_bits_in_the_rows():
+    import flashrwkv_b200 as F
+
+    N, C, V = (1 << 20) + 1003, 2056, 300
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.empty(V, C, dtype=torch.bfloat16, device="cuda").normal_(0, 2 / C ** 0.5, generator=gen)
+    x = torch.empty(N, C, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    t = torch.randint(V, (N,), generator=gen, device="cuda")
+    t[5:900] = -100  # the rows that take part move, the last too
+    x.requires_grad_()
+    rows = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    up = torch.zeros_like(rows)
+    up[-700:] = 1
+    dx = torch.autograd.grad(rows, x, up)[0]
+    last = slice(N - 700, N)
+    want, q = _plain_rows(x.detach()[last], w, t[last])
+    assert float((rows.detach()[last].double() - want).abs().max()) <= 2 * 2 * C * U * float(
+        (x.detach()[last].double().abs() @ w.double().abs().T).max()) + 2 ** -19
+    q[torch.arange(700), t[last]] -= 1
+    want_dx = q @ w.double()
+    assert float((dx[last].double() - want_dx).norm()) <= 4e-3 * 2 ** 0.5 * float(want_dx.norm())
+    assert bool((dx[:-700] == 0).all()) and bool((rows[5:900] == 0).all())
+
+
+def test_inference_mode_and_another_current_stream():
+    """Called from a stream of its own right behind the kernels that make its inputs there; and without autograd."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(300, 264, 2100, 13)
+    want = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    with torch.inference_mode():
+        assert torch.equal(F.pretrain_head_cross_entropy_bf16(x, w, t), want)
+        total, out = F.pretrain_tmix_add_layer_norm_bf16(x, x, w[0], w[1])
+        assert out.shape == x.shape
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000)
+        y = (x.float() * 2).to(torch.bfloat16).requires_grad_()
+        loss = F.pretrain_head_cross_entropy_bf16(y, w, t)
+        grad = torch.autograd.grad(loss, y)[0]
+    side.synchronize()
+    z = (x.float() * 2).to(torch.bfloat16).requires_grad_()
+    again = F.pretrain_head_cross_entropy_bf16(z, w, t)
+    assert torch.equal(again, loss) and torch.equal(torch.autograd.grad(again, z)[0], grad)
+
+
+def test_two_calls_at_once_on_two_streams():
+    import flashrwkv_b200 as F
+
+    cases = []
+    for k, shape in enumerate(((700, 264, 9000), (40, 512, 30000))):
+        x, w, t, _ = _rows(*shape, 20 + k)
+        x.requires_grad_(), w.requires_grad_()
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+        cases.append((x, w, t, [loss.detach(), *torch.autograd.grad(loss, (x, w))], torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for x, w, t, _, stream in cases:
+            with torch.cuda.stream(stream):
+                loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+                got.append([loss.detach(), *torch.autograd.grad(loss, (x, w))])
+        torch.cuda.synchronize()
+        for (_, _, _, want, _), have in zip(cases, got):
+            for a, b in zip(want, have):
+                assert torch.equal(a, b)
+
+
+def test_losses_accumulate_over_micro_batches_into_one_weight():
+    """Two losses alive at once over the same weight, run backward together: the leaves receive the sum of their gradients."""
+    import flashrwkv_b200 as F
+
+    x1, w, t1, _ = _rows(70, 72, 600, 30)
+    x2, _, t2, _ = _rows(90, 72, 600, 31)
+    for v in (x1, x2, w):
+        v.requires_grad_()
+    a, b = F.pretrain_head_cross_entropy_bf16(x1, w, t1), F.pretrain_head_cross_entropy_bf16(x2, w, t2)
+    ((a + b) * 0.5).backward()
+    g1 = torch.autograd.grad(F.pretrain_head_cross_entropy_bf16(x1, w, t1), (x1, w), torch.tensor(0.5, device="cuda"))
+    g2 = torch.autograd.grad(F.pretrain_head_cross_entropy_bf16(x2, w, t2), (x2, w), torch.tensor(0.5, device="cuda"))
+    assert torch.equal(x1.grad, g1[0]) and torch.equal(x2.grad, g2[0]) and torch.equal(w.grad, g1[1] + g2[1])
+    # the same row taken from a leaf that is used in place afterwards is refused, as by any operator that needs it again
+    loss = F.pretrain_head_cross_entropy_bf16(x1, w, t1)
+    with torch.no_grad():
+        x1.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

@@ -237,3 +237,27 @@ def test_refusals_on_the_device():
     for eps in (0.0, -1.0, float("nan"), float("inf"), 1e-60):
         with pytest.raises(ValueError, match="eps must be positive"):
             F.pretrain_tmix_layer_norm_bf16(x, w, b, eps=eps)
+
+
+def test_offsets_beyond_32_bits():
+    import flashrwkv_b200 as F
+
+    rows, C = 270_000, 8192  # 2.2e9 values
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(rows, C, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    w = torch.ones(C, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    b = torch.zeros(C, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    x.requires_grad_()
+    out = F.pretrain_tmix_layer_norm_bf16(x, w, b)
+    g = torch.zeros_like(out)
+    g[-3:] = torch.empty_like(g[-3:]).normal_(generator=gen)
+    dx, dw, db = torch.autograd.grad(out, (x, w, b), g)
+    few = x.detach()[-3:].contiguous().requires_grad_()
+    want = F.pretrain_tmix_layer_norm_bf16(few, w, b)
+    assert torch.equal(out[-3:], want)
+    ex, ew, eb = torch.autograd.grad(want, (few, w, b), g[-3:].contiguous())
+    assert torch.equal(dx[-3:], ex) and bool((dx[:-3] == 0).all())
+    # three terms per column, added in another order among zeros: 3 u of their sum of magnitudes, then the rounding to bf16
+    slack = 3 * U * (g[-3:].double().abs() * (1 + want.double().abs())).sum(0)
+    assert bool(((dw.double() - ew.double()).abs() <= 2 * HALF * ew.double().abs() + slack).all())
+    assert bool(((db.double() - eb.double()).abs() <= 2 * HALF * eb.double().abs() + slack).all())
