@@ -112,7 +112,7 @@ struct SplitSizes {
   int channels, vocab, most_x, most_w, pairs;
   int workers_x;     // pairs, or CTAs that work alone, for grad_x
   long long room_x;  // rows of fp32 parts of grad_x
-  bool fixed;        // several pieces: what the host has room for, whatever the count
+  bool fixed;        // several pieces: what the host has chosen, whatever the count
 };
 
 // the cheapest number of parts, by one warp
@@ -206,8 +206,8 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
   }
   if (warp == 0) {
     int most_x = sizes.most_x, splits_x = most_x, splits_w = sizes.most_w;
-    if (!sizes.fixed && done > 0) {
-      // fewer rows than the host has made room for leave room for more parts
+    if (!sizes.fixed && done > 0 && done < rows) {
+      // fewer rows than the host has chosen for, which leave room for more parts
       if (most_x > 1) most_x = (int)min((long long)kMaxSplits, sizes.room_x / done);
       splits_x = choose_splits(most_x, (float)done, (float)sizes.channels, (float)sizes.vocab, (float)sizes.workers_x, lane);
       splits_w = choose_splits(sizes.most_w, (float)sizes.vocab, (float)sizes.channels, (float)done, (float)sizes.pairs, lane);
@@ -272,12 +272,12 @@ struct FinishArgs {
   float* row_losses;
   float* loss;               // the last CTA of the last piece to arrive adds the row losses, in row order; or null
   int* arrived;
-  int ctas;                  // of all pieces
+  int ctas;                  // of all pieces, the first part of a row each
 };
 
-// Called by every CTA with its row losses written.  The sum does not depend on who arrives last.
+// Called by every CTA that writes row losses.  The sum does not depend on who arrives last.
 __device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count, float* scratch) {
-  if (a.loss == nullptr) return;
+  if (a.loss == nullptr || blockIdx.y > 0) return;
   __shared__ bool last;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -434,8 +434,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     }
   }
   __syncthreads();
-  if (bad) return;
-  for (int k = tid; k < top; k += kFinishThreads) {
+  for (int k = tid; k < top && !bad; k += kFinishThreads) {
     if (a.labels.teacher != nullptr && a.labels.teacher[entry + k] == -INFINITY) continue;
     const long long v = a.labels.at(entry + k);
     if (v < 8ll * from || v >= 8ll * to) continue;
@@ -707,7 +706,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     // entries then is two rounds of requests)
     const int parts = by_warps || !grads ? 1 : (l.piece_rows >= 148 ? 1 : (l.piece_rows > 18 ? 296 / l.piece_rows : 16));
     const int ctas = by_warps ? (l.piece_rows + kFinishThreads / 32 - 1) / (kFinishThreads / 32) : l.piece_rows;
-    f.ctas = ctas * parts * l.pieces;
+    f.ctas = ctas * l.pieces;
     if (by_warps)
       launch_chained(losses_kernel, dim3(ctas), dim3(kFinishThreads), 0, s, f);
     else
