@@ -55,6 +55,7 @@ struct Params {
   int channels, vocab;
   Splits splits;           // kGradX, kGradWeight
   float log2_scale;        // kStats
+  const int* main_column;
   float2* stats;
   int stats_tiles;
   bool power;              // kStats: the exponentials are wanted
@@ -286,12 +287,14 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
       const bool empty = u.kb_begin == u.kb_end;
       const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
       if (!empty) ++t;
+      const int m = u.m0 + row_in_tile, n = u.n0 + column0;
+      int main = -1;  // kStats: where the row's label lies in this warp's columns
+      if (P == kStats && m < m_end) main = prm.main_column[prm.rows.piece_begin + m] - n;
       // Warp-uniform outcome: the tensor-memory loads below need the whole warp.  Once a wait has run out, this unit and all
       // later ones read as NaN.
       if (ok && !empty && !wait(&acc_full[acc], aph)) ok = false;
       umma::fence_after_sync();
       const uint32_t source = source0 + acc * kTile;
-      const int m = u.m0 + row_in_tile, n = u.n0 + column0;
       // the accumulator goes back to the issuer as soon as its last columns are in registers
       const auto release = [&] {
         if (ok && !empty) {
@@ -319,20 +322,24 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
 #pragma unroll
             for (int j = 0; j < kStatsTile; ++j) z[j] = j < valid ? z[j] : -INFINITY;
           }
+          if (__any_sync(0xffffffffu, main >= 0 && main < kStatsTile)) {
+#pragma unroll
+            for (int j = 0; j < kStatsTile; ++j) z[j] = j == main ? -INFINITY : z[j];
+          }
           // a NaN gets past the maximum, but not past the sum
           float high[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < kStatsTile; ++j) high[j & 3] = fmaxf(high[j & 3], z[j]);
-          const float reference = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3])) * prm.log2_scale;
+          const float most = fmaxf(fmaxf(high[0], high[1]), fmaxf(high[2], high[3]));
+          const float reference = most == -INFINITY ? 0.f : most * prm.log2_scale;  // nothing here: zeros, not inf - inf
 #pragma unroll
           for (int j = 0; j < kStatsTile; ++j) {
             z[j] = ex2_approx(fmaf(z[j], prm.log2_scale, -reference));
             sum[j & 3] += z[j];
           }
-          if (m < m_end) {
+          if (m < m_end)
             prm.stats[(long long)m * prm.stats_tiles + n / kStatsTile] =
-                make_float2(reference, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-          }
+                make_float2(most == -INFINITY ? -INFINITY : reference, (sum[0] + sum[1]) + (sum[2] + sum[3]));
           // rows of a box that take no part get what is there: nothing reads it
           if (prm.power && m - lane < m_end) {
             store_box<__half>(&prm.map_out, n, m - lane, box, z, lane);
@@ -487,7 +494,8 @@ int pair_count() {
 }
 
 int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
-                       float log2_scale, float2* stats, void* power, long long ldp, int* error_flag,
+                       float log2_scale, const int* main_column, float2* stats, void* power, long long ldp,
+                       int* error_flag,
                        cudaStream_t stream) {
   const bool few = one_cta(rows.piece_rows);
   Params prm{};
@@ -495,6 +503,7 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
   prm.channels = channels;
   prm.vocab = vocab;
   prm.log2_scale = log2_scale;
+  prm.main_column = main_column;
   prm.stats = stats;
   prm.stats_tiles = (vocab + kStatsTile - 1) / kStatsTile;
   prm.power = power != nullptr;

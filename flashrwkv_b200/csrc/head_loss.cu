@@ -1,11 +1,18 @@
 // The head's losses for training: the vocabulary projection, its softmax, a loss against labels or against a teacher's
 // highest logits, and the gradients of the rows and of the weight, without ever holding the logits.
 //
-//   z_n = W x_n / T            q_n = softmax(z_n)           lse_n = log sum_v exp(z_nv)
-//   label t:                   loss_n = lse_n - z_nt                                        (T = 1, one entry, p = 1)
+//   z_n = W x_n / T            q_n = softmax(z_n)
+//   label t:                   loss_n = -log q_nt                                           (T = 1, one entry, p = 1)
 //   teacher entries (t_k, l_k): p = softmax(l / T) over the entries that are there (l > -inf),
-//                              loss_n = T^2 sum_k p_k (log p_k - z_n,t_k + lse_n)
+//                              loss_n = T^2 sum_k p_k (log p_k - log q_n,t_k)
 //   g_nv = scale_n T (q_nv - sum over k with t_k = v of p_k)      dx = g W,  dW = g^T x
+//
+// A row that is nearly certain of its label has a loss and a label gradient that are differences of nearly equal numbers in
+// these forms (lse - z, q - 1).  They are taken from what is small instead: the label t (of a teacher: its highest entry)
+// stays out of the sums, O = log of the sum of exp z_v over the other v, d = O - z_t, and
+//   -log q_t = log(1 + e^d),   1 - q_t = e^d / (1 + e^d),   log q_k = z_k - z_t - log(1 + e^d),
+//   g_t = scale T (sum of the p_k of other columns - (1 - q_t)),
+// so that both keep their relative precision down to the smallest losses.
 //
 // Passes over a piece of the rows (all of them while 2 rows x vocabulary bytes fit kPieceBytes):
 //   plan     numbers the rows that have a label; rows without one take no part in any product (compact_kernel copies the
@@ -13,7 +20,7 @@
 //   stats    z on the tensor cores; the epilogue leaves, per 128 columns, each row's maximum and sum of exponentials, and for
 //            gradients the exponentials themselves in fp16, relative to that maximum (error 2^-12 of each, where a bf16
 //            value would add 2^-9 to the one rounding that g needs as a tensor-core operand)
-//   finish   per row: lse from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
+//   finish   per row: O from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
 //            the exponentials times their tile's factor in place, now g in bf16; the labels' entries from fp32
 //   products dx and dW
 // so a step costs three products of 2 rows x vocabulary x channels, not the four of recomputing z for the backward pass,
@@ -57,15 +64,30 @@ struct Labels {
 };
 
 // ---- plan: which rows take part --------------------------------------------------------------------------------------
-// flags[row] = the teacher has an entry for this row; a warp per row
-__global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* __restrict__ flags, int rows) {
+// highest[row] = the first of the teacher's highest entries for this row, -1 where it has none; a warp per row
+__global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* __restrict__ highest, int rows) {
   chain_begin();
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= rows) return;
-  bool any = false;
-  for (int k = lane; k < labels.top; k += 32) any |= !(labels.teacher[(long long)row * labels.top + k] == -INFINITY);
-  any = __any_sync(0xffffffffu, any);
-  if (lane == 0) flags[row] = any;
+  float most = -INFINITY;
+  int which = -1;
+  for (int k = lane; k < labels.top; k += 32) {
+    const float t = labels.teacher[(long long)row * labels.top + k];
+    if (!(t == -INFINITY) && (which < 0 || t > most)) {  // a NaN is an entry too: its row becomes NaN
+      most = t;
+      which = k;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float t = __shfl_xor_sync(0xffffffffu, most, o);
+    const int w = __shfl_xor_sync(0xffffffffu, which, o);
+    if (w >= 0 && (which < 0 || t > most || (t == most && w < which))) {
+      most = t;
+      which = w;
+    }
+  }
+  if (lane == 0) highest[row] = which;
 }
 
 // Copies the rows that take part together; the others get a zero loss and a zero gradient.  The rows behind the last, up
@@ -139,13 +161,14 @@ __device__ int choose_splits(int most, float rows, float columns, float k, float
   return which;
 }
 
-// One CTA numbers the rows in order: position[row] = compact number or -1, row_map its inverse.  `position` holds the
-// teacher's flags on entry.
-__global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position, int* __restrict__ row_map,
+// One CTA numbers the rows in order: position[row] = compact number or -1, row_map its inverse, main_column the label's column
+// (the teacher's highest entry's) by compact number, -1 where it lies outside the vocabulary.
+__global__ __launch_bounds__(1024) void plan_kernel(Labels labels, const int* __restrict__ highest, int* position,
+                                                    int* __restrict__ row_map, int* __restrict__ main_column,
                                                     Plan* __restrict__ plan, SplitSizes sizes, CompactArgs compact,
                                                     int* __restrict__ error_flag, int rows) {
   chain_begin();
-  constexpr int kEach = 8;  // consecutive rows of a thread; the flags come in row order through shared memory
+  constexpr int kEach = 8;  // consecutive rows of a thread; what is in use comes in row order through shared memory
   __shared__ int warp_sums[32];
   __shared__ __align__(8) unsigned char flags[1024 * kEach];
   __shared__ int list[1024 * kEach];  // the rows in use of this round, so that they leave in whole lines
@@ -157,7 +180,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
     for (int i = 0; i < kEach; ++i) {
       const int row = min(begin + i * 1024 + (int)threadIdx.x, rows - 1);
       if (labels.teacher != nullptr) {
-        label[i] = position[row];
+        label[i] = __ldg(highest + row);
       } else if (labels.wide) {
         label[i] = __ldg(static_cast<const long long*>(labels.index) + row);
       } else {
@@ -167,7 +190,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int at = i * 1024 + threadIdx.x;
-      flags[at] = begin + at < rows && label[i] != (labels.teacher != nullptr ? 0 : labels.ignore_index);
+      flags[at] = begin + at < rows && label[i] != (labels.teacher != nullptr ? -1 : labels.ignore_index);
     }
     __syncthreads();
     const uint2 mine8 = *reinterpret_cast<const uint2*>(flags + threadIdx.x * kEach);
@@ -200,7 +223,12 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, int* position
         if (first + i < rows) position[first + i] = where[i];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < used_here; i += 1024) row_map[done + i] = list[i];
+    for (int i = threadIdx.x; i < used_here; i += 1024) {
+      const int row = list[i];
+      const long long v = labels.teacher != nullptr ? labels.at((long long)row * labels.top + __ldg(highest + row)) : labels.at(row);
+      row_map[done + i] = row;
+      main_column[done + i] = v >= 0 && v < sizes.vocab ? (int)v : -1;
+    }
     done += used_here;
     __syncthreads();
   }
@@ -257,11 +285,34 @@ __device__ __forceinline__ float label_logit(const bf16* x_row, const bf16* w_ro
   return dot;
 }
 
+constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
+
+// What a row's loss and gradients are made of, from the others' maximum and sum (in units of log2) and the label's z.
+struct RowSums {
+  float excess;    // log(1 + e^d) = -log q_t
+  float missing;   // 1 - q_t
+  float lse2;      // log2 of the sum over the whole vocabulary
+};
+__device__ __forceinline__ RowSums row_sums(float high, float sum, float z) {
+  // z log2(e) in two parts, so that d does not lose to the size of either term
+  const float z2 = z * kLog2e, z2_rest = fmaf(z, kLog2e, -z2) + z * 1.9259629911e-8f;
+  const float others = log2f(sum);  // -inf where there are none
+  const float d = ((high - z2) - z2_rest + others) * kLn2;
+  RowSums r;
+  const float e = expf(-fabsf(d)), small = log1pf(e);
+  r.excess = d > 0.f ? d + small : small;
+  r.missing = d > 0.f ? 1.f / (1.f + e) : e / (1.f + e);
+  r.lse2 = z2 + r.excess * kLog2e;
+  if (d != d) r.excess = r.missing = r.lse2 = d;
+  return r;
+}
+
 struct FinishArgs {
   Rows rows;
   Labels labels;
   const bf16* x;
   const bf16* weight;
+  const int* highest;        // of a teacher's entries, by row of x
   const float2* stats;       // [row of the piece][tiles]
   int vocab, channels;
   uint4* g;            // exponentials in, logit gradients out, ldg values per row; null without gradients
@@ -311,6 +362,7 @@ __global__ __launch_bounds__(kFinishThreads) void losses_kernel(const FinishArgs
     for (int t = lane; t < tiles; t += 32) high = fmaxf(high, __ldg(&stats[t].x));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+    if (high == -INFINITY) high = 0.f;  // no others
 #pragma unroll 4
     for (int t = lane; t < tiles; t += 32) {
       const float2 s = __ldg(stats + t);
@@ -319,7 +371,7 @@ __global__ __launch_bounds__(kFinishThreads) void losses_kernel(const FinishArgs
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float logit = inside ? label_logit(a.x + n * a.channels, a.weight + v * a.channels, a.channels / 8, lane) : 0.f;
-    if (lane == 0) a.row_losses[n] = inside ? (high * 0.6931471805599453f - logit) + logf(sum) : quiet_nan();
+    if (lane == 0) a.row_losses[n] = inside ? row_sums(high, sum, logit).excess : quiet_nan();
   }
   arrive_and_sum(a, count, scratch);
 }
@@ -354,15 +406,12 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   float high = -INFINITY, sum = 0.f;
   for (int t = tid; t < tiles; t += kFinishThreads) high = fmaxf(high, stats[t].x);
   high = block_reduce(high, scratch, true);
+  if (high == -INFINITY) high = 0.f;  // no others
   for (int t = tid; t < tiles; t += kFinishThreads) {
     const float2 s = stats[t];
     sum = fmaf(s.y, ex2_approx(s.x - high), sum);
   }
   sum = block_reduce(sum, scratch, false);
-  const float lse2 = high + log2f(sum);
-  // lse - z is taken as (max - z) + log(sum): both terms are small where the label is likely
-  const float max_z = high * 0.6931471805599453f, log_sum = logf(sum);
-  for (int t = tid; t < tiles; t += kFinishThreads) factor[t] = stats[t].x - lse2;
 
   // the labels' logits: a warp per entry
   const long long entry = n * top;
@@ -377,27 +426,30 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   }
   bad = __syncthreads_or(bad);
 
+  const int main = a.labels.teacher != nullptr ? a.highest[n] : 0;
+  const RowSums row = row_sums(high, sum, logit[main]);
+  for (int t = tid; t < tiles; t += kFinishThreads) factor[t] = stats[t].x - row.lse2;
+
   float loss;
   if (a.labels.teacher == nullptr) {
     if (tid == 0) share[0] = 1.f;
-    loss = (max_z - logit[0]) + log_sum;
+    loss = row.excess;
   } else {
-    float most = -INFINITY, total = 0.f;
-    for (int k = tid; k < top; k += kFinishThreads) most = fmaxf(most, a.labels.teacher[entry + k] * a.labels.inv_temperature);
-    most = block_reduce(most, scratch, true);
+    const float most = a.labels.teacher[entry + main] * a.labels.inv_temperature;
+    float rest = 0.f;  // of the exponentials, beside the highest entry's 1
     for (int k = tid; k < top; k += kFinishThreads) {
       const float p = expf(a.labels.teacher[entry + k] * a.labels.inv_temperature - most);
       share[k] = p;
-      total += p;
+      if (k != main) rest += p;
     }
-    total = block_reduce(total, scratch, false);
-    const float log_total = logf(total);
+    rest = block_reduce(rest, scratch, false);
+    const float log_total = log1pf(rest);
     float part = 0.f;
     for (int k = tid; k < top; k += kFinishThreads) {
-      const float p = share[k] / total;
+      const float p = share[k] / (1.f + rest);
       share[k] = p;
       const float log_p = a.labels.teacher[entry + k] * a.labels.inv_temperature - most - log_total;
-      if (!(p == 0.f)) part = fmaf(p, (max_z - logit[k]) + (log_sum + log_p), part);  // an absent entry has p = 0
+      if (!(p == 0.f)) part = fmaf(p, (log_p + row.excess) - (logit[k] - logit[main]), part);  // an absent entry has p = 0
     }
     loss = a.labels.temperature * a.labels.temperature * block_reduce(part, scratch, false);
   }
@@ -438,12 +490,19 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     if (a.labels.teacher != nullptr && a.labels.teacher[entry + k] == -INFINITY) continue;
     const long long v = a.labels.at(entry + k);
     if (v < 8ll * from || v >= 8ll * to) continue;
-    float p = 0.f;  // an index may occur more than once: each occurrence writes the same value
-    for (int j = 0; j < top; ++j)
-      if ((a.labels.teacher == nullptr || !(a.labels.teacher[entry + j] == -INFINITY)) && a.labels.at(entry + j) == v)
-        p += share[j];
-    const float q = ex2_approx(logit[k] * 1.4426950408889634f - lse2);
-    reinterpret_cast<bf16*>(g)[v] = IO::store(scale * (q - p));
+    // an index may occur more than once: each occurrence writes the same value
+    const bool of_main = v == a.labels.at(entry + main);
+    float here = 0.f, elsewhere = 0.f;
+    for (int j = 0; j < top; ++j) {
+      if (a.labels.teacher != nullptr && a.labels.teacher[entry + j] == -INFINITY) continue;
+      if (a.labels.at(entry + j) == v)
+        here += share[j];
+      else
+        elsewhere += share[j];
+    }
+    // q - p, or for the main column (1 - p) - (1 - q)
+    const float slope = of_main ? elsewhere - row.missing : ex2_approx(logit[k] * kLog2e - row.lse2) - here;
+    reinterpret_cast<bf16*>(g)[v] = IO::store(scale * slope);
   }
 }
 
@@ -541,7 +600,7 @@ struct Layout {
   long long ldg, ldx;
   int piece_rows, pieces, splits_x, splits_w;
   bool parts_x, parts_w;
-  size_t position, row_map, plan, x_compact, stats, power, partial_x, partial_w, bytes;
+  size_t position, row_map, highest, main_column, plan, x_compact, stats, power, partial_x, partial_w, bytes;
 };
 
 size_t take(size_t& at, size_t bytes) {
@@ -581,6 +640,8 @@ Layout layout_of(long long rows, int channels, int vocab, bool grad_x, bool grad
   l.plan = take(at, sizeof(Plan));
   l.position = take(at, rows * 4);
   l.row_map = take(at, rows * 4);
+  l.highest = take(at, rows * 4);
+  l.main_column = take(at, rows * 4);
   l.x_compact = take(at, (size_t)rows * l.ldx * 2);
   l.stats = take(at, (size_t)tiles * l.piece_rows * 8);
   l.power = take(at, grads ? (size_t)l.piece_rows * l.ldg * 2 : 0);
@@ -639,6 +700,8 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   const int* count = &plan->count;
   int* position = reinterpret_cast<int*>(ws + l.position);
   int* row_map = reinterpret_cast<int*>(ws + l.row_map);
+  int* highest = reinterpret_cast<int*>(ws + l.highest);
+  int* main_column = reinterpret_cast<int*>(ws + l.main_column);
   float2* stats = reinterpret_cast<float2*>(ws + l.stats);
   void* power = grads ? ws + l.power : nullptr;
   float* partial_x = l.parts_x ? reinterpret_cast<float*>(ws + l.partial_x) : nullptr;
@@ -656,7 +719,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
 
   const dim3 by_warp((rows + 7) / 8);
   if (a.teacher_logits != nullptr) {
-    launch_chained(teacher_rows_kernel, by_warp, dim3(256), 0, s, labels, position, rows);
+    launch_chained(teacher_rows_kernel, by_warp, dim3(256), 0, s, labels, highest, rows);
     if (int rc = check_launch("teacher_rows_kernel")) return rc;
   }
   const SplitSizes sizes{a.channels, a.vocab, l.splits_x, l.splits_w, pair_count(),
@@ -671,7 +734,8 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   compact.pieces = a.channels / 8;
   compact.pitch = (int)(l.ldx / 8);
   compact.always = l.ldx != a.channels;
-  launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, position, row_map, plan, sizes, compact, a.error_flag, rows);
+  launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, highest, position, row_map, main_column, plan,
+                 sizes, compact, a.error_flag, rows);
   if (int rc = check_launch("plan_kernel")) return rc;
   if (rows > kFewRows) {
     launch_chained(compact_kernel, by_warp, dim3(256), 0, s, compact, count);
@@ -682,7 +746,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   for (int piece = 0; piece < l.pieces; ++piece) {
     const Rows here{count, row_map, rows, compact.always, l.ldx, piece * l.piece_rows, l.piece_rows};
     if (int rc = launch_logit_stats(a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab,
-                                    (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature), stats, power, l.ldg,
+                                    (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature), main_column, stats, power, l.ldg,
                                     a.error_flag, s))
       return rc;
     FinishArgs f{};
@@ -690,6 +754,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.labels = labels;
     f.x = static_cast<const bf16*>(a.x);
     f.weight = static_cast<const bf16*>(a.weight);
+    f.highest = highest;
     f.stats = stats;
     f.vocab = a.vocab;
     f.channels = a.channels;

@@ -23,9 +23,11 @@ struct Rows {
 
 // Statistics of the logits z = x W^T / T: for every 128 vocabulary columns and every row of the piece
 // stats[row][tile] = (max, sum exp2(z' - max)) with z' = z log2(e) / T, and, with `power`, the fp16 values
-// exp2(z' - max) in power[row][ldp] (zeros behind the vocabulary).
+// exp2(z' - max) in power[row][ldp] (zeros behind the vocabulary).  The column main_column[compact row] of a row, its label,
+// stays out of them (-1: none does); of no column at all they are (-inf, 0).
 int launch_logit_stats(const void* x, const void* x_compact, const void* weight, const Rows& rows, int channels, int vocab,
-                       float log2_scale, float2* stats, void* power, long long ldp, int* error_flag,
+                       float log2_scale, const int* main_column, float2* stats, void* power, long long ldp,
+                       int* error_flag,
                        cudaStream_t stream);
 
 // The time of a rows x columns product whose contraction of `blocks` blocks of 64 is cut into s parts: a wave of pairs takes

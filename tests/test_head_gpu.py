@@ -535,3 +535,63 @@ def test_losses_accumulate_over_micro_batches_into_one_weight():
         x1.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("N,C,V", [(40, 64, 300), (25, 1032, 5000), (1, 256, 129), (6, 2048, 900)])
+@pytest.mark.parametrize("teacher", [False, True])
+def test_rows_that_are_nearly_certain(N, C, V, teacher):
+    """Losses from ordinary to 1e-20 keep their relative precision, and so do the gradients of each row by itself: with d the
+    distance of the others' log sum from the label's logit the loss is log(1 + e^d), whose relative error is at most d's
+    error, e_n above; g then has that relative error and its one rounding.  A teacher that is nearly certain as well (its
+    second entry between 1e-9 and 1e-1 of the first) has a loss that is a difference of two such terms, each with a relative
+    error of e_n + 16 u."""
+    import flashrwkv_b200 as F
+    from oracle import head_norm_oracle as O
+
+    gen = torch.Generator().manual_seed(N + C)
+    w = (torch.randn(V, C, generator=gen) * 2 / C ** 0.5).to(torch.bfloat16).cuda()
+    t = torch.randint(V, (N,), generator=gen).cuda()
+    sure = torch.linspace(0, 14, N)[:, None].cuda() if N > 1 else torch.tensor([[7.0]], device="cuda")
+    x = (torch.randn(N, C, generator=gen).cuda() * 0.5 + sure * w[t].float()).to(torch.bfloat16)
+    x.requires_grad_(), w.requires_grad_()
+    if teacher:
+        idx = torch.stack((t, (t + 1) % V), 1)
+        gap = torch.logspace(-9, -1, N).log().cuda() if N > 1 else torch.tensor([-8.0], device="cuda")
+        logits = torch.stack((torch.zeros(N, device="cuda"), gap), 1)
+        shares, _ = O.teacher_shares(logits, 1.0)
+        rows = F.pretrain_head_distill_bf16(x, w, logits, idx, reduction="none")
+    else:
+        idx, shares = t[:, None], torch.ones(N, 1, dtype=torch.float64, device="cuda")
+        rows = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    z = x.detach().double() @ w.detach().double().T
+    B = (x.detach().double().abs() @ w.detach().double().abs().T).amax(1)
+    e = 2 * (2 * C * U * B) + (300 + V // 128 + 1) * U + 2 ** -20 + 32 * U * z.abs().amax(1)
+    others = z.clone()
+    others[torch.arange(N), t] = float("-inf")
+    d = torch.logsumexp(others, 1) - z[torch.arange(N), t]
+    excess = torch.nn.functional.softplus(d)
+    if teacher:
+        p2 = shares[:, 1]
+        second = z[torch.arange(N), idx[:, 1]] - z[torch.arange(N), t]
+        want = excess - torch.log1p(torch.exp(gap.double())) + p2 * (gap.double() - second)
+        bound = (e + 16 * U) * (excess + torch.exp(gap.double())) + p2 * (e + 16 * U) * (1 + gap.double().abs() + second.abs())
+    else:
+        want, bound = excess, e * excess
+    assert teacher or N == 1 or (float(want.min()) < 1e-6 and float(want.max()) > 1)
+    _near(rows.detach(), want, bound + 2.0 ** -140, "row losses")
+    # each row's gradient by itself
+    g = torch.exp(z - z[torch.arange(N), t][:, None] - excess[:, None])
+    missing = torch.sigmoid(d)
+    if teacher:
+        g[torch.arange(N), idx[:, 1]] -= p2
+        g[torch.arange(N), t] = p2 - missing
+    else:
+        g[torch.arange(N), t] = -missing
+    dx = torch.autograd.grad(rows.sum(), x)[0].double()
+    want_dx = g @ w.detach().double()
+    scale = ((g ** 2) @ (w.detach().double() ** 2)).sum(1) + (want_dx ** 2).sum(1)
+    if teacher:  # q - p of an entry is a difference too
+        slack = 2 * (e + 16 * U) * (missing + p2) * w.detach().double().norm(dim=1).amax() * 2
+    else:
+        slack = 2 * e * scale.sqrt()
+    assert bool(((dx - want_dx).norm(dim=1) <= 4e-3 * scale.sqrt() + slack).all())
