@@ -161,9 +161,9 @@ __device__ int choose_splits(int most, float rows, float columns, float k, float
   return which;
 }
 
-// One CTA numbers the rows in order (8192 in 7 us, most of it two round trips): position[row] = compact number or -1, row_map its
-// inverse, main_column the label's column
-// (the teacher's highest entry's) by compact number, -1 where it lies outside the vocabulary.
+// One CTA numbers the rows in order (8192 in 7 us, most of it two round trips): position[row] = compact number or -1, row_map
+// its inverse, main_column the label's column (the teacher's highest entry's) by compact number, -1 where it lies outside the
+// vocabulary.
 __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, const int* __restrict__ highest, int* position,
                                                     int* __restrict__ row_map, int* __restrict__ main_column,
                                                     Plan* __restrict__ plan, SplitSizes sizes, CompactArgs compact,

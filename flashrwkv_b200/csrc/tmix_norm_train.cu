@@ -8,14 +8,15 @@
 //
 // A row belongs to a group of T threads with V 16-byte pieces each, which stays in registers from its one read to its
 // one write: every tensor crosses HBM once, which is the bound of both passes (forward 2 or 4, backward 3 or 4 tensors
-// of rows x C).  Groups of one warp need no barrier; small groups share a CTA of 256 threads.  Forward: four pieces per
+// of rows x C).  Groups of one warp need no barrier; small groups share a CTA of 256 threads (backward 512).  Forward: four pieces per
 // thread (8192 x 4096 in 25 us; two pieces 33 us, for want of bytes under way; with residual 38 us, its bytes take 42 at
 // the rate of a plain copy).  Backward: two pieces per thread; a CTA walks a slab of rows, keeps the column sums of dw and
 // db in registers along the walk, requests the next row before it reduces the present one, does its arithmetic on fp32
-// pairs (the pass is bound by instruction issue as much as by bytes) and writes one fp32 partial per CTA;
+// pairs (the pass is bound by instruction issue as much as by bytes) and writes one fp32 partial per CTA, one CTA per SM;
 // sum_slabs_kernel adds the partials in a fixed order, so the parameter gradients are the same on every run.  8192 x 4096
-// in 39 us, with a second gradient into the sum 47 us, where the bytes take 31 and 42.  A ring of rows in shared memory in
-// place of the row in registers was slower (56 us): the bytes were not what it waited for.
+// in 38 us, with a second gradient into the sum 49 us, where the bytes take 31 and 42, and 4 us for the slabs (two CTAs of
+// half the threads per SM: 41, 49 and 7).  A ring of rows in shared memory in place of the row in registers was slower (56
+// us): the bytes were not what it waited for.
 //
 // The reference has the inference forms only (flashrwkv2/tmix/normalization/__init__.py:31-90).
 
@@ -178,7 +179,7 @@ __device__ __forceinline__ void unpack_pairs(const uint4& u, f32x2 (&f)[4]) {
   }
 }
 
-__host__ __device__ constexpr int backward_threads(int T) { return T < 256 ? 256 : T; }
+__host__ __device__ constexpr int backward_threads(int T) { return T < 512 ? 512 : T; }
 
 // One row of the backward pass as it comes from memory.
 template <int V>
@@ -206,7 +207,7 @@ __device__ __forceinline__ void load_row(RowPieces<V>& r, const bf16* s, const b
 
 // kSum: a gradient reaches s beside the one through the norm.  kParams: dw and db are wanted.
 template <int T, int V, bool kSum, bool kParams>
-__global__ __launch_bounds__(backward_threads(T), backward_threads(T) >= 512 ? 1 : 2) void norm_backward_kernel(
+__global__ __launch_bounds__(backward_threads(T), 1) void norm_backward_kernel(
     const bf16* __restrict__ dy, const bf16* __restrict__ dsum, const bf16* __restrict__ s,
     const bf16* __restrict__ weight, const float* __restrict__ mean, const float* __restrict__ rstd,
     bf16* __restrict__ dx, bf16* __restrict__ dw, bf16* __restrict__ db, float* __restrict__ partials, long long rows,
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(kSumWarps * 32) void sum_slabs_kernel(const float* 
 
 // ---- host side -----------------------------------------------------------------------------------------------------
 constexpr int kMaxChannels = 512 * 4 * 8;
-constexpr int kSlabsPerSm = 2;
+constexpr int kSlabsPerSm = 1;
 constexpr int kForwardPieces = 4, kBackwardPieces = 2;
 
 constexpr int kKnownDevices = 64;  // what a device answered once is kept: the queries cost as much as a launch
@@ -452,7 +453,7 @@ struct NormPlan {
   int slabs;
   long long rows_per_cta;
 };
-// Slabs of at least four rows, and no more than `resident` CTAs per SM at once: fewer slabs mean fewer partials.
+// Slabs of at least four rows, and no more of them than one wave of CTAs: fewer slabs mean fewer partials.
 NormPlan plan_backward(long long rows, int resident, int dev) {
   const long long most = (long long)sm_count(dev) * resident;
   long long slabs = (rows + 3) / 4;
