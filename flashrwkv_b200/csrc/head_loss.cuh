@@ -57,7 +57,8 @@ int launch_grad_weight(const void* g, long long ldg, const void* x, const void* 
                        cudaStream_t stream);
 
 // Up to 128 rows one CTA works alone on a 128 x 256 tile: a pair's tile would be half empty, and the loads of W, which bound
-// the product then, would wait for twice the tensor-core time per byte.
+// the product then, would wait for twice the tensor-core time per byte (a step of 16 x 65536 x 1024 164 us by pairs, 152 alone; 128 x 65536 x 2048
+// 287 and 271 us).
 constexpr bool one_cta(long long rows) { return rows <= kTile / 2; }
 
 int pair_count();  // of CTAs that the current device runs at once

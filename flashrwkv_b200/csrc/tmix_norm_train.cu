@@ -335,8 +335,8 @@ __global__ __launch_bounds__(backward_threads(T), 1) void norm_backward_kernel(
   }
 }
 
-// dw and db of rows too wide for one CTA's registers to hold the column sums beside the row: a pass of its own over s and
-// dy.  A warp takes 256 channels, a CTA's four warps a quarter of its slab each.
+// dw and db of rows too wide for one CTA's registers to hold the column sums beside the row (above 8192 channels): a pass of
+// its own over s and dy (2048 x 16384: 89 us in all, 132 with sums that spill).  A warp takes 256 channels, a CTA's four warps a quarter of its slab each.
 __global__ __launch_bounds__(128) void norm_columns_kernel(const bf16* __restrict__ dy, const bf16* __restrict__ s,
                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
                                                            float* __restrict__ partials, long long rows, int channels,
@@ -419,32 +419,16 @@ __global__ __launch_bounds__(kSumWarps * 32) void sum_slabs_kernel(const float* 
 
 // ---- host side -----------------------------------------------------------------------------------------------------
 constexpr int kMaxChannels = 512 * 4 * 8;
-constexpr int kSlabsPerSm = 1;
 constexpr int kForwardPieces = 4, kBackwardPieces = 2;
 
 constexpr int kKnownDevices = 64;  // what a device answered once is kept: the queries cost as much as a launch
 
-int sm_count(int dev) {
+int sm_count() {
   static std::atomic<int> known[kKnownDevices];
-  int n = 0;
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
   if (dev < kKnownDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-  if (dev < kKnownDevices) known[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
-
-int current_device() {
-  int dev = 0;
-  return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
-}
-
-// CTAs of a kernel that an SM holds, 0 on an error
-template <auto kernel>
-int resident_ctas(int dev, int threads) {
-  static std::atomic<int> known[kKnownDevices];
-  int n = 0;
-  if (dev < kKnownDevices && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess) return 0;
   if (dev < kKnownDevices) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
@@ -454,8 +438,8 @@ struct NormPlan {
   long long rows_per_cta;
 };
 // Slabs of at least four rows, and no more of them than one wave of CTAs: fewer slabs mean fewer partials.
-NormPlan plan_backward(long long rows, int resident, int dev) {
-  const long long most = (long long)sm_count(dev) * resident;
+NormPlan plan_backward(long long rows) {
+  const long long most = sm_count();
   long long slabs = (rows + 3) / 4;
   if (slabs > most) slabs = most;
   const long long per = (rows + slabs - 1) / slabs;
@@ -519,7 +503,7 @@ extern "C" int frwkv_pretrain_layer_norm_forward(const void* x, const void* resi
 
 extern "C" long long frwkv_pretrain_layer_norm_workspace_floats(long long rows, int channels) {
   if (rows <= 0 || channels <= 0) return 0;
-  const long long slabs = frwkv::plan_backward(rows, frwkv::kSlabsPerSm, frwkv::current_device()).slabs;
+  const long long slabs = frwkv::plan_backward(rows).slabs;
   return slabs * 2 * channels;
 }
 
@@ -544,12 +528,9 @@ extern "C" int frwkv_pretrain_layer_norm_backward(const void* grad_out, const vo
     constexpr int T = decltype(t)::value, V = decltype(v)::value;
     constexpr bool kApart = T > 512;  // the column sums take a pass of their own
     const bool parameters = grad_weight != nullptr;
-    NormPlan plan{};
+    const NormPlan plan = plan_backward(rows);
     const auto run = [&](auto sum_known, auto params) {
       constexpr auto kernel = norm_backward_kernel<T, V, decltype(sum_known)::value, decltype(params)::value>;
-      const int dev = current_device(), resident = resident_ctas<kernel>(dev, backward_threads(T));
-      if (resident < 1) return fail(FRWKV_ERR_CUDA, "pretrain_layer_norm_backward: no CTA fits an SM");
-      plan = plan_backward(rows, resident < kSlabsPerSm ? resident : kSlabsPerSm, dev);
       launch_chained(kernel, dim3(plan.slabs), dim3(backward_threads(T)), 0, s, static_cast<const bf16*>(grad_out),
                      static_cast<const bf16*>(grad_sum), static_cast<const bf16*>(sum), static_cast<const bf16*>(weight), mean,
                      rstd, static_cast<bf16*>(grad_x), static_cast<bf16*>(grad_weight), static_cast<bf16*>(grad_bias),
