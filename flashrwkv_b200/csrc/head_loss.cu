@@ -51,6 +51,12 @@ constexpr double kTruncation = 1.03e-9;
 constexpr int kFinishThreads = 256;
 constexpr int kFewRows = 64;  // copied by the plan: a launch less (2 us) while a warp has two rows at most
 
+// Rows of labels that a warp each finishes rather than a CTA: a step of 8000 x 1000 x 512 takes 78 us so and 122 by CTAs, 4000 x
+// 4096 x 256 81 and 100, 3000 x 8000 x 768 138 and 146, but 100 x 8000 x 768 51 and 48, and 300 x 16000 x 256 80 and 54.
+constexpr bool short_rows(long long ldg, int rows) {
+  return rows > kFewRows && (ldg <= 4096 || (ldg <= 8192 && rows >= 1024));
+}
+
 struct Labels {
   const void* index;        // [rows][top] int32 or int64
   bool wide;                // int64
@@ -345,14 +351,37 @@ __device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count, f
   if (threadIdx.x == 0) *a.loss = a.mean && count > 0 ? v / (float)count : v;  // no row takes part: 0
 }
 
-// The losses of labels alone, without gradients: a warp per row (4096 x 65536 in 13 us; a CTA per row took 51).
-__global__ __launch_bounds__(kFinishThreads) void losses_kernel(const FinishArgs a) {
+// what a row's logit gradients are scaled by, NaN with its loss
+__device__ __forceinline__ float grad_scale_of(const FinishArgs& a, long long n, int count, float loss) {
+  float scale = a.labels.temperature;
+  if (a.mean) scale /= (float)count;
+  if (a.row_grads != nullptr) scale *= a.row_grads[n];
+  if (a.grad_scale != nullptr) scale *= *a.grad_scale;
+  return loss != loss ? quiet_nan() : scale;
+}
+// eight fp16 exponentials to bf16 logit gradients
+__device__ __forceinline__ uint4 scaled(const uint4& e, float f) {
+  const uint32_t in[4] = {e.x, e.y, e.z, e.w};
+  uint32_t out[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const float2 t = Io16<__half>::unpack(in[h]);
+    out[h] = IO::pack(t.x * f, t.y * f);
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+// What finish_kernel does, by a warp per row and for labels alone: without gradients (4096 x 65536 in 13 us; a CTA per row took
+// 51), and with them where rows are short and a CTA would mostly wait for its own reductions (short_rows).
+__global__ __launch_bounds__(kFinishThreads) void finish_by_warps_kernel(const FinishArgs a) {
   chain_begin();
   __shared__ float scratch[kFinishThreads / 32];
   const int tiles = (a.vocab + kStatsTile - 1) / kStatsTile, lane = threadIdx.x & 31;
   const int count = *a.rows.count, left = count - a.rows.piece_begin;
   const int rows_here = left < 0 ? 0 : (left < a.rows.piece_rows ? left : a.rows.piece_rows);
   const int r = blockIdx.x * (kFinishThreads / 32) + (threadIdx.x >> 5);
+  const int groups = (int)(a.ldg / 8);
+  uint4* g = a.g + (long long)r * groups;
   if (r < rows_here) {
     const long long n = a.rows.row_map[a.rows.piece_begin + r];
     const long long v = a.labels.at(n);
@@ -372,7 +401,27 @@ __global__ __launch_bounds__(kFinishThreads) void losses_kernel(const FinishArgs
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float logit = inside ? label_logit(a.x + n * a.channels, a.weight + v * a.channels, a.channels / 8, lane) : 0.f;
-    if (lane == 0) a.row_losses[n] = inside ? row_sums(high, sum, logit).excess : quiet_nan();
+    const RowSums row = row_sums(high, sum, logit);
+    const float loss = inside ? row.excess : quiet_nan();
+    if (lane == 0) a.row_losses[n] = loss;
+    if (a.g != nullptr) {
+      const float scale = grad_scale_of(a, n, count, loss);
+      for (int begin = lane; begin < groups; begin += 128) {
+        uint4 e[4];  // four pieces requested together
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (begin + 32 * j < groups) e[j] = g[begin + 32 * j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = begin + 32 * j;
+          if (i < groups) g[i] = scaled(e[j], scale * ex2_approx(__ldg(&stats[i / (kStatsTile / 8)].x) - row.lse2));
+        }
+      }
+      __syncwarp();
+      if (lane == 0 && inside) reinterpret_cast<bf16*>(g)[v] = IO::store(-scale * row.missing);
+    }
+  } else if (a.g != nullptr && r < a.rows.piece_rows && r < ((rows_here + 63) & ~63)) {
+    for (int i = lane; i < groups; i += 32) g[i] = make_uint4(0u, 0u, 0u, 0u);
   }
   arrive_and_sum(a, count, scratch);
 }
@@ -462,11 +511,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   arrive_and_sum(a, count, scratch);
   if (a.g == nullptr) return;
 
-  float scale = a.labels.temperature;
-  if (a.mean) scale /= (float)count;
-  if (a.row_grads != nullptr) scale *= a.row_grads[n];
-  if (a.grad_scale != nullptr) scale *= *a.grad_scale;
-  if (loss != loss) scale = quiet_nan();
+  const float scale = grad_scale_of(a, n, count, loss);
   __syncthreads();  // the tiles' factors and the shares
   for (int begin = from + tid; begin < to; begin += 4 * kFinishThreads) {
     uint4 e[4];  // four pieces requested together
@@ -476,17 +521,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = begin + j * kFinishThreads;
-      if (i < to) {
-        const float f = scale * ex2_approx(factor[i / (kStatsTile / 8)]);
-        const uint32_t in[4] = {e[j].x, e[j].y, e[j].z, e[j].w};
-        uint32_t out[4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const float2 t = Io16<__half>::unpack(in[h]);
-          out[h] = IO::pack(t.x * f, t.y * f);
-        }
-        g[i] = make_uint4(out[0], out[1], out[2], out[3]);
-      }
+      if (i < to) g[i] = scaled(e[j], scale * ex2_approx(factor[i / (kStatsTile / 8)]));
     }
   }
   __syncthreads();
@@ -771,14 +806,14 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.row_losses = a.row_losses;
     f.loss = a.loss;
     f.arrived = &plan->arrived;
-    const bool by_warps = !grads && a.teacher_logits == nullptr;
+    const bool by_warps = a.teacher_logits == nullptr && (!grads || short_rows(l.ldg, l.piece_rows));
     // few rows are cut into parts, so that the device has two CTAs per SM to run (at most 16 parts of a row: one of 65536
     // entries then is two rounds of requests; 16 rows of 65536 take 10 us, 14 whole)
     const int parts = by_warps || !grads ? 1 : (l.piece_rows >= 148 ? 1 : (l.piece_rows > 18 ? 296 / l.piece_rows : 16));
     const int ctas = by_warps ? (l.piece_rows + kFinishThreads / 32 - 1) / (kFinishThreads / 32) : l.piece_rows;
     f.ctas = ctas * l.pieces;
     if (by_warps)
-      launch_chained(losses_kernel, dim3(ctas), dim3(kFinishThreads), 0, s, f);
+      launch_chained(finish_by_warps_kernel, dim3(ctas), dim3(kFinishThreads), 0, s, f);
     else
       launch_chained(finish_kernel, dim3(ctas, parts), dim3(kFinishThreads), finish_smem, s, f);
     if (int rc = check_launch("finish_kernel")) return rc;
