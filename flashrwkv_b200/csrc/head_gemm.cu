@@ -1,9 +1,11 @@
 // The three matrix products of the head's losses on the 5th-generation tensor cores:
 //
 //   statistics    z = x W^T                 per 128 columns: row maximum and sum of exponentials (and the exponentials)
-//   grad_x        dx = g W                  contraction over the vocabulary
-//   grad_weight   dW = g^T x                contraction over the rows
+//   dx = g W                                contraction over the vocabulary
+//   dW = g^T x                              contraction over the rows
 //
+// The last two share a launch: the units of dW fill what the last units of dx leave of the device (a step of 4096 x 8192 x 512
+// 134 us in two launches, 125 in one; 33 x 8191 x 512 44 and 39).
 // One persistent kernel, specialised by warp and run by pairs of CTAs (tcgen05, cta_group::2): a pair owns a 256 x 256
 // output tile, each CTA loads its 128 rows of A and its half of B, so that a byte of shared memory feeds twice the
 // arithmetic of a single CTA's 128 x 256 tile, which is bound by the fill of its shared memory.
@@ -15,9 +17,9 @@
 // All three operand layouts are read where they lie: x and W are K-major in z = x W^T; W in g W, and both g and x in g^T x,
 // are MN-major (the contraction index numbers the rows of the matrix in memory).  The number of rows that take part is known
 // on the device only (labels may be missing), so the kernels read it there.
-// 4096 x 32768 x 2048 (0.55 TFLOP each): 346, 366 and 337 us, tensor pipe 92 to 97 % active at the 1.45 to 1.55 GHz that the
+// 4096 x 32768 x 2048 (0.55 TFLOP each), each alone: 346, 366 and 337 us, tensor pipe 92 to 97 % active at the 1.45 to 1.55 GHz that the
 // power cap leaves; the library's plain products of these shapes take 357, 355 and 346 us.  With few rows the loads of W
-// bound it: 16 x 65536 x 1024 in 33 us for the statistics and 26 for dx (134 MB), 41 for dW, which is written.
+// bound it: 16 x 65536 x 1024 in 33 us for the statistics and 66 for both gradients (134 MB read, twice, and 134 written).
 // Every wait is bounded; a role whose wait runs out sets the error flag and leaves, the others run into their own limits,
 // outputs that could not be made are NaN.
 
@@ -48,59 +50,81 @@ struct Ring {
 };
 constexpr uint32_t kTmemCols = 2 * kTile;
 
-enum Product { kStats, kGradX, kGradWeight };
-
+// One launch makes the statistics; another both gradients, whose units follow one another (the long ones of dx first).
 struct Params {
-  CUtensorMap map_a, map_b;
-  CUtensorMap map_compact;  // kStats: A, kGradWeight: B, when some rows take no part
-  CUtensorMap map_out;      // kStats: the exponentials, kGradWeight: the bf16 gradient
+  CUtensorMap map_a, map_b;            // of x and W, or of g and W for dx
+  CUtensorMap map_a_weight, map_b_weight;  // gradients: of g and x for dW
+  CUtensorMap map_compact;             // of x, where some rows take no part or all are copied
+  CUtensorMap map_out;                 // the exponentials, or the bf16 dW
   Rows rows;
   int channels, vocab;
-  Splits splits;           // kGradX, kGradWeight
-  float log2_scale;        // kStats
+  float log2_scale;        // statistics
   const int* main_column;
   float2* stats;
   int stats_tiles;
-  bool power;              // kStats: the exponentials are wanted
-  bf16* out;               // kGradX, kGradWeight
-  float* partials;
-  bool add;
+  bool power;              // the exponentials are wanted
+  Splits splits_x, splits_w;  // gradients
+  bf16* grad_x;            // null: not wanted
+  bf16* grad_weight;
+  float* partials_x;
+  float* partials_w;
+  bool add;                // to what partials_w holds
 };
 
 struct Unit {
+  bool of_weight;  // gradients: dW, not dx
   int m0, n0, split, kb_begin, kb_end;
   int width;  // columns of the tile, a multiple of 32: the last tile of a row may need fewer than 256
 };
 
-// the work of a launch, from the number of rows that take part
-template <Product P, int kCtas>
-struct Work {
+// the units of one product, from the number of rows that take part
+template <int kCtas>
+struct Part {
   static constexpr int kRows = kHalf * kCtas;
   int tiles_m, tiles_n, units, kb_total, splits, columns;
-  __device__ Work(const Params& p, int rows_here) {
-    const int m = P == kGradWeight ? p.vocab : rows_here;
-    const int n = P == kStats ? p.vocab : p.channels;
-    const int k = P == kStats ? p.channels : (P == kGradX ? p.vocab : rows_here);
+  __device__ void set(bool wanted, int m, int n, int k, int parts) {
     columns = n;
     tiles_m = (m + kRows - 1) / kRows;
     tiles_n = (n + kTile - 1) / kTile;
     kb_total = (k + kBK - 1) / kBK;
-    splits = P == kStats || p.partials == nullptr ? 1 : *p.splits.chosen;
-    units = tiles_m * tiles_n * splits;
+    splits = parts;
+    units = wanted ? tiles_m * tiles_n * splits : 0;
   }
   // Pairs that run at the same time work on neighbouring tiles of the same part of the contraction, so that they share
   // their operands in L2.  Statistics: rows vary fastest (the whole x against a few tiles of W); the gradients: columns.
-  __device__ Unit at(int unit) const {
+  __device__ Unit at(int unit, bool rows_first) const {
     Unit u;
     const int tiles = tiles_m * tiles_n;
     u.split = unit / tiles;
     const int t = unit - u.split * tiles;
-    u.m0 = (P == kStats ? t % tiles_m : t / tiles_n) * kRows;
-    u.n0 = (P == kStats ? t / tiles_m : t % tiles_n) * kTile;
+    u.m0 = (rows_first ? t % tiles_m : t / tiles_n) * kRows;
+    u.n0 = (rows_first ? t / tiles_m : t % tiles_n) * kTile;
     const int right = columns - u.n0;
     u.width = right < kTile ? (right + 31) & ~31 : kTile;
     u.kb_begin = (int)((long long)kb_total * u.split / splits);
     u.kb_end = (int)((long long)kb_total * (u.split + 1) / splits);
+    u.of_weight = false;
+    return u;
+  }
+};
+template <bool kGrads, int kCtas>
+struct Work {
+  Part<kCtas> first, second;  // the statistics, or dx and dW
+  int units;
+  __device__ Work(const Params& p, int rows_here) {
+    if (kGrads) {
+      first.set(p.grad_x != nullptr, rows_here, p.channels, p.vocab, p.partials_x != nullptr ? *p.splits_x.chosen : 1);
+      second.set(p.grad_weight != nullptr, p.vocab, p.channels, rows_here, p.partials_w != nullptr ? *p.splits_w.chosen : 1);
+    } else {
+      first.set(true, rows_here, p.vocab, p.channels, 1);
+      second.units = 0;
+    }
+    units = first.units + second.units;
+  }
+  __device__ Unit at(int unit) const {
+    if (!kGrads || unit < first.units) return first.at(unit, !kGrads);
+    Unit u = second.at(unit - first.units, false);
+    u.of_weight = true;
     return u;
   }
 };
@@ -137,13 +161,12 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, 
   }
 }
 
-template <Product P, int kCtas>
+template <bool kGrads, int kCtas>
 __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
   using R = Ring<kCtas>;
   constexpr bool kPair = kCtas == 2;
   constexpr int kStages = R::kStages;
   constexpr uint32_t kStageBytes = R::kStageBytes;
-  constexpr bool kAMn = P == kGradWeight, kBMn = P != kStats;
   extern __shared__ unsigned char smem_raw[];
   __shared__ uint64_t full_bar[kStages], empty_bar[kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_holder;
@@ -155,6 +178,10 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
   if (tid == 32) {  // the maps are parameters of this launch: fetched while the kernel before still runs
     umma2::prefetch_map(&prm.map_a);
     umma2::prefetch_map(&prm.map_b);
+    if (kGrads) {
+      umma2::prefetch_map(&prm.map_a_weight);
+      umma2::prefetch_map(&prm.map_b_weight);
+    }
   }
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -184,7 +211,7 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
   const int left = count - prm.rows.piece_begin;
   const int rows_here = left < 0 ? 0 : (left < prm.rows.piece_rows ? left : prm.rows.piece_rows);
   const bool compact = prm.rows.copied || count != prm.rows.total;
-  const Work<P, kCtas> work(prm, rows_here);
+  const Work<kGrads, kCtas> work(prm, rows_here);
   const int pair = blockIdx.x / kCtas, pairs = gridDim.x / kCtas;  // "pair" is the CTA where it works alone
   bool ok = true;
 
@@ -192,12 +219,13 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
     return __all_sync(0xffffffffu, umma::mbar_wait(bar, parity)) != 0;
   };
   if (warp == 0) {
-    const CUtensorMap* map_a = P == kStats && compact ? &prm.map_compact : &prm.map_a;
-    const CUtensorMap* map_b = P == kGradWeight && compact ? &prm.map_compact : &prm.map_b;
-    const int a_row = P == kStats ? prm.rows.piece_begin : 0, b_row = P == kGradWeight ? prm.rows.piece_begin : 0;
     uint32_t it = 0;
     for (int unit = pair; unit < work.units && ok; unit += pairs) {
       const Unit u = work.at(unit);
+      const bool a_mn = kGrads && u.of_weight;
+      const CUtensorMap* map_a = a_mn ? &prm.map_a_weight : (!kGrads && compact ? &prm.map_compact : &prm.map_a);
+      const CUtensorMap* map_b = !a_mn ? &prm.map_b : (compact ? &prm.map_compact : &prm.map_b_weight);
+      const int a_row = kGrads ? 0 : prm.rows.piece_begin, b_row = a_mn ? prm.rows.piece_begin : 0;
       const int m = u.m0 + (int)rank * kHalf, n = u.n0 + (int)rank * (u.width / kCtas);
       for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
         const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
@@ -213,13 +241,13 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
         };
         if (umma2::elect_one()) {
           if (rank == 0) umma::mbar_expect_tx(&full_bar[s], kCtas * kStageBytes);
-          if (kAMn) {
-            load(a_dst, map_a, m, a_row + k);
-            load(a_dst + 8192, map_a, m + 64, a_row + k);
+          if (a_mn) {
+            load(a_dst, map_a, m, k);
+            load(a_dst + 8192, map_a, m + 64, k);
           } else {
             load(a_dst, map_a, k, a_row + m);
           }
-          if (kBMn) {
+          if (kGrads) {
 #pragma unroll
             for (int j = 0; j < 4 / kCtas; ++j) load(b_dst + j * 8192, map_b, n + 64 * j, b_row + k);
           } else {
@@ -236,9 +264,8 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      const uint64_t a_desc = kAMn ? umma2::desc_mn_major(tiles_base) : umma2::desc_k_major(tiles_base);
-      const uint64_t b_desc = kBMn ? umma2::desc_mn_major(tiles_base + kOperandBytes) : umma2::desc_k_major(tiles_base + kOperandBytes);
-      constexpr uint32_t kAStep = (kAMn ? 2048 : 32) >> 4, kBStep = (kBMn ? 2048 : 32) >> 4;  // 16 contraction values
+      const uint64_t b_desc = kGrads ? umma2::desc_mn_major(tiles_base + kOperandBytes) : umma2::desc_k_major(tiles_base + kOperandBytes);
+      constexpr uint32_t kBStep = (kGrads ? 2048 : 32) >> 4;  // 16 contraction values
       const auto commit = [](uint64_t* bar) {
         if (kPair)
           umma2::commit_both(bar);
@@ -254,7 +281,10 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
         if (!wait(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
         umma::fence_after_sync();
         const uint32_t d_tmem = tmem + acc * kTile;
-        const uint32_t idesc = umma2::idesc_bf16(kHalf * kCtas, u.width, kAMn, kBMn);
+        const bool a_mn = kGrads && u.of_weight;
+        const uint32_t idesc = umma2::idesc_bf16(kHalf * kCtas, u.width, a_mn, kGrads);
+        const uint64_t a_desc = a_mn ? umma2::desc_mn_major(tiles_base) : umma2::desc_k_major(tiles_base);
+        const uint32_t a_step = (a_mn ? 2048 : 32) >> 4;
         for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
           const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
           if (!wait(&full_bar[s], ph)) { ok = false; break; }
@@ -265,9 +295,9 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
             for (int ks = 0; ks < kBK / 16; ++ks) {
               const uint32_t add = (kb > u.kb_begin || ks > 0) ? 1u : 0u;
               if (kPair)
-                umma2::mma_bf16(d_tmem, a + ks * kAStep, b + ks * kBStep, idesc, add);
+                umma2::mma_bf16(d_tmem, a + ks * a_step, b + ks * kBStep, idesc, add);
               else
-                umma2::mma_bf16_alone(d_tmem, a + ks * kAStep, b + ks * kBStep, idesc, add);
+                umma2::mma_bf16_alone(d_tmem, a + ks * a_step, b + ks * kBStep, idesc, add);
             }
             commit(&empty_bar[s]);
           }
@@ -282,7 +312,6 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
     const int column0 = (warp - 2) / 4 * kStatsTile;
     const uint32_t source0 = tmem + ((32u * quarter) << 16) + column0;
     const int row_in_tile = (int)rank * kHalf + 32 * (int)quarter + lane;
-    const int m_end = P == kGradWeight ? prm.vocab : rows_here;
     const uint32_t box = tiles_base + kStages * kStageBytes + (warp - 2) * kBoxBytes;
     uint32_t t = 0;
     for (int unit = pair; unit < work.units; unit += pairs) {
@@ -291,8 +320,9 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
       const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
       if (!empty) ++t;
       const int m = u.m0 + row_in_tile, n = u.n0 + column0;
-      int main = -1;  // kStats: where the row's label lies in this warp's columns
-      if (P == kStats && m < m_end) main = prm.main_column[prm.rows.piece_begin + m] - n;
+      const int m_end = u.of_weight ? prm.vocab : rows_here;
+      int main = -1;  // statistics: where the row's label lies in this warp's columns
+      if (!kGrads && m < m_end) main = prm.main_column[prm.rows.piece_begin + m] - n;
       // Warp-uniform outcome: the tensor-memory loads below need the whole warp.  Once a wait has run out, this unit and all
       // later ones read as NaN.
       if (ok && !empty && !wait(&acc_full[acc], aph)) ok = false;
@@ -307,7 +337,7 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
             umma2::arrive_cluster(kPair ? umma2::in_leader(&acc_empty[acc]) : umma::smem_u32(&acc_empty[acc]));
         }
       };
-      if (P == kStats) {
+      if (!kGrads) {
         float z[kStatsTile];
         if (ok && !empty) {
           uint32_t(&v)[kStatsTile / 32][32] = reinterpret_cast<uint32_t(&)[kStatsTile / 32][32]>(z);
@@ -350,10 +380,11 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
           }
         }
       } else {
-        const long long slot = (long long)u.split * (P == kGradX ? rows_here : prm.vocab);
+        const long long slot = (long long)u.split * m_end;
+        float* const partials = u.of_weight ? prm.partials_w : prm.partials_x;
         const bool inside = m < m_end;
-        const int row = P == kGradX && inside && prm.partials == nullptr ? prm.rows.row_map[prm.rows.piece_begin + m] : m;
-        const bool wide = (prm.channels & 15) == 0 && (reinterpret_cast<uintptr_t>(prm.out) & 31u) == 0;
+        const int row = !u.of_weight && inside && partials == nullptr ? prm.rows.row_map[prm.rows.piece_begin + m] : m;
+        const bool wide = (prm.channels & 15) == 0 && (reinterpret_cast<uintptr_t>(prm.grad_x) & 31u) == 0;
 #pragma unroll 1
         for (int c0 = 0; c0 < kStatsTile; c0 += 64) {
           float z[64];
@@ -367,13 +398,13 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
             for (int j = 0; j < 64; ++j) z[j] = ok ? 0.f : quiet_nan();
           }
           if (c0 == 64) release();
-          if (prm.partials != nullptr) {
+          if (partials != nullptr) {
             if (!inside) continue;
-            float* dst = prm.partials + (slot + m) * prm.channels + n + c0;
+            float* dst = partials + (slot + m) * prm.channels + n + c0;
 #pragma unroll
             for (int h = 0; h < 64; h += 8) {
               if (n + c0 + h < prm.channels) {  // channels are a multiple of 8
-                if (prm.add) {
+                if (u.of_weight && prm.add) {
                   const float4 a = *reinterpret_cast<const float4*>(dst + h), b = *reinterpret_cast<const float4*>(dst + h + 4);
                   z[h] += a.x; z[h + 1] += a.y; z[h + 2] += a.z; z[h + 3] += a.w;
                   z[h + 4] += b.x; z[h + 5] += b.y; z[h + 6] += b.z; z[h + 7] += b.w;
@@ -384,10 +415,10 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
                 store32(dst + h, o, true);
               }
             }
-          } else if (P == kGradWeight) {
+          } else if (u.of_weight) {
             if (n + c0 < prm.channels && m - lane < m_end) store_box<bf16>(&prm.map_out, n + c0, m - lane, box, z, lane);
           } else if (inside) {
-            bf16* dst = prm.out + (long long)row * prm.channels + n + c0;
+            bf16* dst = prm.grad_x + (long long)row * prm.channels + n + c0;
 #pragma unroll
             for (int h = 0; h < 64; h += 16) {
               uint32_t o[8];
@@ -405,9 +436,9 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
       }
     }
   }
-  if (P != kGradX && warp >= 2 && lane == 0) umma2::bulk_wait();  // this warp's stores, before the kernel may end
+  if (warp >= 2 && lane == 0) umma2::bulk_wait();  // this warp's stores, before the kernel may end
   if (!ok) {
-    if (error_flag != nullptr) atomicExch(error_flag, 1 + (int)P);
+    if (error_flag != nullptr) atomicExch(error_flag, kGrads ? 2 : 1);
     // give copies and MMAs that may still be in flight time to finish before the shared and tensor memory go away
     for (int i = 0; i < 64; ++i) __nanosleep(1000);
   }
@@ -423,14 +454,14 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
   }
 }
 
-template <Product P>
+template <bool kGrads>
 __global__ __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) void head_gemm_kernel(const __grid_constant__ Params prm,
                                                                                           int* error_flag) {
-  head_gemm<P, 2>(prm, error_flag);
+  head_gemm<kGrads, 2>(prm, error_flag);
 }
-template <Product P>
+template <bool kGrads>
 __global__ __launch_bounds__(kThreads, 1) void head_gemm_alone_kernel(const __grid_constant__ Params prm, int* error_flag) {
-  head_gemm<P, 1>(prm, error_flag);
+  head_gemm<kGrads, 1>(prm, error_flag);
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
@@ -464,10 +495,10 @@ bool make_map(CUtensorMap* map, const void* base, long long rows, long long colu
 
 long long tiles_of(long long n) { return (n + kTile - 1) / kTile; }
 
-// `units`: at most so many; a product with parts may be cut finer than the host knows and takes every pair
-template <Product P, int kCtas>
+// `units`: at most so many
+template <bool kGrads, int kCtas>
 int launch(const Params& prm, long long units, int* error_flag, cudaStream_t stream) {
-  constexpr auto kernel = kCtas == 2 ? head_gemm_kernel<P> : head_gemm_alone_kernel<P>;
+  constexpr auto kernel = kCtas == 2 ? head_gemm_kernel<kGrads> : head_gemm_alone_kernel<kGrads>;
   static std::atomic<bool> ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = 64;
@@ -515,44 +546,40 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
       !make_map(&prm.map_b, weight, vocab, channels, channels, few ? kTile : kHalf) ||
       (power != nullptr && !make_map(&prm.map_out, power, rows.piece_rows, ldp, ldp, 32)))
     return map_failure();
-  if (few) return launch<kStats, 1>(prm, tiles_of(vocab), error_flag, stream);
-  return launch<kStats, 2>(prm, tiles_of(rows.piece_rows) * tiles_of(vocab), error_flag, stream);
+  if (few) return launch<false, 1>(prm, tiles_of(vocab), error_flag, stream);
+  return launch<false, 2>(prm, tiles_of(rows.piece_rows) * tiles_of(vocab), error_flag, stream);
 }
 
-int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab,
-                  const Splits& splits, void* grad_x, float* partials, int* error_flag, cudaStream_t stream) {
+int launch_gradients(const void* g, long long ldg, const void* x, const void* x_compact, const void* weight, const Rows& rows,
+                     int channels, int vocab, const GradTarget& to_x, const GradTarget& to_weight, bool add, int* error_flag,
+                     cudaStream_t stream) {
   Params prm{};
   prm.rows = rows;
   prm.channels = channels;
   prm.vocab = vocab;
-  prm.splits = splits;
-  prm.out = static_cast<bf16*>(grad_x);
-  prm.partials = partials;
-  if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kHalf) ||
-      !make_map(&prm.map_b, weight, vocab, channels, channels, kBK))
-    return map_failure();
-  const long long units = tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1);
-  if (one_cta(rows.piece_rows)) return launch<kGradX, 1>(prm, units, error_flag, stream);
-  return launch<kGradX, 2>(prm, tiles_of(rows.piece_rows) * units, error_flag, stream);
-}
-
-int launch_grad_weight(const void* g, long long ldg, const void* x, const void* x_compact, const Rows& rows, int channels,
-                       int vocab, const Splits& splits, void* grad_weight, float* partials, bool add, int* error_flag,
-                       cudaStream_t stream) {
-  Params prm{};
-  prm.rows = rows;
-  prm.channels = channels;
-  prm.vocab = vocab;
-  prm.splits = splits;
-  prm.out = static_cast<bf16*>(grad_weight);
-  prm.partials = partials;
+  prm.splits_x = to_x.splits;
+  prm.splits_w = to_weight.splits;
+  prm.grad_x = static_cast<bf16*>(to_x.grad);
+  prm.grad_weight = static_cast<bf16*>(to_weight.grad);
+  prm.partials_x = to_x.partials;
+  prm.partials_w = to_weight.partials;
   prm.add = add;
-  if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kBK) ||
-      !make_map(&prm.map_b, x, rows.total, channels, channels, kBK) ||
+  if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kHalf) ||
+      !make_map(&prm.map_b, weight, vocab, channels, channels, kBK) ||
+      !make_map(&prm.map_a_weight, g, rows.piece_rows, vocab, ldg, kBK) ||
+      !make_map(&prm.map_b_weight, x, rows.total, channels, channels, kBK) ||
       !make_map(&prm.map_compact, x_compact, rows.total, channels, rows.ldx, kBK) ||
-      (partials == nullptr && !make_map(&prm.map_out, grad_weight, vocab, channels, channels, 32)))
+      (to_weight.grad != nullptr && to_weight.partials == nullptr &&
+       !make_map(&prm.map_out, to_weight.grad, vocab, channels, channels, 32)))
     return map_failure();
-  return launch<kGradWeight, 2>(prm, tiles_of(vocab) * tiles_of(channels) * (splits.most > 1 ? 1 << 10 : 1), error_flag, stream);
+  // at most so many units; a product with parts may be cut finer than the host knows and takes every pair
+  const bool alone = one_cta(rows.piece_rows);
+  const auto units = [&](const GradTarget& t, long long m) {
+    const long long tiles = (alone ? (m + kHalf - 1) / kHalf : tiles_of(m)) * tiles_of(channels);
+    return t.grad == nullptr ? 0 : (t.partials != nullptr ? tiles << 10 : tiles);
+  };
+  const long long most = units(to_x, rows.piece_rows) + units(to_weight, vocab);
+  return alone ? launch<true, 1>(prm, most, error_flag, stream) : launch<true, 2>(prm, most, error_flag, stream);
 }
 
 }  // namespace head

@@ -817,19 +817,17 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     else
       launch_chained(finish_kernel, dim3(ctas, parts), dim3(kFinishThreads), finish_smem, s, f);
     if (int rc = check_launch("finish_kernel")) return rc;
-    if (a.grad_x != nullptr) {
-      if (int rc = launch_grad_x(power, l.ldg, a.weight, here, a.channels, a.vocab, Splits{&plan->splits_x, l.splits_x}, a.grad_x, partial_x,
-                                 a.error_flag, s))
+    if (grads) {
+      const GradTarget to_x{a.grad_x, partial_x, Splits{&plan->splits_x, l.splits_x}};
+      const GradTarget to_weight{a.grad_weight, partial_w, Splits{&plan->splits_w, l.splits_w}};
+      if (int rc = launch_gradients(power, l.ldg, a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab, to_x, to_weight,
+                                    piece > 0, a.error_flag, s))
         return rc;
-      if (l.parts_x)
+      if (a.grad_x != nullptr && l.parts_x)
         if (int rc = launch_sum_parts(partial_x, a.grad_x, row_map, plan, true, here.piece_begin, l.piece_rows, a.channels,
                                       l.splits_x, s))
           return rc;
     }
-    if (a.grad_weight != nullptr)
-      if (int rc = launch_grad_weight(power, l.ldg, a.x, ws + l.x_compact, here, a.channels, a.vocab,
-                                      Splits{&plan->splits_w, l.splits_w}, a.grad_weight, partial_w, piece > 0, a.error_flag, s))
-        return rc;
   }
   if (a.grad_weight != nullptr && l.parts_w)
     if (int rc = launch_sum_parts(partial_w, a.grad_weight, row_map, plan, false, 0, a.vocab, a.channels, l.splits_w, s)) return rc;

@@ -45,16 +45,20 @@ struct Splits {
   int most;           // partial sums have room for `most` parts of all rows; 1: none are kept
 };
 
-// grad_x[row_map[row]] = g[row] W, contraction over the vocabulary: with room for one part bf16 rows go straight to grad_x,
-// else fp32 parts to partials[part][rows that take part][channels].
-int launch_grad_x(const void* g, long long ldg, const void* weight, const Rows& rows, int channels, int vocab,
-                  const Splits& splits, void* grad_x, float* partials, int* error_flag, cudaStream_t stream);
+// Where a gradient goes: with room for one part bf16 straight to `grad` (null: not wanted), else fp32 parts to
+// partials[part][rows of the product][channels].
+struct GradTarget {
+  void* grad;
+  float* partials;
+  Splits splits;
+};
 
-// grad_weight = g^T x, contraction over the rows of the piece: bf16 straight to grad_weight, or (partials given) fp32 parts in
-// partials[part][vocab][channels], added to what they hold where `add`.
-int launch_grad_weight(const void* g, long long ldg, const void* x, const void* x_compact, const Rows& rows, int channels,
-                       int vocab, const Splits& splits, void* grad_weight, float* partials, bool add, int* error_flag,
-                       cudaStream_t stream);
+// One launch for both gradients: grad_x[row_map[row]] = g[row] W, contraction over the vocabulary (its parts have the rows that
+// take part), and grad_weight = g^T x, contraction over the rows of the piece (its parts are added to what they hold where
+// `add`).  The units of dW fill what the last units of dx leave of the device.
+int launch_gradients(const void* g, long long ldg, const void* x, const void* x_compact, const void* weight, const Rows& rows,
+                     int channels, int vocab, const GradTarget& to_x, const GradTarget& to_weight, bool add, int* error_flag,
+                     cudaStream_t stream);
 
 // Up to 128 rows one CTA works alone on a 128 x 256 tile: a pair's tile would be half empty, and the loads of W, which bound
 // the product then, would wait for twice the tensor-core time per byte (a step of 16 x 65536 x 1024 164 us by pairs, 152 alone; 128 x 65536 x 2048
