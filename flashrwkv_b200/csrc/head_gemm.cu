@@ -481,7 +481,8 @@ EncodeTiledFn encode_tiled() {
   return fn;
 }
 
-// [rows][columns] 16-bit values (copied as they are) with rows `stride` values apart, boxes of 64 columns x box_rows, 128-byte swizzle, zeros outside
+// [rows][columns] 16-bit values (copied as they are) with rows `stride` values apart, boxes of 64 columns x box_rows,
+// 128-byte swizzle, zeros outside
 bool make_map(CUtensorMap* map, const void* base, long long rows, long long columns, long long stride, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};

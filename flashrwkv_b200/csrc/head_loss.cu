@@ -22,7 +22,7 @@
 //            value would add 2^-9 to the one rounding that g needs as a tensor-core operand)
 //   finish   per row: O from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
 //            the exponentials times their tile's factor in place, now g in bf16; the labels' entries from fp32
-//   products dx and dW
+//   products dx and dW, in one launch
 // so a step costs three products of 2 rows x vocabulary x channels, not the four of recomputing z for the backward pass,
 // and the weight is read twice.  The price is that gradients are made with the loss, before the upstream gradient is known:
 // scale_kernel applies it afterwards (it leaves at once where the gradient is one).
@@ -546,9 +546,9 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
 }
 
 // ---- small passes ------------------------------------------------------------------------------------------------------
-// out[row_map ? row_map[row_begin + row] : row][c] = sum of the parts, bound by their bytes (2 x 8192 x 2048 in 38 us).  A thread takes four columns of every kWarps-th part;
-// with eight warps to an output (many parts of few rows: 32 of 33 x 512 in 4 us, 14 with one) their sums are added in warp
-// order.
+// out[row_map ? row_map[row_begin + row] : row][c] = sum of the parts, bound by their bytes (two of 8192 x 2048 in 38 us).  A
+// thread takes four columns of every kWarps-th part; with eight warps to an output (many parts of few rows: 32 of 33 x 512 in 4
+// us, 14 with one) their sums are added in warp order.
 template <int kWarps>
 __global__ __launch_bounds__(256) void sum_parts_kernel(const float4* __restrict__ partials, uint2* __restrict__ out,
                                                         const int* __restrict__ row_map, const Plan* __restrict__ plan,
@@ -782,12 +782,12 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     if (int rc = check_launch("compact_kernel")) return rc;
   }
 
+  const float log2_scale = (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature);
   const size_t finish_smem = (size_t)(tiles + 2 * a.top) * sizeof(float);
   for (int piece = 0; piece < l.pieces; ++piece) {
     const Rows here{count, row_map, rows, compact.always, l.ldx, piece * l.piece_rows, l.piece_rows};
-    if (int rc = launch_logit_stats(a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab,
-                                    (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature), main_column, stats, power, l.ldg,
-                                    a.error_flag, s))
+    if (int rc = launch_logit_stats(a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab, log2_scale, main_column, stats,
+                                    power, l.ldg, a.error_flag, s))
       return rc;
     FinishArgs f{};
     f.rows = here;
