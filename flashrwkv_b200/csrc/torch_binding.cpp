@@ -30,6 +30,14 @@ frwkv_stream_t current_stream(const torch::Tensor& t) {
   return reinterpret_cast<frwkv_stream_t>(at::cuda::getCurrentCUDAStream(t.device().index()).stream());
 }
 
+// which capture the tensor's current stream is in; 0 for none
+int64_t capture_of(const torch::Tensor& t) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(t.device().index()).stream(), &status, &id));
+  return status == cudaStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
+}
+
 void check_rc(int rc) {
   if (rc == FRWKV_OK) return;
   TORCH_CHECK(false, frwkv_last_error());
@@ -2113,7 +2121,8 @@ HeadResult head_pass(const HeadInputs& in, bool mean, bool want_x, bool want_wei
 
 // Forward makes the losses and, for a scalar loss, the gradients with them: the product that gives the logits is then done
 // once.  The upstream gradient scales them in place, which uses them up; a second backward pass through the same node makes
-// them anew.  Row losses have an upstream gradient per row, which has to be known first: their backward pass makes both.
+// them anew, and so does one that is captured without its forward pass (each of its replays would scale them once more) or
+// follows a captured one (whose replays write them).  Row losses have an upstream gradient per row, which has to be known first: their backward pass makes both.
 struct HeadLoss : torch::autograd::Function<HeadLoss> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
                                const torch::Tensor& labels, const std::optional<torch::Tensor>& teacher,
@@ -2128,6 +2137,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     ctx->saved_data["reduction"] = reduction;
     if (scalar && (want_x || want_weight)) {
       ctx->saved_data["grads"] = c10::IValue(std::make_tuple(r.grad_x, r.grad_weight));
+      ctx->saved_data["capture"] = capture_of(x);
     }
     return scalar ? r.loss : r.row_losses;
   }
@@ -2140,7 +2150,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     const auto upstream = grads[0].contiguous();
     torch::Tensor gx, gw;
     const auto kept = ctx->saved_data.find("grads");
-    if (kept != ctx->saved_data.end()) {
+    if (kept != ctx->saved_data.end() && ctx->saved_data["capture"].toInt() == capture_of(saved[0])) {
       const auto pair = kept->second.toTuple();
       gx = want_x ? pair->elements()[0].toTensor() : torch::Tensor();
       gw = want_weight ? pair->elements()[1].toTensor() : torch::Tensor();

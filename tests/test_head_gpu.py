@@ -595,3 +595,31 @@ def test_rows_that_are_nearly_certain(N, C, V, teacher):
     else:
         slack = 2 * e * scale.sqrt()
     assert bool(((dx - want_dx).norm(dim=1) <= 4e-3 * scale.sqrt() + slack).all())
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_a_captured_backward_pass_of_a_call_made_before_may_be_replayed(reduction):
+    """The gradients that the loss left behind are used up by one pass; every replay has to make them again."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(300, 264, 2100, 21)
+    t[::7] = -100
+    x.requires_grad_(), w.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        up = torch.full((300,) if reduction == "none" else (), 2.0, device="cuda")
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction=reduction)
+        again = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction=reduction)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        held = torch.autograd.grad(loss, (x, w), up, retain_graph=True)
+    for scale in (2.0, 2.0, 0.5):
+        with torch.cuda.stream(side):
+            up.fill_(scale)
+            g.replay()
+            want = torch.autograd.grad(again, (x, w), up, retain_graph=True)
+        side.synchronize()
+        for a, b in zip(held, want):
+            assert torch.allclose(a.float(), b.float(), rtol=2**-6, atol=2**-7 * float(b.abs().max()))
