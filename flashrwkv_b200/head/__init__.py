@@ -4,7 +4,8 @@
 never kept: their exponentials live in a workspace of at most 1 GiB while a call runs (pieces of the rows where that is
 less than rows x V x 2 bytes).  The gradients of a scalar loss are made together with it, in the forward call, and only
 for the inputs that require one; the upstream gradient scales them when the backward pass runs.  A backward pass repeated
-over a retained graph makes them again.  The backward passes are not differentiable themselves.
+over a retained graph, or captured apart from its forward pass, makes them again.  The backward passes are not
+differentiable themselves.
 
 The reference fuses its cross entropy with an L2 penalty of the largest logit (`csrc/sm90/head/l2wrap_ce`), which is not
 part of these operators; it has no distillation.

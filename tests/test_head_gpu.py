@@ -623,3 +623,36 @@ def test_a_captured_backward_pass_of_a_call_made_before_may_be_replayed(reductio
         side.synchronize()
         for a, b in zip(held, want):
             assert torch.allclose(a.float(), b.float(), rtol=2**-6, atol=2**-7 * float(b.abs().max()))
+
+
+def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves():
+    """Refused where that graph was made on the default stream; made on another stream it is no hindrance."""
+    import flashrwkv_b200 as F
+
+    def leaves():
+        x, w, t, _ = _rows(40, 128, 500, 22)
+        return x.requires_grad_(), w.requires_grad_(), t
+
+    x, w, t = leaves()
+    alive = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    with pytest.raises(RuntimeError, match="default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            F.pretrain_head_cross_entropy_bf16(x, w, t).backward()
+    torch.cuda.synchronize()
+    alive.backward()
+    want = [x.grad, w.grad]
+
+    x, w, t = leaves()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    side.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        F.pretrain_head_cross_entropy_bf16(x, w, t).backward()
+    g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip((x.grad, w.grad), want):
+        assert torch.equal(a, b)
+    del alive

@@ -261,3 +261,27 @@ def test_offsets_beyond_32_bits():
     slack = 3 * U * (g[-3:].double().abs() * (1 + want.double().abs())).sum(0)
     assert bool(((dw.double() - ew.double()).abs() <= 2 * HALF * ew.double().abs() + slack).all())
     assert bool(((db.double() - eb.double()).abs() <= 2 * HALF * eb.double().abs() + slack).all())
+
+
+def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves():
+    """Refused where that graph was made on the default stream and the leaf's gradient is asked for."""
+    import flashrwkv_b200 as F
+
+    x, r = (torch.randn(6, 5, 64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w, b = (torch.randn(64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    go = torch.randn_like(x)
+    for call in (lambda: F.pretrain_tmix_layer_norm_bf16(x, w, b), lambda: F.pretrain_tmix_add_layer_norm_bf16(x, r, w, b)[1]):
+        alive = call()
+        with pytest.raises(RuntimeError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(call(), (w, b), go)
+        torch.cuda.synchronize()
+        want = torch.autograd.grad(alive, (w, b), go)
+        del alive
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held = torch.autograd.grad(call(), (w, b), go)
+        g.replay()
+        torch.cuda.synchronize()
+        for got, value in zip(held, want):
+            assert torch.equal(got, value)
