@@ -2033,7 +2033,8 @@ void note_eager_leaves(AutogradContext* ctx, std::initializer_list<torch::Tensor
   if (eager) ctx->saved_data["eager"] = eager;
 }
 
-void refuse_eager_leaves(AutogradContext* ctx) {
+void refuse_eager_leaves(AutogradContext* ctx, const torch::Tensor& on) {
+  if (!capture_of(on)) return;  // an eager backward pass may wait on any stream, whatever its forward pass ran in
   const auto noted = ctx->saved_data.find("eager");
   if (noted == ctx->saved_data.end()) return;
   const int64_t eager = noted->second.toInt();
@@ -2056,8 +2057,9 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order();
-    refuse_eager_leaves(ctx);
-    auto [gx, gw, gb] = norm_backward(torch::Tensor(), grads[0], ctx->get_saved_variables(),
+    const auto saved = ctx->get_saved_variables();
+    refuse_eager_leaves(ctx, saved[0]);
+    auto [gx, gw, gb] = norm_backward(torch::Tensor(), grads[0], saved,
                                       ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
     return {gx, gw, gb, torch::Tensor()};
   }
@@ -2075,8 +2077,9 @@ struct AddLayerNormTrain : torch::autograd::Function<AddLayerNormTrain> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order();
-    refuse_eager_leaves(ctx);
-    auto [gx, gw, gb] = norm_backward(grads[0], grads[1], ctx->get_saved_variables(),
+    const auto saved = ctx->get_saved_variables();
+    refuse_eager_leaves(ctx, saved[0]);
+    auto [gx, gw, gb] = norm_backward(grads[0], grads[1], saved,
                                       ctx->needs_input_grad(2) || ctx->needs_input_grad(3));
     return {gx, gx, gw, gb, torch::Tensor()};
   }
@@ -2177,8 +2180,8 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order();
-    refuse_eager_leaves(ctx);
     const auto saved = ctx->get_saved_variables();
+    refuse_eager_leaves(ctx, saved[0]);
     const bool want_x = ctx->needs_input_grad(0), want_weight = ctx->needs_input_grad(1);
     const int64_t reduction = ctx->saved_data["reduction"].toInt();
     const auto upstream = grads[0].contiguous();

@@ -656,3 +656,20 @@ def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves():
     for a, b in zip((x.grad, w.grad), want):
         assert torch.equal(a, b)
     del alive
+
+
+def test_an_eager_backward_pass_behind_a_captured_forward_pass_beside_an_eager_graph():
+    """Only a captured backward pass cannot reach leaves of the default stream; this one makes the gradients anew."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(40, 128, 500, 23)
+    x.requires_grad_(), w.requires_grad_()
+    alive = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, t)
+    g.replay()
+    torch.cuda.synchronize()
+    got = torch.autograd.grad(loss, (x, w))
+    for a, b in zip((loss, *got), (alive, *torch.autograd.grad(alive, (x, w)))):
+        assert torch.equal(a, b)

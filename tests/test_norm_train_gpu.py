@@ -285,3 +285,22 @@ def test_a_captured_backward_pass_beside_an_eager_graph_of_the_same_leaves():
         torch.cuda.synchronize()
         for got, value in zip(held, want):
             assert torch.equal(got, value)
+
+
+def test_an_eager_backward_pass_behind_a_captured_forward_pass_beside_an_eager_graph():
+    """Only a captured backward pass cannot reach leaves of the default stream."""
+    import flashrwkv_b200 as F
+
+    x, r = (torch.randn(6, 5, 64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w, b = (torch.randn(64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    go = torch.randn_like(x)
+    for call in (lambda: F.pretrain_tmix_layer_norm_bf16(x, w, b), lambda: F.pretrain_tmix_add_layer_norm_bf16(x, r, w, b)[1]):
+        alive = call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        g.replay()
+        torch.cuda.synchronize()
+        got = torch.autograd.grad(out, (x, w, b), go)
+        for a, c in zip((out, *got), (alive, *torch.autograd.grad(alive, (x, w, b), go))):
+            assert torch.equal(a, c)
