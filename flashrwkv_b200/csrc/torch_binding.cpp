@@ -2016,31 +2016,19 @@ void refuse_second_order() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "this operator's backward pass is not itself differentiable (create_graph)");
 }
 
-// A leaf's gradients are gathered on the stream on which the first living graph over it was made.  When that is the default
-// stream, which cannot take part in a capture, autograd's attempt to wait on it inside one leaves the process in no state to
-// go on: such a call is refused before autograd gets there.  Which inputs are meant stands in "eager", a bit each.
-void note_eager_leaves(AutogradContext* ctx, std::initializer_list<torch::Tensor> inputs) {
-  if (!capture_of(*inputs.begin())) return;
-  int64_t eager = 0, bit = 1;
-  for (const auto& t : inputs) {
-    if (t.requires_grad() && t.is_leaf()) {
-      const auto gather = torch::autograd::impl::try_get_grad_accumulator(t);
-      const auto stream = gather ? gather->stream() : std::nullopt;
-      if (stream.has_value() && stream->id() == 0) eager |= bit;
-    }
-    bit <<= 1;
-  }
-  if (eager) ctx->saved_data["eager"] = eager;
-}
-
-void refuse_eager_leaves(AutogradContext* ctx, const torch::Tensor& on) {
+// Autograd makes the stream of every node that receives a gradient wait on the stream of the node that made it, and a leaf's
+// gradients are gathered on the stream on which the first living graph over it was made.  Inside a capture the default stream
+// cannot wait: autograd's attempt leaves the process in no state to go on.  A captured backward pass that would hand a
+// gradient there is refused before autograd gets to it, wherever its forward pass ran.
+void refuse_default_stream(const torch::Tensor& on) {
   if (!capture_of(on)) return;  // an eager backward pass may wait on any stream, whatever its forward pass ran in
-  const auto noted = ctx->saved_data.find("eager");
-  if (noted == ctx->saved_data.end()) return;
-  const int64_t eager = noted->second.toInt();
-  for (size_t i = 0; eager >> i; ++i) {
-    TORCH_CHECK(!(eager >> i & 1) || !ctx->needs_input_grad(i),
-                "a graph made on the default stream over the same leaf still lives: drop its outputs, or make it on another "
+  const auto node = torch::autograd::get_current_node();
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i);
+    if (!next.is_valid() || !node->task_should_compute_output(i)) continue;
+    const auto stream = next.function->stream();
+    TORCH_CHECK(!stream.has_value() || stream->id() != 0,
+                "a graph made on the default stream over the same input still lives: drop its outputs, or make it on another "
                 "stream, before a backward pass is captured");
   }
 }
@@ -2051,14 +2039,13 @@ struct LayerNormTrain : torch::autograd::Function<LayerNormTrain> {
     torch::Tensor sum, out, stats;
     norm_forward(x, nullptr, weight, bias, eps, sum, out, stats);
     ctx->save_for_backward({x, weight, stats});
-    note_eager_leaves(ctx, {x, weight, bias});
     ctx->set_materialize_grads(false);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order();
     const auto saved = ctx->get_saved_variables();
-    refuse_eager_leaves(ctx, saved[0]);
+    refuse_default_stream(saved[0]);
     auto [gx, gw, gb] = norm_backward(torch::Tensor(), grads[0], saved,
                                       ctx->needs_input_grad(1) || ctx->needs_input_grad(2));
     return {gx, gw, gb, torch::Tensor()};
@@ -2071,14 +2058,13 @@ struct AddLayerNormTrain : torch::autograd::Function<AddLayerNormTrain> {
     torch::Tensor sum, out, stats;
     norm_forward(x, &residual, weight, bias, eps, sum, out, stats);
     ctx->save_for_backward({sum, weight, stats});
-    note_eager_leaves(ctx, {x, residual, weight, bias});
     ctx->set_materialize_grads(false);
     return {sum, out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order();
     const auto saved = ctx->get_saved_variables();
-    refuse_eager_leaves(ctx, saved[0]);
+    refuse_default_stream(saved[0]);
     auto [gx, gw, gb] = norm_backward(grads[0], grads[1], saved,
                                       ctx->needs_input_grad(2) || ctx->needs_input_grad(3));
     return {gx, gx, gw, gb, torch::Tensor()};
@@ -2167,7 +2153,6 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
     const bool scalar = reduction != 0;
     auto r = head_pass(in, reduction == 2, want_x && scalar, want_weight && scalar, torch::Tensor(), torch::Tensor());
     ctx->save_for_backward({x, weight, labels, in.teacher});
-    note_eager_leaves(ctx, {x, weight});
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["reduction"] = reduction;
@@ -2181,7 +2166,7 @@ struct HeadLoss : torch::autograd::Function<HeadLoss> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     refuse_second_order();
     const auto saved = ctx->get_saved_variables();
-    refuse_eager_leaves(ctx, saved[0]);
+    refuse_default_stream(saved[0]);
     const bool want_x = ctx->needs_input_grad(0), want_weight = ctx->needs_input_grad(1);
     const int64_t reduction = ctx->saved_data["reduction"].toInt();
     const auto upstream = grads[0].contiguous();

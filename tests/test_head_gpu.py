@@ -673,3 +673,30 @@ def test_an_eager_backward_pass_behind_a_captured_forward_pass_beside_an_eager_g
     got = torch.autograd.grad(loss, (x, w))
     for a, b in zip((loss, *got), (alive, *torch.autograd.grad(alive, (x, w)))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_backward_pass_captured_apart_beside_an_eager_graph_of_the_same_leaves(reduction):
+    """The forward pass ran eagerly, on a stream that may be captured; the leaves belong to the default stream all the same."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(40, 128, 500, 24)
+    x.requires_grad_(), w.requires_grad_()
+    alive = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction=reduction)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        up = torch.full_like(alive.detach(), 0.5)
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction=reduction)
+    side.synchronize()
+    for leaves in ((x, w), (x,), (w,)):
+        with pytest.raises(RuntimeError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                torch.autograd.grad(loss, leaves, up, retain_graph=True)
+        torch.cuda.synchronize()
+    want = torch.autograd.grad(alive, (x, w), up)
+    with torch.cuda.stream(side):
+        got = torch.autograd.grad(loss, (x, w), up)
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)

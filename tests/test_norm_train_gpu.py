@@ -304,3 +304,37 @@ def test_an_eager_backward_pass_behind_a_captured_forward_pass_beside_an_eager_g
         got = torch.autograd.grad(out, (x, w, b), go)
         for a, c in zip((out, *got), (alive, *torch.autograd.grad(alive, (x, w, b), go))):
             assert torch.equal(a, c)
+
+
+def test_a_backward_pass_captured_apart_from_its_forward_pass():
+    """Refused while the leaves belong to a graph of the default stream; without one it is captured and replayed."""
+    import flashrwkv_b200 as F
+
+    x, r = (torch.randn(6, 5, 64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    w, b = (torch.randn(64, device="cuda").bfloat16().requires_grad_() for _ in range(2))
+    go = torch.randn_like(x)
+    side = torch.cuda.Stream()
+    for call in (lambda: F.pretrain_tmix_layer_norm_bf16(x, w, b), lambda: F.pretrain_tmix_add_layer_norm_bf16(x, r, w, b)[1]):
+        alive = call()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out = call()
+        side.synchronize()
+        for leaves in ((x, w, b), (x,), (b,)):
+            with pytest.raises(RuntimeError, match="default stream"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                    torch.autograd.grad(out, leaves, go, retain_graph=True)
+            torch.cuda.synchronize()
+        want = torch.autograd.grad(alive, (x, w, b), go)
+        del alive, out
+        with torch.cuda.stream(side):
+            out = call()
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            held = torch.autograd.grad(out, (x, w, b), go)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(held, want):
+            assert torch.equal(a, c)
+        del out
