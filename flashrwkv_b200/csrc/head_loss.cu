@@ -333,10 +333,13 @@ struct FinishArgs {
   int ctas;                  // of all pieces, the first part of a row each
 };
 
-// Called by every CTA that writes row losses.  The sum does not depend on who arrives last.
-__device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count, float* scratch) {
+// Called by every CTA that writes row losses.  The sum does not depend on who arrives last.  It runs in 64 bits and is rounded
+// once, with the division of a mean: in fp32 the 65536 additions of a thread (2^24 rows), all rounded the same way where the
+// row losses are alike, lose up to 1e-3 of it.
+__device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count) {
   if (a.loss == nullptr || blockIdx.y > 0) return;
   __shared__ bool last;
+  __shared__ double sums[kFinishThreads / 32];
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
@@ -345,10 +348,17 @@ __device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count, f
   __syncthreads();
   if (!last) return;
   __threadfence();
-  float v = 0.f;
-  for (int i = threadIdx.x; i < a.rows.total; i += kFinishThreads) v += __ldcg(a.row_losses + i);
-  v = block_reduce(v, scratch, false);
-  if (threadIdx.x == 0) *a.loss = a.mean && count > 0 ? v / (float)count : v;  // no row takes part: 0
+  double v = 0.0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < a.rows.total; i += kFinishThreads) v += (double)__ldcg(a.row_losses + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x > 0) return;
+#pragma unroll
+  for (int i = 1; i < kFinishThreads / 32; ++i) v += sums[i];
+  *a.loss = (float)(a.mean && count > 0 ? v / (double)count : v);  // no row takes part: 0
 }
 
 // what a row's logit gradients are scaled by, NaN with its loss
@@ -375,7 +385,6 @@ __device__ __forceinline__ uint4 scaled(const uint4& e, float f) {
 // 51), and with them where rows are short and a CTA would mostly wait for its own reductions (short_rows).
 __global__ __launch_bounds__(kFinishThreads) void finish_by_warps_kernel(const FinishArgs a) {
   chain_begin();
-  __shared__ float scratch[kFinishThreads / 32];
   const int tiles = (a.vocab + kStatsTile - 1) / kStatsTile, lane = threadIdx.x & 31;
   const int count = *a.rows.count, left = count - a.rows.piece_begin;
   const int rows_here = left < 0 ? 0 : (left < a.rows.piece_rows ? left : a.rows.piece_rows);
@@ -423,7 +432,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_by_warps_kernel(const F
   } else if (a.g != nullptr && r < a.rows.piece_rows && r < ((rows_here + 63) & ~63)) {
     for (int i = lane; i < groups; i += 32) g[i] = make_uint4(0u, 0u, 0u, 0u);
   }
-  arrive_and_sum(a, count, scratch);
+  arrive_and_sum(a, count);
 }
 
 // A row's loss, and with gradients its exponentials in place to logit gradients: bound by the bytes of the row there and back
@@ -449,7 +458,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     // zeros behind the last row, to the end of its block of the contraction over rows
     if (a.g != nullptr && r < ((rows_here + 63) & ~63))
       for (int i = from + tid; i < to; i += kFinishThreads) g[i] = make_uint4(0u, 0u, 0u, 0u);
-    arrive_and_sum(a, count, scratch);
+    arrive_and_sum(a, count);
     return;
   }
   const long long n = a.rows.row_map[a.rows.piece_begin + r];
@@ -508,7 +517,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   }
   if (bad) loss = quiet_nan();  // a label outside the vocabulary
   if (tid == 0 && blockIdx.y == 0) a.row_losses[n] = loss;
-  arrive_and_sum(a, count, scratch);
+  arrive_and_sum(a, count);
   if (a.g == nullptr) return;
 
   const float scale = grad_scale_of(a, n, count, loss);

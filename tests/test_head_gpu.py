@@ -700,3 +700,27 @@ def test_a_backward_pass_captured_apart_beside_an_eager_graph_of_the_same_leaves
     side.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("teacher", [False, True])
+@pytest.mark.parametrize("N", [1, 9000, (1 << 20) + 77])
+def test_the_scalar_loss_of_many_like_rows(N, teacher):
+    """Row losses that are all the same round the same way in every addition of a binade.  Their sum and their mean are each
+    rounded once, to half a step (2^-24); the sum of doubles that they are compared with is off by N 2^-53 at most."""
+    import flashrwkv_b200 as F
+
+    gen = torch.Generator().manual_seed(N)
+    w = torch.randn(3, 8, generator=gen).to(torch.bfloat16).cuda()
+    x = torch.randn(1, 8, generator=gen).to(torch.bfloat16).cuda().expand(N, 8).contiguous()
+    t = torch.full((N, 1), 2, device="cuda")
+    t[N // 2] = 0  # and one that differs
+
+    def call(reduction):
+        if teacher:
+            return F.pretrain_head_distill_bf16(x, w, torch.zeros(N, 1, device="cuda"), t, reduction=reduction)
+        return F.pretrain_head_cross_entropy_bf16(x, w, t[:, 0], reduction=reduction)
+
+    total = float(call("none").double().sum())
+    bound = (U + N * 2.0 ** -52) * total
+    assert abs(float(call("sum")) - total) <= bound
+    assert abs(float(call("mean")) - total / N) <= bound / N
