@@ -13,7 +13,8 @@
 //               the leader's barrier
 //   warp 1      (leader) MMA issuer: four tcgen05.mma per stage into one of two accumulators in tensor memory; commits
 //               release the stage, and hand over the accumulator, in both CTAs
-//   warps 2..9  epilogue of the other accumulator meanwhile: a warp takes 32 rows and 128 columns
+//   warps 2..9  epilogue of the other accumulator meanwhile: a warp takes 32 rows and 128 columns (of the statistics it adds
+//               a wide contraction's parts first, kPartChannels)
 // All three operand layouts are read where they lie: x and W are K-major in z = x W^T; W in g W, and both g and x in g^T x,
 // are MN-major (the contraction index numbers the rows of the matrix in memory).  The number of rows that take part is known
 // on the device only (labels may be missing), so the kernels read it there.
@@ -49,6 +50,9 @@ struct Ring {
   static constexpr uint32_t kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;  // + slack to align the tiles
 };
 constexpr uint32_t kTmemCols = 2 * kTile;
+constexpr int kPartBlocks = kPartChannels / kBK;
+// of a logit's contraction, an accumulator each
+__device__ __forceinline__ int parts_of(int blocks) { return (blocks + kPartBlocks - 1) / kPartBlocks; }
 
 // One launch makes the statistics; another both gradients, whose units follow one another (the long ones of dx first).
 struct Params {
@@ -276,35 +280,39 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
       for (int unit = pair; unit < work.units && ok; unit += pairs) {
         const Unit u = work.at(unit);
         if (u.kb_begin == u.kb_end) continue;  // nothing to contract: the epilogue writes zeros
-        const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
-        ++t;
-        if (!wait(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
-        umma::fence_after_sync();
-        const uint32_t d_tmem = tmem + acc * kTile;
         const bool a_mn = kGrads && u.of_weight;
         const uint32_t idesc = umma2::idesc_bf16(kHalf * kCtas, u.width, a_mn, kGrads);
         const uint64_t a_desc = a_mn ? umma2::desc_mn_major(tiles_base) : umma2::desc_k_major(tiles_base);
         const uint32_t a_step = (a_mn ? 2048 : 32) >> 4;
-        for (int kb = u.kb_begin; kb < u.kb_end; ++kb, ++it) {
-          const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
-          if (!wait(&full_bar[s], ph)) { ok = false; break; }
+        const int blocks = u.kb_end - u.kb_begin, parts = kGrads ? 1 : parts_of(blocks);
+        for (int part = 0; part < parts && ok; ++part) {
+          const int begin = u.kb_begin + blocks * part / parts, end = u.kb_begin + blocks * (part + 1) / parts;
+          const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
+          ++t;
+          if (!wait(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
           umma::fence_after_sync();
-          const uint64_t a = a_desc + s * (kStageBytes >> 4), b = b_desc + s * (kStageBytes >> 4);
-          if (umma2::elect_one()) {
+          const uint32_t d_tmem = tmem + acc * kTile;
+          for (int kb = begin; kb < end; ++kb, ++it) {
+            const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
+            if (!wait(&full_bar[s], ph)) { ok = false; break; }
+            umma::fence_after_sync();
+            const uint64_t a = a_desc + s * (kStageBytes >> 4), b = b_desc + s * (kStageBytes >> 4);
+            if (umma2::elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kBK / 16; ++ks) {
-              const uint32_t add = (kb > u.kb_begin || ks > 0) ? 1u : 0u;
-              if (kPair)
-                umma2::mma_bf16(d_tmem, a + ks * a_step, b + ks * kBStep, idesc, add);
-              else
-                umma2::mma_bf16_alone(d_tmem, a + ks * a_step, b + ks * kBStep, idesc, add);
+              for (int ks = 0; ks < kBK / 16; ++ks) {
+                const uint32_t add = (kb > begin || ks > 0) ? 1u : 0u;
+                if (kPair)
+                  umma2::mma_bf16(d_tmem, a + ks * a_step, b + ks * kBStep, idesc, add);
+                else
+                  umma2::mma_bf16_alone(d_tmem, a + ks * a_step, b + ks * kBStep, idesc, add);
+              }
+              commit(&empty_bar[s]);
             }
-            commit(&empty_bar[s]);
+            __syncwarp();
           }
+          if (ok && umma2::elect_one()) commit(&acc_full[acc]);
           __syncwarp();
         }
-        if (ok && umma2::elect_one()) commit(&acc_full[acc]);
-        __syncwarp();
       }
     }
   } else {
@@ -317,20 +325,24 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
     for (int unit = pair; unit < work.units; unit += pairs) {
       const Unit u = work.at(unit);
       const bool empty = u.kb_begin == u.kb_end;
-      const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
-      if (!empty) ++t;
+      uint32_t acc = 0;
       const int m = u.m0 + row_in_tile, n = u.n0 + column0;
       const int m_end = u.of_weight ? prm.vocab : rows_here;
       int main = -1;  // statistics: where the row's label lies in this warp's columns
       if (!kGrads && m < m_end) main = prm.main_column[prm.rows.piece_begin + m] - n;
-      // Warp-uniform outcome: the tensor-memory loads below need the whole warp.  Once a wait has run out, this unit and all
-      // later ones read as NaN.
-      if (ok && !empty && !wait(&acc_full[acc], aph)) ok = false;
-      umma::fence_after_sync();
-      const uint32_t source = source0 + acc * kTile;
-      // the accumulator goes back to the issuer as soon as its last columns are in registers
+      // The next accumulator.  Warp-uniform outcome: the tensor-memory loads below need the whole warp.  Once a wait has run
+      // out, this unit and all later ones read as NaN.
+      const auto take = [&] {
+        acc = t & 1u;
+        const uint32_t aph = (t >> 1) & 1u;
+        ++t;
+        if (ok && !wait(&acc_full[acc], aph)) ok = false;
+        umma::fence_after_sync();
+        return source0 + acc * kTile;
+      };
+      // it goes back to the issuer as soon as its last columns are in registers
       const auto release = [&] {
-        if (ok && !empty) {
+        if (ok) {
           umma::fence_before_sync();
           __syncwarp();
           if (lane == 0)
@@ -339,16 +351,38 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
       };
       if (!kGrads) {
         float z[kStatsTile];
-        if (ok && !empty) {
-          uint32_t(&v)[kStatsTile / 32][32] = reinterpret_cast<uint32_t(&)[kStatsTile / 32][32]>(z);
+        {
+          const uint32_t source = take();  // a logit has channels: there is a first part
+          if (ok) {
+            uint32_t(&v)[kStatsTile / 32][32] = reinterpret_cast<uint32_t(&)[kStatsTile / 32][32]>(z);
 #pragma unroll
-          for (int i = 0; i < kStatsTile / 32; ++i) umma::tmem_ld32(source + 32 * i, v[i]);
-          umma::tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int j = 0; j < kStatsTile; ++j) z[j] = ok ? 0.f : quiet_nan();
+            for (int i = 0; i < kStatsTile / 32; ++i) umma::tmem_ld32(source + 32 * i, v[i]);
+            umma::tmem_ld_wait();
+          }
+          release();
         }
-        release();
+#pragma unroll 1
+        for (int part = parts_of(u.kb_end - u.kb_begin); part > 1; --part) {
+          const uint32_t source = take();
+          if (ok) {
+#pragma unroll
+            for (int i = 0; i < kStatsTile / 16; ++i) {
+              uint32_t v[16];
+              umma::tmem_ld16(source + 16 * i, v);
+              umma::tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                asm volatile("" : "+r"(v[j]));  // there after the wait only
+                z[16 * i + j] += __uint_as_float(v[j]);
+              }
+            }
+          }
+          release();
+        }
+        if (!ok) {
+#pragma unroll
+          for (int j = 0; j < kStatsTile; ++j) z[j] = quiet_nan();
+        }
         const int valid = prm.vocab - n;  // columns inside the vocabulary, possibly none or more than there are here
         if (valid > 0) {
           if (valid < kStatsTile) {
@@ -385,6 +419,7 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
         const bool inside = m < m_end;
         const int row = !u.of_weight && inside && partials == nullptr ? prm.rows.row_map[prm.rows.piece_begin + m] : m;
         const bool wide = (prm.channels & 15) == 0 && (reinterpret_cast<uintptr_t>(prm.grad_x) & 31u) == 0;
+        const uint32_t source = empty ? 0u : take();
 #pragma unroll 1
         for (int c0 = 0; c0 < kStatsTile; c0 += 64) {
           float z[64];
@@ -397,7 +432,7 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
 #pragma unroll
             for (int j = 0; j < 64; ++j) z[j] = ok ? 0.f : quiet_nan();
           }
-          if (c0 == 64) release();
+          if (c0 == 64 && !empty) release();
           if (partials != nullptr) {
             if (!inside) continue;
             float* dst = partials + (slot + m) * prm.channels + n + c0;

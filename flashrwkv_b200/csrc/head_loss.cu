@@ -42,12 +42,6 @@ using IO = Io16<bf16>;
 constexpr long long kPieceBytes = 1ll << 30;   // exponentials of one piece
 constexpr long long kStatsBytes = 1ll << 28;   // statistics of one piece
 constexpr int kMaxTop = 512;
-// The tensor core truncates where it adds an instruction's 16 products to its fp32 accumulator, so logits come out small, by a
-// share that grows with the number of additions: 2.8e-7, 1.04e-6, 2.13e-6 and 4.2e-6 of the logit at 256, 1024, 2048 and
-// 4096 channels (65536 logits each against 64 bits, for |z| from 6 to 32; smaller ones lose a little less), which is
-// 1.03e-9 per channel.  Left alone it moved the mean loss of 8192 x 65536 x 2048 by 5e-6 of itself.  The scale that turns
-// logits into exponents makes the mean good; what remains of a logit's error is random, 3e-7.
-constexpr double kTruncation = 1.03e-9;
 constexpr int kFinishThreads = 256;
 constexpr int kFewRows = 64;  // copied by the plan: a launch less (2 us) while a warp has two rows at most
 
@@ -791,7 +785,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     if (int rc = check_launch("compact_kernel")) return rc;
   }
 
-  const float log2_scale = (float)(1.4426950408889634 * (1.0 + kTruncation * a.channels) * labels.inv_temperature);
+  const float log2_scale = (float)(1.4426950408889634 * labels.inv_temperature);
   const size_t finish_smem = (size_t)(tiles + 2 * a.top) * sizeof(float);
   for (int piece = 0; piece < l.pieces; ++piece) {
     const Rows here{count, row_map, rows, compact.always, l.ldx, piece * l.piece_rows, l.piece_rows};

@@ -9,6 +9,15 @@ namespace head {
 
 constexpr int kTile = 256;       // rows and columns of an output tile
 constexpr int kStatsTile = 128;  // vocabulary columns of one maximum and sum of exponentials
+// The tensor core truncates where it adds an instruction's 16 products to its fp32 accumulator, so a logit loses a share of its
+// running sum with every addition: with all channels in one accumulator 1.0e-6, 2.2e-6, 4.3e-6 and 6.9e-5 of itself at 1024,
+// 2048, 4096 and 65536 channels of random rows, 1.1e-5, 2.2e-5, 4.5e-5 and 7.2e-4 where the large products come first, nothing
+// where the sums are exact.  So the contraction is cut into parts of equal length, of at most so many channels, that the
+// epilogue adds in registers, rounding to nearest: the 1024 channels' share is the most that any width loses, and the mean
+// loss of 2048 x 65536 x 1024 to 4096 is off by 6e-7 of itself (with parts of 512 3e-7).  A part costs the epilogue one more
+// read of the accumulator: statistics of 4096 x 65536 x 640 take 250 us with one part and 300 with two, of 2048 x 65536 x 2048
+// 350 us with one, 355 with two, 390 with four.
+constexpr int kPartChannels = 1024;
 
 // The rows that take part are numbered 0..count-1 ("compact rows"); the first *count entries of row_map are their numbers
 // in x.  A product works on a piece of them: compact rows piece_begin .. piece_begin + piece_rows - 1, cut at *count.

@@ -724,3 +724,62 @@ def test_the_scalar_loss_of_many_like_rows(N, teacher):
     bound = (U + N * 2.0 ** -52) * total
     assert abs(float(call("sum")) - total) <= bound
     assert abs(float(call("mean")) - total / N) <= bound / N
+
+
+def _growing_row(kind, N, C, gen):
+    """Rows x [N,C] and a vector w [C] whose dot products lie between 12 and 31 and gather their magnitude in one way each."""
+    def uniform(*shape, low=0.1, high=1.1):
+        return low + (high - low) * torch.rand(*shape, generator=gen)
+
+    w = uniform(C, low=0.5, high=1.5)
+    if kind == "exact":  # whole numbers times one power of two: every sum of fewer than 2^24 units is exact
+        x = torch.randint(1, 128, (N, C), generator=gen).float()
+        return (x * 2.0 ** -int(torch.log2(x.sum(1).max() / 30).ceil())).to(torch.bfloat16), torch.ones(C, dtype=torch.bfloat16)
+    if kind == "even":
+        x = uniform(N, C)
+    elif kind == "sparse":
+        x = torch.zeros(N, C)
+        x.scatter_(1, torch.stack([torch.randperm(C, generator=gen)[:5] for _ in range(N)]), uniform(N, 5))
+    elif kind == "random":
+        w = torch.randn(C, generator=gen) * 2 / C ** 0.5
+        x = torch.randn(N, C, generator=gen) + 6 * w
+    else:
+        x = 1e-4 * uniform(N, C)
+        x[:, slice(0, 16) if kind == "first" else slice(C - 16, C)] = uniform(N, 16)
+    x = x * (22 / (x @ w)[:, None])
+    return x.to(torch.bfloat16), w.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("N", [100, 300])
+@pytest.mark.parametrize("kind", ["exact", "even", "first", "last", "sparse", "random"])
+@pytest.mark.parametrize("C", [128, 1024, 1032, 2056, 4096, 16384, 65536])
+def test_a_logit_however_its_sum_grows(C, kind, N):
+    """The label's logit is 0 and the only other one z, so a row's loss is log(1 + e^z).  An accumulator takes 1024 channels at
+    most; it loses up to one unit (2 u of the sum of magnitudes so far, B at the end) per product, and its parts are added with
+    a rounding of u B each.  Scaling to powers of two, back to natural units and the last addition are six roundings, of the
+    numbers that they are done with included: 6 u z, which is all that a sum without roundings may be off by."""
+    import flashrwkv_b200 as F
+
+    x, w = _growing_row(kind, N, C, torch.Generator().manual_seed(C))
+    x, w = x.cuda(), torch.stack((torch.zeros_like(w), w)).cuda()
+    z, B = x.double() @ w[1].double(), x.double().abs() @ w[1].double().abs()
+    assert 12 < float(z.min()) and float(z.max()) < 31
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, torch.zeros(N, dtype=torch.int64, device="cuda"), reduction="none")
+    parts = -(-C // 1024)
+    sums = 0 if kind == "exact" else (2 * min(C, 1024 + 64) + parts) * U * B
+    _near(loss, torch.nn.functional.softplus(z, threshold=100), sums + 6 * U * z, "row losses")
+
+
+@pytest.mark.parametrize("N,C,V", [(300, 2056, 2100), (140, 4104, 700), (20, 4104, 3001), (128, 8200, 300)])
+def test_logits_of_several_parts(N, C, V):
+    """Odd and even numbers of accumulators to a logit, tiles that follow one another in each, with the gradients behind them."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(N, C, V, N + C + V)
+    t[::5] = -100
+    used = t != -100
+    x.requires_grad_(), w.requires_grad_()
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="sum")
+    r = _reference(x.detach(), w.detach(), t[:, None], used.double()[:, None], 1.0, torch.ones(N, device="cuda"))
+    assert abs(float(loss.detach()) - float(r["loss"].sum())) <= float(r["eloss"].sum()) + U * float(r["loss"].sum())
+    _check_grads(*torch.autograd.grad(loss, (x, w)), r)
