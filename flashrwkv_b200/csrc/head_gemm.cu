@@ -50,9 +50,12 @@ struct Ring {
   static constexpr uint32_t kSmem = kStages * kStageBytes + kEpilogueWarps * kBoxBytes + 1024;  // + slack to align the tiles
 };
 constexpr uint32_t kTmemCols = 2 * kTile;
-constexpr int kPartBlocks = kPartChannels / kBK;
-// of a logit's contraction, an accumulator each
-__device__ __forceinline__ int parts_of(int blocks) { return (blocks + kPartBlocks - 1) / kPartBlocks; }
+// the parts of a unit's contraction that take an accumulator each
+template <bool kGrads>
+__device__ __forceinline__ int parts_of(int blocks) {
+  constexpr int kMost = (kGrads ? kGradPart : kPartChannels) / kBK;
+  return (blocks + kMost - 1) / kMost;
+}
 
 // One launch makes the statistics; another both gradients, whose units follow one another (the long ones of dx first).
 struct Params {
@@ -284,9 +287,10 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
         const uint32_t idesc = umma2::idesc_bf16(kHalf * kCtas, u.width, a_mn, kGrads);
         const uint64_t a_desc = a_mn ? umma2::desc_mn_major(tiles_base) : umma2::desc_k_major(tiles_base);
         const uint32_t a_step = (a_mn ? 2048 : 32) >> 4;
-        const int blocks = u.kb_end - u.kb_begin, parts = kGrads ? 1 : parts_of(blocks);
+        const int blocks = u.kb_end - u.kb_begin, parts = parts_of<kGrads>(blocks);
         for (int part = 0; part < parts && ok; ++part) {
-          const int begin = u.kb_begin + blocks * part / parts, end = u.kb_begin + blocks * (part + 1) / parts;
+          const int begin = u.kb_begin + blocks * part / parts;
+          const int end = u.kb_begin + blocks * (part + 1) / parts;
           const uint32_t acc = t & 1u, aph = (t >> 1) & 1u;
           ++t;
           if (!wait(&acc_empty[acc], aph ^ 1u)) { ok = false; break; }
@@ -349,40 +353,35 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
             umma2::arrive_cluster(kPair ? umma2::in_leader(&acc_empty[acc]) : umma::smem_u32(&acc_empty[acc]));
         }
       };
-      if (!kGrads) {
-        float z[kStatsTile];
-        {
-          const uint32_t source = take();  // a logit has channels: there is a first part
-          if (ok) {
-            uint32_t(&v)[kStatsTile / 32][32] = reinterpret_cast<uint32_t(&)[kStatsTile / 32][32]>(z);
+      float z[kStatsTile];
+      for (int part = 0, parts = parts_of<kGrads>(u.kb_end - u.kb_begin); part < parts; ++part) {
+        const uint32_t source = take();
+        if (!ok) break;
+        if (part == 0) {
+          uint32_t(&v)[kStatsTile / 32][32] = reinterpret_cast<uint32_t(&)[kStatsTile / 32][32]>(z);
 #pragma unroll
-            for (int i = 0; i < kStatsTile / 32; ++i) umma::tmem_ld32(source + 32 * i, v[i]);
+          for (int i = 0; i < kStatsTile / 32; ++i) umma::tmem_ld32(source + 32 * i, v[i]);
+          umma::tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < kStatsTile / 16; ++i) {
+            uint32_t v[16];
+            umma::tmem_ld16(source + 16 * i, v);
             umma::tmem_ld_wait();
-          }
-          release();
-        }
-#pragma unroll 1
-        for (int part = parts_of(u.kb_end - u.kb_begin); part > 1; --part) {
-          const uint32_t source = take();
-          if (ok) {
 #pragma unroll
-            for (int i = 0; i < kStatsTile / 16; ++i) {
-              uint32_t v[16];
-              umma::tmem_ld16(source + 16 * i, v);
-              umma::tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                asm volatile("" : "+r"(v[j]));  // there after the wait only
-                z[16 * i + j] += __uint_as_float(v[j]);
-              }
+            for (int j = 0; j < 16; ++j) {
+              asm volatile("" : "+r"(v[j]));  // there after the wait only
+              z[16 * i + j] += __uint_as_float(v[j]);
             }
           }
-          release();
         }
-        if (!ok) {
+        release();
+      }
+      if (empty || !ok) {
 #pragma unroll
-          for (int j = 0; j < kStatsTile; ++j) z[j] = quiet_nan();
-        }
+        for (int j = 0; j < kStatsTile; ++j) z[j] = ok ? 0.f : quiet_nan();
+      }
+      if (!kGrads) {
         const int valid = prm.vocab - n;  // columns inside the vocabulary, possibly none or more than there are here
         if (valid > 0) {
           if (valid < kStatsTile) {
@@ -419,20 +418,9 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
         const bool inside = m < m_end;
         const int row = !u.of_weight && inside && partials == nullptr ? prm.rows.row_map[prm.rows.piece_begin + m] : m;
         const bool wide = (prm.channels & 15) == 0 && (reinterpret_cast<uintptr_t>(prm.grad_x) & 31u) == 0;
-        const uint32_t source = empty ? 0u : take();
-#pragma unroll 1
-        for (int c0 = 0; c0 < kStatsTile; c0 += 64) {
-          float z[64];
-          if (ok && !empty) {
-            uint32_t(&v)[2][32] = reinterpret_cast<uint32_t(&)[2][32]>(z);
-            umma::tmem_ld32(source + c0, v[0]);
-            umma::tmem_ld32(source + c0 + 32, v[1]);
-            umma::tmem_ld_wait();
-          } else {
 #pragma unroll
-            for (int j = 0; j < 64; ++j) z[j] = ok ? 0.f : quiet_nan();
-          }
-          if (c0 == 64 && !empty) release();
+        for (int c0 = 0; c0 < kStatsTile; c0 += 64) {
+          float* const y = z + c0;
           if (partials != nullptr) {
             if (!inside) continue;
             float* dst = partials + (slot + m) * prm.channels + n + c0;
@@ -441,24 +429,24 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
               if (n + c0 + h < prm.channels) {  // channels are a multiple of 8
                 if (u.of_weight && prm.add) {
                   const float4 a = *reinterpret_cast<const float4*>(dst + h), b = *reinterpret_cast<const float4*>(dst + h + 4);
-                  z[h] += a.x; z[h + 1] += a.y; z[h + 2] += a.z; z[h + 3] += a.w;
-                  z[h + 4] += b.x; z[h + 5] += b.y; z[h + 6] += b.z; z[h + 7] += b.w;
+                  y[h] += a.x; y[h + 1] += a.y; y[h + 2] += a.z; y[h + 3] += a.w;
+                  y[h + 4] += b.x; y[h + 5] += b.y; y[h + 6] += b.z; y[h + 7] += b.w;
                 }
                 uint32_t o[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(z[h + j]);
+                for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(y[h + j]);
                 store32(dst + h, o, true);
               }
             }
           } else if (u.of_weight) {
-            if (n + c0 < prm.channels && m - lane < m_end) store_box<bf16>(&prm.map_out, n + c0, m - lane, box, z, lane);
+            if (n + c0 < prm.channels && m - lane < m_end) store_box<bf16>(&prm.map_out, n + c0, m - lane, box, y, lane);
           } else if (inside) {
             bf16* dst = prm.grad_x + (long long)row * prm.channels + n + c0;
 #pragma unroll
             for (int h = 0; h < 64; h += 16) {
               uint32_t o[8];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) o[j] = IO::pack(z[h + 2 * j], z[h + 2 * j + 1]);
+              for (int j = 0; j < 8; ++j) o[j] = IO::pack(y[h + 2 * j], y[h + 2 * j + 1]);
               const int room = prm.channels - (n + c0 + h);
               if (room >= 16) {
                 store32(dst + h, o, wide);

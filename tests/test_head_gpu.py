@@ -783,3 +783,43 @@ def test_logits_of_several_parts(N, C, V):
     r = _reference(x.detach(), w.detach(), t[:, None], used.double()[:, None], 1.0, torch.ones(N, device="cuda"))
     assert abs(float(loss.detach()) - float(r["loss"].sum())) <= float(r["eloss"].sum()) + U * float(r["loss"].sum())
     _check_grads(*torch.autograd.grad(loss, (x, w)), r)
+
+
+@pytest.mark.parametrize("N,C,V", [(9472, 512, 20011), (100, 37888, 8200)])
+def test_gradients_of_several_parts(N, C, V):
+    """As many tiles of dx as run at once, so that a tile's contraction over the vocabulary is not cut between pairs (or single
+    CTAs) and takes several accumulators; 9472 rows are several of dW's as well."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(N, C, V, N + C + V)
+    t[::5] = -100
+    t[5 * N // 6:] = t.clamp_min(0)[5 * N // 6:]
+    used = t != -100
+    x.requires_grad_(), w.requires_grad_()
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="sum")
+    got = torch.autograd.grad(loss, (x, w))
+    r = _reference(x.detach(), w.detach(), t[:, None], used.double()[:, None], 1.0, torch.ones(N, device="cuda"))
+    assert abs(float(loss.detach()) - float(r["loss"].sum())) <= float(r["eloss"].sum()) + U * float(r["loss"].sum())
+    _check_grads(*got, r)
+
+
+def test_a_weight_gradient_of_many_rows_whose_large_terms_come_first():
+    """A label whose logit lies 40 below the others has the logit gradient -up exactly, here a power of two: dW[label] is a sum
+    of exact products, of one sign.  An accumulator takes 4096 of them at most and loses up to one unit (2 u of the sum) per
+    product, the 32 parts are added with u each.  The roundings of the results to bf16 are independent: in the mean over 9472
+    columns they stay below five deviations, 5 rho / sqrt(3 * 9472)."""
+    import flashrwkv_b200 as F
+
+    N, C, V = 131072, 9472, 512  # 2 x 37 tiles: none of them is cut between pairs
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = (0.5 + torch.rand(N, C, generator=gen, device="cuda", dtype=torch.float32)).to(torch.bfloat16)
+    w = torch.zeros(V, C, device="cuda", dtype=torch.bfloat16)
+    w[0] = -(2.0 ** -8)
+    w.requires_grad_()
+    up = torch.full((N,), 2.0 ** -14, device="cuda")
+    up[:64] = 1.0
+    rows = F.pretrain_head_cross_entropy_bf16(x, w, torch.zeros(N, dtype=torch.int32, device="cuda"), reduction="none")
+    got = torch.autograd.grad(rows, w, up)[0][0].double()
+    want = -sum(u.double() @ p.double() for u, p in zip(up.split(8192), x.split(8192)))
+    off = float(((got - want) / want).mean())
+    assert abs(off) <= 2 * 4096 * U + 32 * U + 5 * RHO / (3 * C) ** 0.5, off
