@@ -491,10 +491,12 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     if (tid == 0) share[0] = 1.f;
     loss = row.excess;
   } else {
-    const float most = a.labels.teacher[entry + main] * a.labels.inv_temperature;
+    // the difference before the temperature: it is as good as the logits are, wherever they lie, and of two that are the type's
+    // lowest value it is 0
+    const float most = a.labels.teacher[entry + main];
     float rest = 0.f;  // of the exponentials, beside the highest entry's 1
     for (int k = tid; k < top; k += kFinishThreads) {
-      const float p = expf(a.labels.teacher[entry + k] * a.labels.inv_temperature - most);
+      const float p = expf((a.labels.teacher[entry + k] - most) * a.labels.inv_temperature);
       share[k] = p;
       if (k != main) rest += p;
     }
@@ -504,7 +506,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
     for (int k = tid; k < top; k += kFinishThreads) {
       const float p = share[k] / (1.f + rest);
       share[k] = p;
-      const float log_p = a.labels.teacher[entry + k] * a.labels.inv_temperature - most - log_total;
+      const float log_p = (a.labels.teacher[entry + k] - most) * a.labels.inv_temperature - log_total;
       if (!(p == 0.f)) part = fmaf(p, (log_p + row.excess) - (logit[k] - logit[main]), part);  // an absent entry has p = 0
     }
     loss = a.labels.temperature * a.labels.temperature * block_reduce(part, scratch, false);

@@ -823,3 +823,32 @@ def test_a_weight_gradient_of_many_rows_whose_large_terms_come_first():
     want = -sum(u.double() @ p.double() for u, p in zip(up.split(8192), x.split(8192)))
     off = float(((got - want) / want).mean())
     assert abs(off) <= 2 * 4096 * U + 32 * U + 5 * RHO / (3 * C) ** 0.5, off
+
+
+@pytest.mark.parametrize("T", [0.25, 0.7, 3.0])
+def test_teacher_logits_far_from_zero(T):
+    """A softmax knows no offset: with logits that are multiples of 2^-6 below 16 an offset of 2^14 is exact in fp32, so that
+    every result keeps its bits.  Entries of the type's lowest value are entries: beside others they have no share, and among
+    themselves equal ones."""
+    import flashrwkv_b200 as F
+
+    x, w, _, gen = _rows(40, 64, 300, 41)
+    logits, idx = _teacher(40, 9, 300, gen, missing=False)
+    logits = (logits.clamp(-15, 15) * 64).round() / 64
+    logits[3, 2:] = float("-inf")
+    x.requires_grad_(), w.requires_grad_()
+
+    def call(logits):
+        loss = F.pretrain_head_distill_bf16(x, w, logits, idx, temperature=T)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    want = call(logits)
+    for offset in (2.0 ** 14, -(2.0 ** 14)):
+        for a, b in zip(call(logits + offset), want):
+            assert torch.equal(a, b)
+    for lowest in (torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min):
+        low, gone = logits.clone(), logits.clone()
+        low[5, 1:], gone[5, 1:] = lowest, float("-inf")
+        low[7], gone[7] = lowest, 0.0
+        for a, b in zip(call(low), call(gone)):
+            assert torch.equal(a, b)
