@@ -45,10 +45,15 @@ constexpr int kMaxTop = 512;
 constexpr int kFinishThreads = 256;
 constexpr int kFewRows = 64;  // copied by the plan: a launch less (2 us) while a warp has two rows at most
 
-// Rows of labels that a warp each finishes rather than a CTA: a step of 8000 x 1000 x 512 takes 78 us so and 122 by CTAs, 4000 x
-// 4096 x 256 81 and 100, 3000 x 8000 x 768 138 and 146, but 100 x 8000 x 768 51 and 48, and 300 x 16000 x 256 80 and 54.
+// Rows of labels that a warp each finishes rather than a CTA.  A step of 256 channels, by warps / by CTAs in us:
+//   vocabulary  300: 29 / 33 at 70 rows, 37 / 43 at 1000, 43 / 66 at 4000      (40 rows, which CTAs share: 26 / 30)
+//              4090: 35 / 37 at 70 rows, 49 / 49 at 1000, 77 / 95 at 4000      (40 rows: 33 / 35)
+//              6000: 61 / 55 at 1100 rows, 74 / 74 at 2000, 93 / 108 at 4000
+//              8190: 72 / 64 at 1100 rows, 86 / 84 at 2000, 109 / 122 at 4000  (40 rows: 37 / 35)
+//             12000: 84 / 72 at 1100 rows, 104 / 98 at 2000, 156 / 164 at 4000
+// A teacher's row is a CTA's always: its entries are what it waits for, and eight warps gather them at once.
 constexpr bool short_rows(long long ldg, int rows) {
-  return rows > kFewRows && (ldg <= 4096 || (ldg <= 8192 && rows >= 1024));
+  return rows > kFewRows && (ldg <= 4096 || (ldg <= 8192 && rows >= 2048));
 }
 
 struct Labels {

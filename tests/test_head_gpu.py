@@ -852,3 +852,19 @@ def test_teacher_logits_far_from_zero(T):
         low[7], gone[7] = lowest, 0.0
         for a, b in zip(call(low), call(gone)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("N,C,V", [(2047, 64, 6000), (2048, 64, 6000), (65, 40, 4096), (65, 40, 4097), (64, 40, 4096)])
+def test_rows_finished_by_warps_and_by_ctas(N, C, V):
+    """Both sides of each edge of the rule that gives a row to a warp or to a CTA."""
+    import flashrwkv_b200 as F
+
+    x, w, t, _ = _rows(N, C, V, N + C + V)
+    t[::6] = -100
+    used = t != -100
+    x.requires_grad_(), w.requires_grad_()
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="sum")
+    got = torch.autograd.grad(loss, (x, w))
+    r = _reference(x.detach(), w.detach(), t[:, None], used.double()[:, None], 1.0, torch.ones(N, device="cuda"))
+    assert abs(float(loss.detach()) - float(r["loss"].sum())) <= float(r["eloss"].sum()) + U * float(r["loss"].sum())
+    _check_grads(*got, r)
