@@ -338,3 +338,25 @@ def test_a_backward_pass_captured_apart_from_its_forward_pass():
         for a, c in zip(held, want):
             assert torch.equal(a, c)
         del out
+
+
+@pytest.mark.parametrize("rows,C", [(9000, 136), (9000, 520), (9000, 1032), (9000, 2056), (4500, 8200), (593, 264), (149, 64)])
+def test_every_row_counts_once_in_the_parameter_gradients(rows, C):
+    """A row's upstream gradient is 1 in the column of its number, 0 elsewhere: the gradient of the bias is the number of rows
+    that share a column, a whole number below 256, exactly, and a row that is lost at a slab's edge, or counted twice, shows as
+    one.  The gradient of the weight is the sum of as many units of xhat, within the bounds above."""
+    import flashrwkv_b200 as F
+    from oracle import head_norm_oracle as O
+
+    i = _inputs(1, rows, C, rows + C)
+    w, b = i["weight"].requires_grad_(), i["bias"].requires_grad_()
+    g = torch.zeros(1, rows, C, dtype=torch.bfloat16, device="cuda")
+    at = torch.arange(rows, device="cuda")
+    g[0, at, at % C] = 1.0
+    dw, db = torch.autograd.grad(F.pretrain_tmix_layer_norm_bf16(i["x"], w, b, eps=EPS), (w, b), g)
+    count = torch.bincount(at % C, minlength=C)
+    assert int(count.max()) < 256 and torch.equal(db, count.to(torch.bfloat16))
+    _, want, _ = O.layer_norm_backward(g, i["x"], w.detach(), EPS)
+    A, rstd = _amplification(i["x"])
+    unit = (i["x"].double() - i["x"].double().mean(-1, keepdim=True)).abs() * rstd
+    _close(dw, want, (rows + 4) * U * (g.double() * unit).sum((0, 1)) + (128 * U * A * g.double()).sum((0, 1)), "d weight")
