@@ -75,6 +75,7 @@ struct Params {
   bf16* grad_weight;
   float* partials_x;
   float* partials_w;
+  GradFactor factor;
   bool add;                // to what partials_w holds
 };
 
@@ -326,6 +327,12 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
     const int row_in_tile = (int)rank * kHalf + 32 * (int)quarter + lane;
     const uint32_t box = tiles_base + kStages * kStageBytes + (warp - 2) * kBoxBytes;
     uint32_t t = 0;
+    float factor = 1.f;
+    if (kGrads) {
+      factor = prm.factor.temperature;
+      if (prm.factor.mean) factor /= (float)count;
+      if (prm.factor.scale != nullptr) factor *= *prm.factor.scale;
+    }
     for (int unit = pair; unit < work.units; unit += pairs) {
       const Unit u = work.at(unit);
       const bool empty = u.kb_begin == u.kb_end;
@@ -380,6 +387,9 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
       if (empty || !ok) {
 #pragma unroll
         for (int j = 0; j < kStatsTile; ++j) z[j] = ok ? 0.f : quiet_nan();
+      } else if (kGrads) {
+#pragma unroll
+        for (int j = 0; j < kStatsTile; ++j) z[j] *= factor;
       }
       if (!kGrads) {
         const int valid = prm.vocab - n;  // columns inside the vocabulary, possibly none or more than there are here
@@ -575,8 +585,8 @@ int launch_logit_stats(const void* x, const void* x_compact, const void* weight,
 }
 
 int launch_gradients(const void* g, long long ldg, const void* x, const void* x_compact, const void* weight, const Rows& rows,
-                     int channels, int vocab, const GradTarget& to_x, const GradTarget& to_weight, bool add, int* error_flag,
-                     cudaStream_t stream) {
+                     int channels, int vocab, const GradTarget& to_x, const GradTarget& to_weight, const GradFactor& factor,
+                     bool add, int* error_flag, cudaStream_t stream) {
   Params prm{};
   prm.rows = rows;
   prm.channels = channels;
@@ -587,6 +597,7 @@ int launch_gradients(const void* g, long long ldg, const void* x, const void* x_
   prm.grad_weight = static_cast<bf16*>(to_weight.grad);
   prm.partials_x = to_x.partials;
   prm.partials_w = to_weight.partials;
+  prm.factor = factor;
   prm.add = add;
   if (!make_map(&prm.map_a, g, rows.piece_rows, vocab, ldg, kHalf) ||
       !make_map(&prm.map_b, weight, vocab, channels, channels, kBK) ||

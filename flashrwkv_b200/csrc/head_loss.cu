@@ -5,13 +5,15 @@
 //   label t:                   loss_n = -log q_nt                                           (T = 1, one entry, p = 1)
 //   teacher entries (t_k, l_k): p = softmax(l / T) over the entries that are there (l > -inf),
 //                              loss_n = T^2 sum_k p_k (log p_k - log q_n,t_k)
-//   g_nv = scale_n T (q_nv - sum over k with t_k = v of p_k)      dx = g W,  dW = g^T x
+//   g_nv = row_n (q_nv - sum over k with t_k = v of p_k)          dx = f g W,  dW = f g^T x
+// row_n is the upstream gradient of a row's loss (1 where there is none), f what all rows share: T, the upstream gradient of
+// the scalar loss, and 1 / rows for a mean.
 //
 // A row that is nearly certain of its label has a loss and a label gradient that are differences of nearly equal numbers in
 // these forms (lse - z, q - 1).  They are taken from what is small instead: the label t (of a teacher: its highest entry)
 // stays out of the sums, O = log of the sum of exp z_v over the other v, d = O - z_t, and
 //   -log q_t = log(1 + e^d),   1 - q_t = e^d / (1 + e^d),   log q_k = z_k - z_t - log(1 + e^d),
-//   g_t = scale T (sum of the p_k of other columns - (1 - q_t)),
+//   g_t = row (sum of the p_k of other columns - (1 - q_t)),
 // so that both keep their relative precision down to the smallest losses.
 //
 // Passes over a piece of the rows (all of them while 2 rows x vocabulary bytes fit kPieceBytes):
@@ -22,7 +24,9 @@
 //            value would add 2^-9 to the one rounding that g needs as a tensor-core operand)
 //   finish   per row: O from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
 //            the exponentials times their tile's factor in place, now g in bf16; the labels' entries from fp32
-//   products dx and dW, in one launch
+//   products dx and dW, in one launch; f is applied to their fp32 sums.  Inside g it would be rounded with it, and the many
+//            labels with 1 - q_t near 1 would all be off by the rounding of 1 / rows, up to 2^-8 with one sign (dx and dW of
+//            777 x 50277 x 1544 by 2.6e-3 in the norm, 1.9e-3 now; their own rounding is 1.7e-3)
 // so a step costs three products of 2 rows x vocabulary x channels, not the four of recomputing z for the backward pass,
 // and the weight is read twice.  The price is that gradients are made with the loss, before the upstream gradient is known:
 // scale_kernel applies it afterwards (it leaves at once where the gradient is one).
@@ -325,7 +329,6 @@ struct FinishArgs {
   long long ldg;
   bool mean;
   const float* row_grads;    // upstream gradients of the row losses, or null
-  const float* grad_scale;   // upstream gradient of the loss, or null
   float* row_losses;
   float* loss;               // the last CTA of the last piece to arrive adds the row losses, in row order; or null
   int* arrived;
@@ -360,13 +363,9 @@ __device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count) {
   *a.loss = (float)(a.mean && count > 0 ? v / (double)count : v);  // no row takes part: 0
 }
 
-// what a row's logit gradients are scaled by, NaN with its loss
-__device__ __forceinline__ float grad_scale_of(const FinishArgs& a, long long n, int count, float loss) {
-  float scale = a.labels.temperature;
-  if (a.mean) scale /= (float)count;
-  if (a.row_grads != nullptr) scale *= a.row_grads[n];
-  if (a.grad_scale != nullptr) scale *= *a.grad_scale;
-  return loss != loss ? quiet_nan() : scale;
+// what a row's logit gradients are scaled by beside the factor that all rows share, NaN with its loss
+__device__ __forceinline__ float grad_scale_of(const FinishArgs& a, long long n, float loss) {
+  return loss != loss ? quiet_nan() : (a.row_grads != nullptr ? a.row_grads[n] : 1.f);
 }
 // eight fp16 exponentials to bf16 logit gradients
 __device__ __forceinline__ uint4 scaled(const uint4& e, float f) {
@@ -413,7 +412,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_by_warps_kernel(const F
     const float loss = inside ? row.excess : quiet_nan();
     if (lane == 0) a.row_losses[n] = loss;
     if (a.g != nullptr) {
-      const float scale = grad_scale_of(a, n, count, loss);
+      const float scale = grad_scale_of(a, n, loss);
       for (int begin = lane; begin < groups; begin += 128) {
         uint4 e[4];  // four pieces requested together
 #pragma unroll
@@ -521,7 +520,7 @@ __global__ __launch_bounds__(kFinishThreads) void finish_kernel(const FinishArgs
   arrive_and_sum(a, count);
   if (a.g == nullptr) return;
 
-  const float scale = grad_scale_of(a, n, count, loss);
+  const float scale = grad_scale_of(a, n, loss);
   __syncthreads();  // the tiles' factors and the shares
   for (int begin = from + tid; begin < to; begin += 4 * kFinishThreads) {
     uint4 e[4];  // four pieces requested together
@@ -793,6 +792,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   }
 
   const float log2_scale = (float)(1.4426950408889634 * labels.inv_temperature);
+  const GradFactor factor{labels.temperature, a.mean != 0, a.grad_scale};
   const size_t finish_smem = (size_t)(tiles + 2 * a.top) * sizeof(float);
   for (int piece = 0; piece < l.pieces; ++piece) {
     const Rows here{count, row_map, rows, compact.always, l.ldx, piece * l.piece_rows, l.piece_rows};
@@ -812,7 +812,6 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.ldg = l.ldg;
     f.mean = a.mean != 0;
     f.row_grads = a.row_grads;
-    f.grad_scale = a.grad_scale;
     f.row_losses = a.row_losses;
     f.loss = a.loss;
     f.arrived = &plan->arrived;
@@ -831,7 +830,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
       const GradTarget to_x{a.grad_x, partial_x, Splits{&plan->splits_x, l.splits_x}};
       const GradTarget to_weight{a.grad_weight, partial_w, Splits{&plan->splits_w, l.splits_w}};
       if (int rc = launch_gradients(power, l.ldg, a.x, ws + l.x_compact, a.weight, here, a.channels, a.vocab, to_x, to_weight,
-                                    piece > 0, a.error_flag, s))
+                                    factor, piece > 0, a.error_flag, s))
         return rc;
       if (a.grad_x != nullptr && l.parts_x)
         if (int rc = launch_sum_parts(partial_x, a.grad_x, row_map, plan, true, here.piece_begin, l.piece_rows, a.channels,

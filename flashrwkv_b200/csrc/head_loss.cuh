@@ -66,12 +66,19 @@ struct GradTarget {
   Splits splits;
 };
 
-// One launch for both gradients: grad_x[row_map[row]] = g[row] W, contraction over the vocabulary (its parts have the rows that
+// What the gradients of all rows share: temperature * (mean ? 1 / *count : 1) * (scale ? *scale : 1).
+struct GradFactor {
+  float temperature;
+  bool mean;
+  const float* scale;  // device
+};
+
+// One launch for both gradients, each times `factor`: grad_x[row_map[row]] = g[row] W, contraction over the vocabulary (its parts have the rows that
 // take part), and grad_weight = g^T x, contraction over the rows of the piece (its parts are added to what they hold where
 // `add`).  The units of dW fill what the last units of dx leave of the device.
 int launch_gradients(const void* g, long long ldg, const void* x, const void* x_compact, const void* weight, const Rows& rows,
-                     int channels, int vocab, const GradTarget& to_x, const GradTarget& to_weight, bool add, int* error_flag,
-                     cudaStream_t stream);
+                     int channels, int vocab, const GradTarget& to_x, const GradTarget& to_weight, const GradFactor& factor,
+                     bool add, int* error_flag, cudaStream_t stream);
 
 // Up to 128 rows one CTA works alone on a 128 x 256 tile: a pair's tile would be half empty, and the loads of W, which bound
 // the product then, would wait for twice the tensor-core time per byte (a step of 16 x 65536 x 1024 164 us by pairs, 152 alone; 128 x 65536 x 2048

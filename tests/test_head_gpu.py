@@ -831,6 +831,7 @@ def test_teacher_logits_far_from_zero(T):
     every result keeps its bits.  Entries of the type's lowest value are entries: beside others they have no share, and among
     themselves equal ones."""
     import flashrwkv_b200 as F
+    from oracle import head_norm_oracle as O
 
     x, w, _, gen = _rows(40, 64, 300, 41)
     logits, idx = _teacher(40, 9, 300, gen, missing=False)
@@ -846,12 +847,16 @@ def test_teacher_logits_far_from_zero(T):
     for offset in (2.0 ** 14, -(2.0 ** 14)):
         for a, b in zip(call(logits + offset), want):
             assert torch.equal(a, b)
+    # An entry without a share has its logit gradient from fp32, where the column of an absent one has it from an fp16
+    # exponential: 2^-11 between them may round to the other bf16 neighbour, so the gradients go by the oracle's bounds.
+    count = torch.full((40,), 1 / 40, device="cuda")
     for lowest in (torch.finfo(torch.float32).min, torch.finfo(torch.bfloat16).min):
         low, gone = logits.clone(), logits.clone()
         low[5, 1:], gone[5, 1:] = lowest, float("-inf")
         low[7], gone[7] = lowest, 0.0
-        for a, b in zip(call(low), call(gone)):
-            assert torch.equal(a, b)
+        loss, dx, dw = call(low)
+        assert torch.equal(loss, call(gone)[0])
+        _check_grads(dx, dw, _reference(x.detach(), w.detach(), idx, O.teacher_shares(low, T)[0], T, count))
 
 
 @pytest.mark.parametrize("N,C,V", [(2047, 64, 6000), (2048, 64, 6000), (65, 40, 4096), (65, 40, 4097), (64, 40, 4096)])
@@ -868,3 +873,31 @@ def test_rows_finished_by_warps_and_by_ctas(N, C, V):
     r = _reference(x.detach(), w.detach(), t[:, None], used.double()[:, None], 1.0, torch.ones(N, device="cuda"))
     assert abs(float(loss.detach()) - float(r["loss"].sum())) <= float(r["eloss"].sum()) + U * float(r["loss"].sum())
     _check_grads(*got, r)
+
+
+@pytest.mark.parametrize("teacher", [False, True])
+@pytest.mark.parametrize("N", [100, 255])
+def test_the_rounding_of_a_mean_is_no_error_that_rows_share(N, teacher):
+    """1 / 255 lies in the middle between two bf16 values: as a factor of the logit gradients it would put all of them off by
+    2^-8 with one sign.  Labels 40 below the other logits have the gradient -1 / N exactly; dW[label] sums N products, 2 N u
+    for any order, and its roundings to bf16 are independent: in the mean over 2048 columns five deviations, 5 rho /
+    sqrt(3 * 2048).  Factors and T are a few roundings of u."""
+    import flashrwkv_b200 as F
+
+    C, V, T = 2048, 300, 1.0 if not teacher else 1.7
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    x = (0.5 + torch.rand(N, C, generator=gen, device="cuda")).to(torch.bfloat16)
+    w = torch.zeros(V, C, device="cuda", dtype=torch.bfloat16)
+    w[7] = -(2.0 ** -5)
+    w.requires_grad_()
+    label = torch.full((N, 1), 7, device="cuda")
+    if teacher:
+        loss = F.pretrain_head_distill_bf16(x, w, torch.zeros(N, 1, device="cuda"), label, temperature=T)
+    else:
+        loss = F.pretrain_head_cross_entropy_bf16(x, w, label[:, 0])
+    for up in (1.0, 0.3):
+        again = torch.autograd.grad(loss, w, torch.tensor(up, device="cuda"), retain_graph=True)[0][7].double()
+        want = -x.double().sum(0) * T * float(torch.tensor(up)) / N
+        off = float(((again - want) / want).mean())
+        # the first pass scales gradients that are rounded already: a second rounding unless the scale is 1
+        assert abs(off) <= (2 * N + 8) * U + 5 * RHO / (3 * C) ** 0.5 * (1 if up == 1.0 else 2 ** 0.5), (up, off)
