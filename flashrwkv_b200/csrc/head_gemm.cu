@@ -332,6 +332,7 @@ __device__ __forceinline__ void head_gemm(const Params& prm, int* error_flag) {
       factor = prm.factor.temperature;
       if (prm.factor.mean) factor /= (float)count;
       if (prm.factor.scale != nullptr) factor *= *prm.factor.scale;
+      if (prm.factor.of_rows != nullptr) factor *= *prm.factor.of_rows;
     }
     for (int unit = pair; unit < work.units; unit += pairs) {
       const Unit u = work.at(unit);

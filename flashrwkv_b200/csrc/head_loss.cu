@@ -6,8 +6,8 @@
 //   teacher entries (t_k, l_k): p = softmax(l / T) over the entries that are there (l > -inf),
 //                              loss_n = T^2 sum_k p_k (log p_k - log q_n,t_k)
 //   g_nv = row_n (q_nv - sum over k with t_k = v of p_k)          dx = f g W,  dW = f g^T x
-// row_n is the upstream gradient of a row's loss (1 where there is none), f what all rows share: T, the upstream gradient of
-// the scalar loss, and 1 / rows for a mean.
+// row_n f is the upstream gradient of a row's loss; f is what all rows share: T, the upstream gradient of the scalar loss, 1 /
+// rows for a mean, and of row losses the largest upstream gradient, which row_n is a share of (1 where there are none).
 //
 // A row that is nearly certain of its label has a loss and a label gradient that are differences of nearly equal numbers in
 // these forms (lse - z, q - 1).  They are taken from what is small instead: the label t (of a teacher: its highest entry)
@@ -25,7 +25,7 @@
 //   finish   per row: O from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
 //            the exponentials times their tile's factor in place, now g in bf16; the labels' entries from fp32
 //   products dx and dW, in one launch; f is applied to their fp32 sums.  Inside g it would be rounded with it, and the many
-//            labels with 1 - q_t near 1 would all be off by the rounding of 1 / rows, up to 2^-8 with one sign (dx and dW of
+//            labels with 1 - q_t near 1 would all be off by the rounding of 1 / rows (or of a common row_n), up to 2^-8 with one sign (dx and dW of
 //            777 x 50277 x 1544 by 2.6e-3 in the norm, 1.9e-3 now; their own rounding is 1.7e-3)
 // so a step costs three products of 2 rows x vocabulary x channels, not the four of recomputing z for the backward pass,
 // and the weight is read twice.  The price is that gradients are made with the loss, before the upstream gradient is known:
@@ -33,6 +33,8 @@
 //
 // The reference fuses the same cross entropy at csrc/sm90/head/l2wrap_ce/pretrain_bf16_forward.cu:282-286 around library
 // products and kept logits; it has no distillation.
+
+#include <cfloat>
 
 #include "head_loss.cuh"
 
@@ -138,6 +140,7 @@ struct Plan {
   int count;     // rows that take part
   int arrived;   // CTAs that have written their losses
   int splits_x, splits_w;
+  float row_scale;  // the largest upstream gradient of a row loss by its magnitude, 1 where none is or all are 0
 };
 struct SplitSizes {
   int channels, vocab, most_x, most_w, pairs;
@@ -176,7 +179,8 @@ __device__ int choose_splits(int most, float rows, float columns, float k, float
 __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, const int* __restrict__ highest, int* position,
                                                     int* __restrict__ row_map, int* __restrict__ main_column,
                                                     Plan* __restrict__ plan, SplitSizes sizes, CompactArgs compact,
-                                                    int* __restrict__ error_flag, int rows) {
+                                                    const float* __restrict__ row_grads, int* __restrict__ error_flag,
+                                                    int rows) {
   chain_begin();
   constexpr int kEach = 8;  // consecutive rows of a thread; what is in use comes in row order through shared memory
   __shared__ int warp_sums[32];
@@ -184,6 +188,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, const int* __
   __shared__ int list[1024 * kEach];  // the rows in use of this round, so that they leave in whole lines
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int done = 0;
+  float row_scale = 0.f;
   for (int begin = 0; begin < rows; begin += 1024 * kEach) {
     long long label[kEach];  // requested together: past the end the last row again
 #pragma unroll
@@ -237,10 +242,21 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, const int* __
       const int row = list[i];
       const long long v = labels.teacher != nullptr ? labels.at((long long)row * labels.top + __ldg(highest + row)) : labels.at(row);
       row_map[done + i] = row;
+      if (row_grads != nullptr) {
+        const float g = fabsf(__ldg(row_grads + row));
+        if (g <= FLT_MAX) row_scale = fmaxf(row_scale, g);  // one that is not finite stays its row's own affair
+      }
       main_column[done + i] = v >= 0 && v < sizes.vocab ? (int)v : -1;
     }
     done += used_here;
     __syncthreads();
+  }
+  if (row_grads != nullptr) {
+    // magnitudes order as their bits do
+    const unsigned most = __reduce_max_sync(0xffffffffu, __float_as_uint(row_scale));
+    if (lane == 0) warp_sums[warp] = (int)most;
+    __syncthreads();
+    row_scale = __uint_as_float(__reduce_max_sync(0xffffffffu, (unsigned)warp_sums[lane]));
   }
   if (warp == 0) {
     int most_x = sizes.most_x, splits_x = most_x, splits_w = sizes.most_w;
@@ -251,7 +267,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(Labels labels, const int* __
       splits_w = choose_splits(sizes.most_w, (float)sizes.vocab, (float)sizes.channels, (float)done, (float)sizes.pairs, lane);
     }
     if (lane == 0) {
-      *plan = Plan{done, 0, splits_x, splits_w};
+      *plan = Plan{done, 0, splits_x, splits_w, row_scale > 0.f ? row_scale : 1.f};
       *error_flag = 0;
     }
   }
@@ -329,6 +345,7 @@ struct FinishArgs {
   long long ldg;
   bool mean;
   const float* row_grads;    // upstream gradients of the row losses, or null
+  const float* row_scale;    // what they are divided by in g
   float* row_losses;
   float* loss;               // the last CTA of the last piece to arrive adds the row losses, in row order; or null
   int* arrived;
@@ -365,7 +382,7 @@ __device__ __forceinline__ void arrive_and_sum(const FinishArgs& a, int count) {
 
 // what a row's logit gradients are scaled by beside the factor that all rows share, NaN with its loss
 __device__ __forceinline__ float grad_scale_of(const FinishArgs& a, long long n, float loss) {
-  return loss != loss ? quiet_nan() : (a.row_grads != nullptr ? a.row_grads[n] : 1.f);
+  return loss != loss ? quiet_nan() : (a.row_grads != nullptr ? a.row_grads[n] / *a.row_scale : 1.f);
 }
 // eight fp16 exponentials to bf16 logit gradients
 __device__ __forceinline__ uint4 scaled(const uint4& e, float f) {
@@ -784,7 +801,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   compact.pitch = (int)(l.ldx / 8);
   compact.always = l.ldx != a.channels;
   launch_chained(plan_kernel, dim3(1), dim3(1024), 0, s, labels, highest, position, row_map, main_column, plan,
-                 sizes, compact, a.error_flag, rows);
+                 sizes, compact, a.row_grads, a.error_flag, rows);
   if (int rc = check_launch("plan_kernel")) return rc;
   if (rows > kFewRows) {
     launch_chained(compact_kernel, by_warp, dim3(256), 0, s, compact, count);
@@ -792,7 +809,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
   }
 
   const float log2_scale = (float)(1.4426950408889634 * labels.inv_temperature);
-  const GradFactor factor{labels.temperature, a.mean != 0, a.grad_scale};
+  const GradFactor factor{labels.temperature, a.mean != 0, a.grad_scale, a.row_grads != nullptr ? &plan->row_scale : nullptr};
   const size_t finish_smem = (size_t)(tiles + 2 * a.top) * sizeof(float);
   for (int piece = 0; piece < l.pieces; ++piece) {
     const Rows here{count, row_map, rows, compact.always, l.ldx, piece * l.piece_rows, l.piece_rows};
@@ -812,6 +829,7 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     f.ldg = l.ldg;
     f.mean = a.mean != 0;
     f.row_grads = a.row_grads;
+    f.row_scale = &plan->row_scale;
     f.row_losses = a.row_losses;
     f.loss = a.loss;
     f.arrived = &plan->arrived;

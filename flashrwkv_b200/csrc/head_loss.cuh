@@ -66,11 +66,12 @@ struct GradTarget {
   Splits splits;
 };
 
-// What the gradients of all rows share: temperature * (mean ? 1 / *count : 1) * (scale ? *scale : 1).
+// What the gradients of all rows share: temperature * (mean ? 1 / *count : 1) * (scale ? *scale : 1) * (of_rows ? *of_rows : 1).
 struct GradFactor {
   float temperature;
   bool mean;
-  const float* scale;  // device
+  const float* scale;    // device
+  const float* of_rows;  // device
 };
 
 // One launch for both gradients, each times `factor`: grad_x[row_map[row]] = g[row] W, contraction over the vocabulary (its parts have the rows that

@@ -901,3 +901,57 @@ def test_the_rounding_of_a_mean_is_no_error_that_rows_share(N, teacher):
         off = float(((again - want) / want).mean())
         # the first pass scales gradients that are rounded already: a second rounding unless the scale is 1
         assert abs(off) <= (2 * N + 8) * U + 5 * RHO / (3 * C) ** 0.5 * (1 if up == 1.0 else 2 ** 0.5), (up, off)
+
+
+@pytest.mark.parametrize("N", [64, 255, 9001])
+def test_upstream_gradients_that_all_rows_share_are_no_shared_error(N):
+    """The mean of row losses taken outside: 1 / rows arrives as every row's upstream gradient.  Labels 40 below the other
+    logits, bounds as above; rows without a label do not count, whatever arrives there."""
+    import flashrwkv_b200 as F
+
+    C, V = 2048, 300
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    x = (0.5 + torch.rand(N, C, generator=gen, device="cuda")).to(torch.bfloat16)
+    w = torch.zeros(V, C, device="cuda", dtype=torch.bfloat16)
+    w[7] = -(2.0 ** -5)
+    w.requires_grad_()
+    t = torch.full((N,), 7, device="cuda")
+    t[3::9] = -100
+    used = t != -100
+    rows = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    for up in (1 / 255, -3e-30, 1.7e30):
+        ups = torch.where(used, torch.full((N,), up, device="cuda"), torch.full((N,), float("inf"), device="cuda"))
+        got = torch.autograd.grad(rows, w, ups, retain_graph=True)[0][7].double()
+        want = -x[used].double().sum(0) * float(ups[0])
+        off = float(((got - want) / want).mean())
+        assert abs(off) <= (2 * N + 8) * U + 5 * RHO / (3 * C) ** 0.5, (up, off)
+
+
+def test_upstream_gradients_that_are_not_finite_or_zero():
+    """They spoil their own rows and the weight's gradient; no other row's."""
+    import flashrwkv_b200 as F
+
+    x, w, t, gen = _rows(50, 64, 300, 50)
+    x.requires_grad_(), w.requires_grad_()
+    rows = F.pretrain_head_cross_entropy_bf16(x, w, t, reduction="none")
+    up = torch.rand(50, generator=gen).cuda()
+    want = torch.autograd.grad(rows, (x, w), up, retain_graph=True)
+    bad = up.clone()
+    bad[4], bad[9] = float("nan"), float("inf")
+    dx, dw = torch.autograd.grad(rows, (x, w), bad, retain_graph=True)
+    hit = torch.zeros(50, dtype=torch.bool, device="cuda")
+    hit[[4, 9]] = True
+    if float(up[hit].max()) < float(up[~hit].max()):  # the scale is another row's
+        assert torch.equal(dx[~hit], want[0][~hit])
+    assert torch.isfinite(dx[~hit]).all() and not torch.isfinite(dx[hit]).all() and not torch.isfinite(dw).any()
+    for zero in (torch.zeros(50, device="cuda"), -torch.zeros(50, device="cuda")):
+        for g in torch.autograd.grad(rows, (x, w), zero, retain_graph=True):
+            assert bool((g == 0).all())
+    one = torch.zeros(50, device="cuda")
+    one[11] = 2.0
+    dx, dw = torch.autograd.grad(rows, (x, w), one, retain_graph=True)
+    few = x.detach()[11:12].clone().requires_grad_()
+    fx, fw = torch.autograd.grad(F.pretrain_head_cross_entropy_bf16(few, w, t[11:12], reduction="none"), (few, w),
+                                 torch.tensor([2.0], device="cuda"))
+    assert float((dx[11].double() - fx[0].double()).norm()) <= RHO * float(fx.double().norm()) and bool((dx[:11] == 0).all())
+    assert float((dw.double() - fw.double()).norm()) <= RHO * float(fw.double().norm())
