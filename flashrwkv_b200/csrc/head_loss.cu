@@ -48,6 +48,12 @@ using IO = Io16<bf16>;
 constexpr long long kPieceBytes = 1ll << 30;   // exponentials of one piece
 constexpr long long kStatsBytes = 1ll << 28;   // statistics of one piece
 constexpr int kMaxTop = 512;
+// What truncation takes from the logits of random rows, per channel of an accumulator (2.8e-7 of the logit at 256 channels, 5.2e-7
+// at 512, 1.0e-6 at 1024): the scale that turns logits into exponents gives it back.  It lies between what exact sums lose,
+// nothing, and what rows lose whose large products come first, 1.1e-8 per channel, so it lowers the largest error and puts it
+// at 1.06e-6 of a logit where nothing was lost; an accumulator takes kPartChannels at most, whatever the width.  The mean loss
+// of 2048 x 65536 x 1024 to 4096 is off by 1e-7 of itself, without it by 6e-7.
+constexpr double kTruncation = 1.03e-9;
 constexpr int kFinishThreads = 256;
 constexpr int kFewRows = 64;  // copied by the plan: a launch less (2 us) while a warp has two rows at most
 
@@ -808,7 +814,8 @@ extern "C" int frwkv_pretrain_head_loss(const frwkv_head_loss_args* args, frwkv_
     if (int rc = check_launch("compact_kernel")) return rc;
   }
 
-  const float log2_scale = (float)(1.4426950408889634 * labels.inv_temperature);
+  const double lost = kTruncation * a.channels / parts_of_channels(a.channels);
+  const float log2_scale = (float)(1.4426950408889634 * (1.0 + lost) * labels.inv_temperature);
   const GradFactor factor{labels.temperature, a.mean != 0, a.grad_scale, a.row_grads != nullptr ? &plan->row_scale : nullptr};
   const size_t finish_smem = (size_t)(tiles + 2 * a.top) * sizeof(float);
   for (int piece = 0; piece < l.pieces; ++piece) {

@@ -13,11 +13,11 @@ constexpr int kStatsTile = 128;  // vocabulary columns of one maximum and sum of
 // running sum with every addition: with all channels in one accumulator 1.0e-6, 2.2e-6, 4.3e-6 and 6.9e-5 of itself at 1024,
 // 2048, 4096 and 65536 channels of random rows, 1.1e-5, 2.2e-5, 4.5e-5 and 7.2e-4 where the large products come first, nothing
 // where the sums are exact.  So the contraction is cut into parts of equal length, of at most so many channels, that the
-// epilogue adds in registers, rounding to nearest: the 1024 channels' share is the most that any width loses, and the mean
-// loss of 2048 x 65536 x 1024 to 4096 is off by 6e-7 of itself (with parts of 512 3e-7).  A part costs the epilogue one more
-// read of the accumulator: statistics of 4096 x 65536 x 640 take 250 us with one part and 300 with two, of 2048 x 65536 x 2048
-// 350 us with one, 355 with two, 390 with four.
+// epilogue adds in registers, rounding to nearest, and the loss grows no further than 1024 channels take it.  A part costs the
+// epilogue one more read of the accumulator: statistics of 4096 x 65536 x 640 take 250 us with one part and 300 with two, of
+// 2048 x 65536 x 2048 350 us with one, 355 with two, 390 with four.
 constexpr int kPartChannels = 1024;
+constexpr int parts_of_channels(int channels) { return (channels + kPartChannels - 1) / kPartChannels; }
 // The gradients' contractions, over the vocabulary or the rows, are cut the same way before a sum loses what shows beside its
 // rounding to bf16 (2^-8): 131072 rows that begin with the large ones were off by 1.6e-3 in one accumulator, by 8e-5 in parts.
 // The time is the same (8192 x 65536 x 2048 5.3 to 5.4 ms either way).

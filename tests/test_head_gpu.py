@@ -757,7 +757,8 @@ def test_a_logit_however_its_sum_grows(C, kind, N):
     """The label's logit is 0 and the only other one z, so a row's loss is log(1 + e^z).  An accumulator takes 1024 channels at
     most; it loses up to one unit (2 u of the sum of magnitudes so far, B at the end) per product, and its parts are added with
     a rounding of u B each.  Scaling to powers of two, back to natural units and the last addition are six roundings, of the
-    numbers that they are done with included: 6 u z, which is all that a sum without roundings may be off by."""
+    numbers that they are done with included: 6 u z.  The scale gives back what random rows lose, 1.03e-9 per channel of an
+    accumulator, to rows that lost nothing too: with the roundings that is all that an exact sum may be off by."""
     import flashrwkv_b200 as F
 
     x, w = _growing_row(kind, N, C, torch.Generator().manual_seed(C))
@@ -767,7 +768,28 @@ def test_a_logit_however_its_sum_grows(C, kind, N):
     loss = F.pretrain_head_cross_entropy_bf16(x, w, torch.zeros(N, dtype=torch.int64, device="cuda"), reduction="none")
     parts = -(-C // 1024)
     sums = 0 if kind == "exact" else (2 * min(C, 1024 + 64) + parts) * U * B
-    _near(loss, torch.nn.functional.softplus(z, threshold=100), sums + 6 * U * z, "row losses")
+    _near(loss, torch.nn.functional.softplus(z, threshold=100), sums + (6 * U + 1.03e-9 * C / parts) * z, "row losses")
+
+
+@pytest.mark.parametrize("C", [256, 1024, 2048, 4096, 8200])
+def test_logits_of_random_rows_carry_no_mean_error(C):
+    """As above, the label's logit 0 and the other's z, so that a row's loss is z + log(1 + e^-z).  An accumulator of P channels
+    that truncates each of its P / 16 additions loses up to one unit, 2^-23 of a sum that is half of the result on average: P /
+    16 * 2^-24 of the logit.  A tenth of that is allowed to the mean over 30000 logits; the scale itself is an fp32 number,
+    2^-24."""
+    import flashrwkv_b200 as F
+
+    gen = torch.Generator().manual_seed(C)
+    w = torch.randn(C, generator=gen) * 2 / C ** 0.5
+    x = (torch.randn(30000, C, generator=gen) + (4 + 4 * torch.rand(30000, 1, generator=gen)) * w).to(torch.bfloat16).cuda()
+    w = torch.stack((torch.zeros(C), w)).to(torch.bfloat16).cuda()
+    z = x.double() @ w[1].double()
+    loss = F.pretrain_head_cross_entropy_bf16(x, w, torch.zeros(30000, dtype=torch.int64, device="cuda"), reduction="none")
+    big = z > 8
+    assert int(big.sum()) > 25000
+    off = (loss.double() - torch.nn.functional.softplus(z, threshold=100)) / z
+    P = C / -(-C // 1024)
+    assert abs(float(off[big].mean())) <= 0.1 * P / 16 * 2.0 ** -24 + 2.0 ** -24
 
 
 @pytest.mark.parametrize("N,C,V", [(300, 2056, 2100), (140, 4104, 700), (20, 4104, 3001), (128, 8200, 300)])
