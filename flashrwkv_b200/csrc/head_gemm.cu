@@ -18,9 +18,10 @@
 // All three operand layouts are read where they lie: x and W are K-major in z = x W^T; W in g W, and both g and x in g^T x,
 // are MN-major (the contraction index numbers the rows of the matrix in memory).  The number of rows that take part is known
 // on the device only (labels may be missing), so the kernels read it there.
-// 4096 x 32768 x 2048 (0.55 TFLOP each), each alone: 346, 366 and 337 us, tensor pipe 92 to 97 % active at the 1.45 to 1.55 GHz that the
-// power cap leaves; the library's plain products of these shapes take 357, 355 and 346 us.  With few rows the loads of W
-// bound it: 16 x 65536 x 1024 in 33 us for the statistics and 66 for both gradients (134 MB read, twice, and 134 written).
+// 4096 x 32768 x 2048 (0.55 TFLOP each): statistics 346 us, both gradients 734 (370 and 339 where dx or dW alone is wanted),
+// tensor pipe 92 to 97 % active at the 1.45 to 1.55 GHz that the power cap leaves; the library's plain products of these
+// shapes take 357, 355 and 346 us.  With few rows the loads of W bound it: 16 x 65536 x 1024 in 33 to 37 us for the
+// statistics and 66 for both gradients (134 MB read, twice, and 134 written).
 // Every wait is bounded; a role whose wait runs out sets the error flag and leaves, the others run into their own limits,
 // outputs that could not be made are NaN.
 

@@ -1,5 +1,6 @@
 // The head's losses for training: the vocabulary projection, its softmax, a loss against labels or against a teacher's
-// highest logits, and the gradients of the rows and of the weight, without ever holding the logits.
+// highest logits, and the gradients of the rows and of the weight, without fp32 logits in memory: a piece of the rows at a time
+// holds one 16-bit value per logit, 1 GiB at most.
 //
 //   z_n = W x_n / T            q_n = softmax(z_n)
 //   label t:                   loss_n = -log q_nt                                           (T = 1, one entry, p = 1)
@@ -20,8 +21,8 @@
 //   plan     numbers the rows that have a label; rows without one take no part in any product (compact_kernel copies the
 //            others together, or does nothing where every row takes part), so what they hold, NaN included, reaches nothing
 //   stats    z on the tensor cores; the epilogue leaves, per 128 columns, each row's maximum and sum of exponentials, and for
-//            gradients the exponentials themselves in fp16, relative to that maximum (error 2^-12 of each, where a bf16
-//            value would add 2^-9 to the one rounding that g needs as a tensor-core operand)
+//            gradients the exponentials themselves in fp16, relative to that maximum (error 2^-11 of each, where a bf16
+//            value would add 2^-8 to the one rounding that g needs as a tensor-core operand)
 //   finish   per row: O from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
 //            the exponentials times their tile's factor in place, now g in bf16; the labels' entries from fp32
 //   products dx and dW, in one launch; f is applied to their fp32 sums.  Inside g it would be rounded with it, and the many

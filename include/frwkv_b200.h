@@ -601,7 +601,8 @@ int frwkv_pretrain_layer_norm_backward(const void* grad_out, const void* grad_su
 
 /*
  * The head's losses for training: z = x weight^T / temperature, softmax over the vocabulary, a loss per row and, where
- * wanted, the gradients of x and weight, without keeping the logits.
+ * wanted, the gradients of x and weight; one 16-bit value per logit of a piece of the rows is kept (1 GiB
+ * at most).
  *   teacher_logits NULL: labels [rows], loss_n = log sum exp z_n - z_n[label]; rows whose label is ignore_index take no part.
  *   teacher_logits fp32 [rows][top], labels [rows][top]: loss_n = temperature^2 KL(p || softmax(z_n)), p = the softmax of
  *   teacher_logits / temperature over the entries that are not -inf; rows without an entry take no part.
