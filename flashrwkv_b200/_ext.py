@@ -52,8 +52,8 @@ def device_error_flags() -> dict:
     """The device error words of the latest launches that use bounded waits, by stage name (a host read: this
     synchronises).  Non-zero = a tensor-core, copy or grid-barrier wait ran out in that stage and its outputs are NaN.
     Stages: `wkv7_chunk_forward`, `wkv7_chunk_backward`, `tmix_linear` (sticky, one word per device),
-    `pretrain_head_loss`, `tmix_decode_layer` (word 7 of its eight); the recurrent decode kernels report through the metadata status word
-    (bit 16) instead."""
+    `pretrain_head_loss`, `tmix_decode_layer` (word 7 of its eight); the recurrent decode kernels report through the
+    metadata status word (bit 16) instead.  A captured call writes its word when it is replayed: read it after a replay."""
     out = {}
     for stage, words in extension().last_error_flags().items():
         out[stage] = int(words[7].item()) if stage == "tmix_decode_layer" else int(words.flatten()[0].item())

@@ -26,8 +26,9 @@
 //   finish   per row: O from the tiles' statistics, the labels' logits as fp32 dot products of their own, the loss, and
 //            the exponentials times their tile's factor in place, now g in bf16; the labels' entries from fp32
 //   products dx and dW, in one launch; f is applied to their fp32 sums.  Inside g it would be rounded with it, and the many
-//            labels with 1 - q_t near 1 would all be off by the rounding of 1 / rows (or of a common row_n), up to 2^-8 with one sign (dx and dW of
-//            777 x 50277 x 1544 by 2.6e-3 in the norm, 1.9e-3 now; their own rounding is 1.7e-3)
+//            labels with 1 - q_t near 1 would all be off by the rounding of 1 / rows (or of a common row_n), up to 2^-8 with
+//            one sign: dx and dW of 777 x 50277 x 1544 by 2.6e-3 in the norm so, 1.9e-3 as it is (rounding the exact
+//            gradients gives 1.7e-3)
 // so a step costs three products of 2 rows x vocabulary x channels, not the four of recomputing z for the backward pass,
 // and the weight is read twice.  The price is that gradients are made with the loss, before the upstream gradient is known:
 // scale_kernel applies it afterwards (it leaves at once where the gradient is one).

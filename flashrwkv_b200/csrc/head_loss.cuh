@@ -74,9 +74,9 @@ struct GradFactor {
   const float* of_rows;  // device
 };
 
-// One launch for both gradients, each times `factor`: grad_x[row_map[row]] = g[row] W, contraction over the vocabulary (its parts have the rows that
-// take part), and grad_weight = g^T x, contraction over the rows of the piece (its parts are added to what they hold where
-// `add`).  The units of dW fill what the last units of dx leave of the device.
+// One launch for both gradients, each times `factor`: grad_x[row_map[row]] = g[row] W, contraction over the vocabulary (its
+// parts have the rows that take part), and grad_weight = g^T x, contraction over the rows of the piece (its parts are added to
+// what they hold where `add`).  The units of dW fill what the last units of dx leave of the device.
 int launch_gradients(const void* g, long long ldg, const void* x, const void* x_compact, const void* weight, const Rows& rows,
                      int channels, int vocab, const GradTarget& to_x, const GradTarget& to_weight, const GradFactor& factor,
                      bool add, int* error_flag, cudaStream_t stream);

@@ -2,11 +2,11 @@
 
 `x [...,C]` are the normalised rows behind the last block and `weight [V,C]` the head's weight, both bf16.  Logits are not
 kept in fp32: while a call runs, a workspace holds one 16-bit value for each logit of a piece of the rows, at most 1 GiB.
-The gradients of a scalar loss are made together with it, in the forward call, and only for the
-inputs that require one; the upstream gradient scales them when the backward pass runs, which costs a pass over them and a
-second rounding to bf16 unless it is 1 (powers of two round nothing).  A backward pass repeated over a retained graph, or
-captured apart from its forward pass, makes them again, at the price of a whole step.  The gradients of row losses are made
-in the backward pass, which repeats the forward's product.  The backward passes are not differentiable themselves.
+The gradients of a scalar loss are made together with it, in the forward call, and only for the inputs that require one; the
+upstream gradient scales them when the backward pass runs, which costs a pass over them and a second rounding to bf16 unless
+it is 1 (powers of two round nothing).  A backward pass repeated over a retained graph, or captured apart from its forward
+pass, makes them again, at the price of a whole step.  The gradients of row losses are made in the backward pass, which
+repeats the forward's product.  The backward passes are not differentiable themselves.
 
 The reference fuses its cross entropy with an L2 penalty of the largest logit (`csrc/sm90/head/l2wrap_ce`), which is not
 part of these operators; it has no distillation.
@@ -49,9 +49,9 @@ def pretrain_head_distill_bf16(x, weight, teacher_logits, teacher_indices, *, te
 
     `teacher_logits` (fp32, fp16 or bf16) and `teacher_indices` (int32 or int64) are `[...,K]`, K up to 512, with x's
     leading shape.  An entry of -inf is absent, whatever its index; a row without any entry takes no part, as a row without
-    a label in `pretrain_head_cross_entropy_bf16`.  An index may occur more than once: each
-    occurrence is an entry of its own in p and in the sum, and in the gradient their shares add up.  An index outside
-    `[0,V)` makes its row's loss and the gradients NaN.  Differentiable in x and weight."""
+    a label in `pretrain_head_cross_entropy_bf16`.  An index may occur more than once: each occurrence is
+    an entry of its own in p and in the sum, and in the gradient their shares add up.  An index outside `[0,V)` makes its
+    row's loss and the gradients NaN.  Differentiable in x and weight."""
     code = _check(reduction, x=x, weight=weight, teacher_logits=teacher_logits, teacher_indices=teacher_indices)
     if not isinstance(temperature, (int, float)) or isinstance(temperature, bool):
         raise ValueError("temperature must be positive")
