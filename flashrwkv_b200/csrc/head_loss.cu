@@ -57,7 +57,9 @@ constexpr int kMaxTop = 512;
 // of 2048 x 65536 x 1024 to 4096 is off by 1e-7 of itself, without it by 6e-7.
 constexpr double kTruncation = 1.03e-9;
 constexpr int kFinishThreads = 256;
-constexpr int kFewRows = 64;  // copied by the plan: a launch less (2 us) while a warp has two rows at most
+// Copied by the plan, a launch less, while a warp has two rows at most: steps of 1 x 50277 x 1544 155 us so and 164 with the
+// launch, of 40 x 32000 x 768 61 and 62, but of 64 x 50277 x 1544 164 and 161.
+constexpr int kFewRows = 64;
 
 // Rows of labels that a warp each finishes rather than a CTA.  A step of 256 channels, by warps / by CTAs in us:
 //   vocabulary  300: 29 / 33 at 70 rows, 37 / 43 at 1000, 43 / 66 at 4000      (40 rows, which CTAs share: 26 / 30)
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(256) void teacher_rows_kernel(Labels labels, int* _
 // Copies the rows that take part together; the others get a zero loss and a zero gradient.  The rows behind the last, up
 // to the next multiple of 64, become zeros: they meet zeros of g in a block of the contraction over rows.  Where every row
 // takes part there is nothing to do, unless rows that are not whole 128-byte lines apart are copied to lines of their own
-// (`always`): TMA reads such rows a quarter slower (a step of 544 x 50277 x 1544 432 us on x as it is, 402 on the copy).
+// (`always`): TMA reads such rows more slowly (a step of 544 x 50277 x 1544 311 us on x as it is, 300 on the copy).
 struct CompactArgs {
   const uint4* x;
   const int* position;

@@ -82,8 +82,9 @@ int launch_gradients(const void* g, long long ldg, const void* x, const void* x_
                      bool add, int* error_flag, cudaStream_t stream);
 
 // Up to 128 rows one CTA works alone on a 128 x 256 tile: a pair's tile would be half empty, and the loads of W, which bound
-// the product then, would wait for twice the tensor-core time per byte (a step of 16 x 65536 x 1024 164 us by pairs, 152 alone; 128 x 65536 x 2048
-// 287 and 271 us).
+// the product then, would wait for twice the tensor-core time per byte.  Steps alone / by pairs in us: 16 x 65536 x 4096 345 /
+// 368, of x's gradient only 211 / 235; 128 x 65536 x 2048 232 / 239; 40 x 32000 x 768 62 / 67; 16 x 65536 x 1024 122 / 120 and
+// 128 x 50277 x 1544 174 / 172 are the ones where pairs were ahead.
 constexpr bool one_cta(long long rows) { return rows <= kTile / 2; }
 
 int pair_count();  // of CTAs that the current device runs at once
